@@ -143,6 +143,23 @@ int sia_paged_gqa_int8_flash_decode(const sia_tensor* q, const sia_tensor* k_poo
                                     void* workspace, size_t workspace_bytes,
                                     const sia_decode_options* opts, void* stream);
 
+/* Decode over 4-bit K/V (the format of sia_quantize_kv_int4); no counterpart
+ * in the reference.  Arguments, results and errors are those of the int8 entry
+ * points but for the cache: k_int4, v_int4 (B', Hkv, S, D / 2) or pools
+ * (num_pages, Hkv, page_size, D / 2) uint8, 16-byte aligned rows (8 at
+ * head_dim 16); k_scale, v_scale the same shape with a last dim of 2 D / g,
+ * f16, 4-byte aligned rows.  q f16|bf16|f32. */
+int sia_attention_flash_decode_int4(const sia_tensor* q, const sia_tensor* k_int4, const sia_tensor* v_int4,
+                                    const sia_tensor* k_scale, const sia_tensor* v_scale,
+                                    const sia_tensor* kv_len, float sm_scale, const sia_tensor* out,
+                                    void* workspace, size_t workspace_bytes, const sia_decode_options* opts,
+                                    void* stream);
+int sia_paged_gqa_int4_flash_decode(const sia_tensor* q, const sia_tensor* k_pool, const sia_tensor* v_pool,
+                                    const sia_tensor* k_scale_pool, const sia_tensor* v_scale_pool,
+                                    const sia_tensor* block_table, const sia_tensor* kv_len, int32_t page_size,
+                                    float sm_scale, const sia_tensor* out, void* workspace,
+                                    size_t workspace_bytes, const sia_decode_options* opts, void* stream);
+
 /* sia_paged_gqa_int8_flash_decode without a workspace argument: no
  * counterpart in the reference.  It is for callers that cannot allocate
  * device memory (code under HIP-graph capture, serving loops and harnesses
@@ -231,6 +248,27 @@ int sia_attention_flash_fwd_workspace_size(const sia_tensor* q, const sia_tensor
  * reference's KVCache dtype) or f32 (the paged pools' dtype). */
 int sia_quantize_kv_int8(const sia_tensor* x, const sia_tensor* out_int8, const sia_tensor* out_scale, void* stream);
 
+/* 4-bit K/V (no counterpart in the reference, whose smallest cache is int8).
+ * A row of D elements is held as D / 2 bytes of codes (SIA_U8) and 2 D / g
+ * fp16 parameters [s0, m0, s1, m1, ...], one step s and minimum m per group of
+ * g = 32, 64 or 128 consecutive elements, g <= D (at D = 16: 16).  Code n
+ * stands for m + n s:  lo, hi = the group's min and max clamped to +-65504,
+ * m = fp16(lo) to nearest, s = fp16(max(0, (hi - m) / 15)) towards zero,
+ * n = (x - m) / s to nearest (ties to even), 0 <= n <= 15, 0 where s = 0; the
+ * differences and quotients are rounded to fp32.  A group with a NaN or an
+ * infinity gets NaN for s and m and reads back as NaN.  Element 8 p + i is in
+ * bits 4 i .. 4 i + 3 of 32-bit word p, and word p of every block of b =
+ * min(D, 128) elements stands at place (p % 4) (b / 32) + p / 4 of the block
+ * (D = 16: in order), the order in which the attention kernels consume it.
+ *
+ * sia_quantize_kv_int4: x (..., D) f16|bf16|f32, 1..4 dims, head_dim
+ * contiguous, 16-byte aligned rows; codes (..., D / 2) uint8, 8-byte aligned
+ * rows; params (..., 2 D / g) f16, 4-byte aligned rows.
+ * sia_dequantize_kv_int4: the values back, out (..., D) f16|bf16|f32, each
+ * rounded once from the fp32 m + n s. */
+int sia_quantize_kv_int4(const sia_tensor* x, const sia_tensor* codes, const sia_tensor* params, void* stream);
+int sia_dequantize_kv_int4(const sia_tensor* codes, const sia_tensor* params, const sia_tensor* out, void* stream);
+
 /* Writes new K/V tokens into a cache.  Replaces the write half of
  * KVCache.update (model/kv_cache.py:133-184), the decode-step
  * quantize_kv_int8 + index_copy_ scatter (ops/attention.py:217-228),
@@ -250,11 +288,28 @@ int sia_quantize_kv_int8(const sia_tensor* x, const sia_tensor* out_int8, const 
  * Destination dtype f16|bf16|f32 (value cast) or int8 (quantised exactly as
  * sia_quantize_kv_int8, with the per-token-per-head scale written to
  * k_scale_dst / v_scale_dst, shaped like the destination without head_dim,
- * f16 or f32).  Positions outside the destination (p >= capacity, page id
+ * f16 or f32) or uint8 (int4: codes of head_dim / 2 bytes, the parameters of
+ * sia_quantize_kv_int4 written to k_scale_dst / v_scale_dst, shaped like the
+ * destination with a last dim of 2 D / g).  Positions outside the destination (p >= capacity, page id
  * outside the pool) are skipped on the device, never written. */
 int sia_kv_write(const sia_tensor* k, const sia_tensor* v, const sia_tensor* k_dst, const sia_tensor* v_dst,
                  const sia_tensor* k_scale_dst, const sia_tensor* v_scale_dst, const sia_tensor* block_table,
                  const sia_tensor* start_pos, int32_t start_pos_host, int32_t page_size, void* stream);
+
+/* Reads cached tokens back as plain tensors (no counterpart in the reference,
+ * whose int8 cache is read by the decode kernels only).
+ * k_src, v_src: a contiguous cache (B' >= B, H, S, D) or, with block_table, a
+ * pool (num_pages, H, page_size, D); f16|bf16|f32, int8 with k_scale / v_scale
+ * (f16|f32), or uint8 (int4) with parameters as k_scale / v_scale; one layout
+ * for both.  v_src and v_out may both be NULL.  k_out, v_out (B, H, T, D)
+ * f16|bf16|f32, any strides with 16-byte aligned rows, receive positions
+ * start_pos_host + start_pos[b] + t (start_pos as in sia_kv_write), each value
+ * rounded once to the output type.  Without start_pos every position must be
+ * inside the source (SIA_ERR_INVALID_ARGUMENT); a device position outside it,
+ * or a page id outside the pool, reads as zeros. */
+int sia_kv_read(const sia_tensor* k_src, const sia_tensor* v_src, const sia_tensor* k_scale, const sia_tensor* v_scale,
+                const sia_tensor* block_table, const sia_tensor* start_pos, int32_t start_pos_host, int32_t page_size,
+                const sia_tensor* k_out, const sia_tensor* v_out, void* stream);
 
 /* RoPE-K fused into the KV write, with q rotated in the same launch.
  * Replaces the captured decode step's apply_rope + quantize_kv_int8 + four

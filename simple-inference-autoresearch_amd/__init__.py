@@ -16,18 +16,34 @@ import torch  # noqa: F401  (load torch's HIP runtime before the library)
 from ._lib import LibraryMissing, SiaError, exported_symbols, library_path, load_library, require_library
 from .decode import (
     attention_flash_decode,
+    attention_flash_decode_int4,
     attention_flash_decode_int8,
     decode_options,
     decode_workspace_size,
     gqa_int8_flash_decode,
     paged_attention_flash_decode,
+    paged_gqa_int4_flash_decode,
     paged_gqa_int8_flash_decode,
 )
 from .prefill import attention_flash_triton, prefill_workspace_size, rope_attention_flash_triton
-from .kv_cache import KVCache, kv_write, quantize_kv_int8, rope_kv_write
+from .kv_cache import (
+    KVCache,
+    dequantize_kv_int4,
+    kv_read,
+    kv_write,
+    quantize_kv_int4,
+    quantize_kv_int8,
+    rope_kv_write,
+)
 from .paged_kv_cache import PagedKVCache
 from .rope import RopeFrequencies, apply_rope, rope_triton
-from .attention import DecodeCtx, decode_step_attention, gqa_attention, rope_decode_step_attention
+from .attention import (
+    DecodeCtx,
+    decode_step_attention,
+    gqa_attention,
+    prefill_step_attention,
+    rope_decode_step_attention,
+)
 from . import plugins  # noqa: F401  (cache builders, transformers attention hook)
 
 __all__ = [
@@ -42,13 +58,19 @@ __all__ = [
     "rope_triton",
     "decode_step_attention",
     "gqa_attention",
+    "kv_read",
     "kv_write",
+    "prefill_step_attention",
+    "quantize_kv_int4",
+    "dequantize_kv_int4",
     "quantize_kv_int8",
     "attention_flash_triton",
     "rope_attention_flash_triton",
     "SiaError",
     "attention_flash_decode",
+    "attention_flash_decode_int4",
     "attention_flash_decode_int8",
+    "paged_gqa_int4_flash_decode",
     "decode_options",
     "decode_workspace_size",
     "exported_symbols",

@@ -108,7 +108,14 @@ _SIGNATURES = {
     "sia_attention_flash_fwd_rope": [_P, _P, _P, _P, _P, _I32, _P, _I32, _I32, _F, _P, _VP, _SZ, _VP],
     "sia_attention_flash_fwd_workspace_size": [_P, _P, ctypes.POINTER(_SZ)],
     "sia_prefill_workspace_size": [_I64, _I64, _I64, _I64, ctypes.POINTER(_SZ)],
+    "sia_attention_flash_decode_int4": [_P, _P, _P, _P, _P, _P, _F, _P, _VP, _SZ,
+                                        ctypes.POINTER(DecodeOptions), _VP],
+    "sia_paged_gqa_int4_flash_decode": [_P, _P, _P, _P, _P, _P, _P, _I32, _F, _P, _VP, _SZ,
+                                        ctypes.POINTER(DecodeOptions), _VP],
     "sia_quantize_kv_int8": [_P, _P, _P, _VP],
+    "sia_quantize_kv_int4": [_P, _P, _P, _VP],
+    "sia_dequantize_kv_int4": [_P, _P, _P, _VP],
+    "sia_kv_read": [_P, _P, _P, _P, _P, _P, _I32, _I32, _P, _P, _VP],
     "sia_kv_write": [_P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _VP],
     "sia_rope_qk": [_P, _P, _P, _P, _I32, _P, _P, _VP],
     "sia_rope_kv_write": [_P, _P, _P, _P, _P, _I32, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _VP],

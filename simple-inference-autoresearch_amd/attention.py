@@ -11,11 +11,15 @@ those lines, so a caller keeps its own projections and RoPE:
   ``(B, T, Hq * D)``.
 * :func:`decode_step_attention` -- the cache write and attention of the
   captured decode step (``ops/attention.py:206-231``) over a contiguous
-  :class:`~.kv_cache.KVCache`: int8 caches quantise the new token on the way
-  in, and the position and length are read on the device from ``ctx``.
+  :class:`~.kv_cache.KVCache`: int8 and 4-bit caches quantise the new token on
+  the way in, and the position and length are read on the device from ``ctx``.
 * :func:`rope_decode_step_attention` -- the same step from the pre-RoPE
   projections (``ops/attention.py:202-231``): RoPE of q and k fused into the
   cache write, then attention.
+* :func:`prefill_step_attention` -- the cache write and attention of one chunk
+  of a prompt behind a cached prefix, whatever the cache holds (the reference's
+  int8 cache returns the chunk alone, ``model/kv_cache.py:133-184``, so that it
+  never sees its prefix).
 * :class:`DecodeCtx` -- the device buffers of ``model/cuda_graph_decode.py:53-56``
   (``cos``, ``sin``, ``pos_index``, ``kv_len``), with int32 positions and
   :meth:`DecodeCtx.set_position` for the per-step update
@@ -26,8 +30,8 @@ from __future__ import annotations
 
 import torch
 
-from .decode import (CONTIG, CONTIG_INT8, _common, _kv_len_tensor, _run_layer, attention_flash_decode,
-                     attention_flash_decode_int8)
+from .decode import (CONTIG, CONTIG_INT4, CONTIG_INT8, _common, _kv_len_tensor, _run_layer, attention_flash_decode,
+                     attention_flash_decode_int4, attention_flash_decode_int8)
 from .kv_cache import KVCache
 from .prefill import attention_flash_triton
 
@@ -43,6 +47,26 @@ def gqa_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: boo
         causal = T > 1
     out = attention_flash_triton(q, k, v, causal=causal, assume_contiguous=True, out_token_major=True)
     return out.view(B, T, Hq * D)
+
+
+def prefill_step_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache: KVCache, layer_idx: int,
+                           start_pos: int) -> torch.Tensor:
+    """Write a chunk of a prompt and attend to it and to its cached prefix, causally.
+
+    ``q (B, Hq, T, D)``, ``k, v (B, Hkv, T, D)`` after RoPE, for positions
+    ``[start_pos, start_pos + T)``; returns ``(B, T, Hq * D)``.  The chunk's own
+    K/V enter as they are, as in :meth:`KVCache.update`'s contract for a
+    quantised cache; its prefix as the cache holds it, read back
+    (:meth:`KVCache.read`).
+    """
+    kc, vc = kv_cache.update(layer_idx, start_pos, k, v)
+    if start_pos and kv_cache.is_quantized:
+        B, H, T, D = k.shape
+        kc, vc = (torch.empty(B, H, start_pos + T, D, dtype=k.dtype, device=k.device) for _ in range(2))
+        kv_cache.read(layer_idx, B, start_pos, out=(kc[:, :, :start_pos], vc[:, :, :start_pos]))
+        kc[:, :, start_pos:].copy_(k)
+        vc[:, :, start_pos:].copy_(v)
+    return gqa_attention(q, kc, vc, causal=True)
 
 
 class DecodeCtx:
@@ -84,8 +108,8 @@ def rope_decode_step_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
     qh = q_rot.transpose(1, 2)
     scale = _common(qh, kv_cache.k_cache, sm_scale)
     kl = _kv_len_tensor(ctx.kv_len, qh.device)
-    ks, vs = (kv_cache.k_scale, kv_cache.v_scale) if kv_cache.is_int8 else (None, None)
-    return _run_layer(CONTIG_INT8 if kv_cache.is_int8 else CONTIG, qh, kv_cache.k_cache, kv_cache.v_cache, ks, vs,
+    kind = CONTIG_INT4 if kv_cache.is_int4 else CONTIG_INT8 if kv_cache.is_int8 else CONTIG
+    return _run_layer(kind, qh, kv_cache.k_cache, kv_cache.v_cache, kv_cache.k_scale, kv_cache.v_scale,
                       layer_idx, None, kl, 0, scale)
 
 
@@ -94,13 +118,15 @@ def decode_step_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_
     """Write this step's K/V and attend: ``q (B, Hq, 1, D)``, ``k, v (B, Hkv, 1, D)`` -> ``(B, 1, Hq, D)``.
 
     Replaces ``ops/attention.py:210-231``: the token is written at
-    ``ctx.pos_index`` (quantised for an int8 cache) and attention covers the
+    ``ctx.pos_index`` (quantised for an int8 or 4-bit cache) and attention covers the
     first ``ctx.kv_len`` cached positions.  Graph safe: every length and
     position is read on the device.
     """
     B = q.shape[0]
     kv_cache.write_decode(layer_idx, ctx.pos_index, k, v)
     kc, vc, ks, vs = kv_cache._layer(layer_idx, B)
+    if kv_cache.is_int4:
+        return attention_flash_decode_int4(q, kc, vc, ks, vs, ctx.kv_len, sm_scale)
     if kv_cache.is_int8:
         return attention_flash_decode_int8(q, kc, vc, ks, vs, ctx.kv_len, sm_scale)
     return attention_flash_decode(q, kc, vc, ctx.kv_len, sm_scale)

@@ -1,6 +1,7 @@
 // Float32 attention kernels (layout and semantics: attn_f32.hpp).
 #include "attn_f32.hpp"
 #include "host_util.hpp"
+#include "int4.hpp"
 
 namespace sia {
 
@@ -26,6 +27,13 @@ __device__ __forceinline__ f32x4 load4<I8>(const char* p) {
   const uint32_t w = __builtin_nontemporal_load((const uint32_t*)p);
   return f32x4{(float)(int8_t)(w & 0xffu), (float)(int8_t)((w >> 8) & 0xffu), (float)(int8_t)((w >> 16) & 0xffu),
                (float)(int8_t)(w >> 24)};
+}
+
+// Four elements of a 4-bit row: the half word of codes at p, the group's parameters at sm.
+__device__ __forceinline__ f32x4 load4_i4(const char* p, const char* sm) {
+  const uint32_t w = *(const uint16_t*)p, x = *(const uint32_t*)sm;
+  const float s = lo_f32(F16{}, x), m = hi_f32(F16{}, x);
+  return f32x4{i4_value(w, 0, s, m), i4_value(w, 1, s, m), i4_value(w, 2, s, m), i4_value(w, 3, s, m)};
 }
 
 template <class T>
@@ -93,6 +101,7 @@ __global__ __launch_bounds__(256) void attn_f32(const F32Args a) {
   constexpr int C = kF32Cols;
   constexpr int STEP = 4 * TPW * U;     // keys per work-group step
   constexpr bool kInt8 = std::is_same<KV, I8>::value;
+  constexpr bool kInt4 = std::is_same<KV, I4>::value;
   __shared__ __attribute__((aligned(16))) float sm[4][C][D + 4];
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -130,13 +139,18 @@ __global__ __launch_bounds__(256) void attn_f32(const F32Args a) {
   }
   const bool paged = a.bt != nullptr;
   const int64_t seq_k = paged ? 0 : (int64_t)b * a.k_s0, seq_v = paged ? 0 : (int64_t)b * a.v_s0;
-  const char* kb = a.k + seq_k + (int64_t)hkv * a.k_sh + j4 * 4 * KV::bytes;
-  const char* vb = a.v + seq_v + (int64_t)hkv * a.v_sh + j4 * 4 * KV::bytes;
+  // byte of the lane's 4 elements in a row: half a word of codes for int4
+  int at;
+  if constexpr (kInt4) at = 4 * i4_place(j4 >> 1, D) + 2 * (j4 & 1);
+  else at = j4 * 4 * KV::bytes;
+  const char* kb = a.k + seq_k + (int64_t)hkv * a.k_sh + at;
+  const char* vb = a.v + seq_v + (int64_t)hkv * a.v_sh + at;
   const char* ksb = nullptr;
   const char* vsb = nullptr;
-  if constexpr (kInt8) {
-    ksb = a.ks + (paged ? 0 : (int64_t)b * a.ks_s0) + (int64_t)hkv * a.ks_sh;
-    vsb = a.vs + (paged ? 0 : (int64_t)b * a.vs_s0) + (int64_t)hkv * a.vs_sh;
+  if constexpr (kInt8 || kInt4) {
+    const int par = kInt4 ? 4 * ((4 * j4) >> a.lg_group) : 0;      // int4: the lane's group
+    ksb = a.ks + (paged ? 0 : (int64_t)b * a.ks_s0) + (int64_t)hkv * a.ks_sh + par;
+    vsb = a.vs + (paged ? 0 : (int64_t)b * a.vs_s0) + (int64_t)hkv * a.vs_sh + par;
   }
   const int32_t* btrow = paged ? a.bt + (int64_t)b * a.bt_sb : nullptr;
 
@@ -156,8 +170,14 @@ __global__ __launch_bounds__(256) void attn_f32(const F32Args a) {
         page = (unsigned)pg < (unsigned long long)a.num_pages ? pg : 0;   // never read outside the pool
         pos = tc - (tc / a.page_size) * a.page_size;
       }
-      kk[u] = load4<KV>(kb + page * a.k_s0 + (int64_t)pos * a.k_sn);
-      vv[u] = load4<KV>(vb + page * a.v_s0 + (int64_t)pos * a.v_sn);
+      if constexpr (kInt4) {
+        // (values, not scaled codes: one rounding each, as they read back)
+        kk[u] = load4_i4(kb + page * a.k_s0 + (int64_t)pos * a.k_sn, ksb + page * a.ks_s0 + (int64_t)pos * a.ks_sn);
+        vv[u] = load4_i4(vb + page * a.v_s0 + (int64_t)pos * a.v_sn, vsb + page * a.vs_s0 + (int64_t)pos * a.vs_sn);
+      } else {
+        kk[u] = load4<KV>(kb + page * a.k_s0 + (int64_t)pos * a.k_sn);
+        vv[u] = load4<KV>(vb + page * a.v_s0 + (int64_t)pos * a.v_sn);
+      }
       if constexpr (kInt8) {
         ksc[u] = scale_at<ST>(ksb + page * a.ks_s0 + (int64_t)pos * a.ks_sn);
         vsc[u] = scale_at<ST>(vsb + page * a.vs_s0 + (int64_t)pos * a.vs_sn);
@@ -372,6 +392,14 @@ int launch_attn_merge(const F32Args& a, int D, int out_dtype, hipStream_t stream
 }
 
 int launch_attn_f32(F32Launch& L) {
+  if (L.kv_dtype == SIA_U8) {   // int4, any q type
+    switch (L.q_dtype) {
+      case SIA_F32: return launch_f32_d<F32, I4, F16>(L);
+      case SIA_F16: return launch_f32_d<F16, I4, F16>(L);
+      case SIA_BF16: return launch_f32_d<BF16, I4, F16>(L);
+      default: break;
+    }
+  }
   if (L.q_dtype == SIA_F32) {
     switch (L.kv_dtype) {
       case SIA_F32: return launch_f32_d<F32, F32, F32>(L);

@@ -7,6 +7,7 @@
 #include "attn_f32.hpp"
 #include "decode_launch.hpp"
 #include "host_util.hpp"
+#include "int4.hpp"
 
 namespace sia {
 const char* last_message();
@@ -141,15 +142,18 @@ int prepare_kv(const sia_tensor* k, const sia_tensor* v, const Geometry& g, bool
   if (k->dtype != v->dtype) return fail(SIA_ERR_INVALID_ARGUMENT, "k and v dtypes differ");
   for (int d = 0; d < 4; ++d)
     if (k->shape[d] != v->shape[d]) return fail(SIA_ERR_INVALID_ARGUMENT, "k and v shapes differ");
-  if (k->shape[1] != g.Hkv || k->shape[3] != g.D)
-    return fail(SIA_ERR_INVALID_ARGUMENT, "k/v must be (*, Hkv=%d, *, D=%d)", g.Hkv, g.D);
+  const bool int4 = k->dtype == SIA_U8;
+  const int64_t row = int4 ? i4_code_bytes(g.D) : g.D;
+  if (k->shape[1] != g.Hkv || k->shape[3] != row)
+    return fail(SIA_ERR_INVALID_ARGUMENT, "k/v must be (*, Hkv=%d, *, %lld)", g.Hkv, (long long)row);
   if (k->stride[3] != 1 || v->stride[3] != 1)
     return fail(SIA_ERR_INVALID_ARGUMENT, "k/v must be contiguous along head_dim");
   if (!aligned16(k->data) || !aligned16(v->data))
     return fail(SIA_ERR_INVALID_ARGUMENT, "k/v base pointers must be 16-byte aligned");
+  const int align = int4 && row < 16 ? 8 : 16;   // (int4 at head_dim 16: rows of 8 bytes)
   for (int d = 0; d < 3; ++d)
-    if (bstride(k, d) % 16 || bstride(v, d) % 16)
-      return fail(SIA_ERR_INVALID_ARGUMENT, "k/v strides must be multiples of 16 bytes");
+    if (bstride(k, d) % align || bstride(v, d) % align)
+      return fail(SIA_ERR_INVALID_ARGUMENT, "k/v strides must be multiples of %d bytes", align);
   DecodeArgs& a = L.a;
   a.k = (const char*)k->data; a.k_s0 = bstride(k, 0); a.k_sh = bstride(k, 1); a.k_sn = bstride(k, 2);
   a.v = (const char*)v->data; a.v_s0 = bstride(v, 0); a.v_sh = bstride(v, 1); a.v_sn = bstride(v, 2);
@@ -204,6 +208,27 @@ int prepare_scales(const sia_tensor* ks, const sia_tensor* vs, const sia_tensor*
   a.scale_vec = ks->stride[2] == 1 && vs->stride[2] == 1 && (uintptr_t)ks->data % al == 0 &&
                 (uintptr_t)vs->data % al == 0 && bstride(ks, 0) % al == 0 && bstride(ks, 1) % al == 0 &&
                 bstride(vs, 0) % al == 0 && bstride(vs, 1) % al == 0;
+  return SIA_OK;
+}
+
+// int4: fp16 steps and minima (*, Hkv, *, 2 D / g) of k and v.
+int prepare_i4_params(const sia_tensor* ks, const sia_tensor* vs, const sia_tensor* k, const Geometry& g, bool paged,
+                      DecodeLaunch& L) {
+  int rc, lgv = 0;
+  if ((rc = check_i4_params(ks, k, g.D, "k_scale", &L.lg_group))) return rc;
+  if ((rc = check_i4_params(vs, k, g.D, "v_scale", &lgv))) return rc;
+  if (lgv != L.lg_group) return fail(SIA_ERR_INVALID_ARGUMENT, "k_scale and v_scale have different group sizes");
+  DecodeArgs& a = L.a;
+  a.ks = (const char*)ks->data; a.ks_s0 = bstride(ks, 0); a.ks_sh = bstride(ks, 1); a.ks_sn = bstride(ks, 2);
+  a.vs = (const char*)vs->data; a.vs_s0 = bstride(vs, 0); a.vs_sh = bstride(vs, 1); a.vs_sn = bstride(vs, 2);
+  if (a.ks_sn > 0x7fffffff || a.vs_sn > 0x7fffffff)
+    return fail(SIA_ERR_UNSUPPORTED, "k_scale/v_scale token stride too large");
+  a.ks_tok = (uint32_t)a.ks_sn; a.vs_tok = (uint32_t)a.vs_sn;
+  if (paged) {
+    if (a.ks_s0 > 0xffffffffLL || a.vs_s0 > 0xffffffffLL)
+      return fail(SIA_ERR_UNSUPPORTED, "k_scale/v_scale page stride too large");
+    a.ks_pg = (uint32_t)a.ks_s0; a.vs_pg = (uint32_t)a.vs_s0;
+  }
   return SIA_OK;
 }
 
@@ -274,6 +299,7 @@ int dispatch_f32(const DecodeLaunch& D, const Geometry& g, int kv_dtype, const s
   a.ncol = g.G;
   a.nchunk = (g.G + kF32Cols - 1) / kF32Cols;
   a.qk_scale = d.qk_scale;
+  a.lg_group = D.lg_group;
   // split: enough items for four per CU, pieces of >= 64 keys (one step of a
   // work-group at head_dim 64; longer ones leave small calls to a few
   // work-groups: with 128, 512 tokens at 8 KV heads ran on 32), within the
@@ -331,7 +357,7 @@ int dispatch(DecodeLaunch& L, int kv_dtype) {
 int decode_any(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, const sia_tensor* ks,
                const sia_tensor* vs, const sia_tensor* bt, const sia_tensor* kv_len, int page_size,
                float sm_scale, const sia_tensor* out, void* ws, size_t ws_bytes,
-               const sia_decode_options* opts, void* stream, bool want_int8) {
+               const sia_decode_options* opts, void* stream, int want) {   // want: SIA_I8, SIA_U8 (int4) or 0
   DecodeLaunch L;
   memset(&L, 0, sizeof(L));
   Geometry g;
@@ -342,7 +368,11 @@ int decode_any(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, co
   L.a.IU = g.IU;
   L.a.UB = g.UB;
   if ((rc = prepare_kv(k, v, g, bt != nullptr, page_size, L))) return rc;
-  if (want_int8) {
+  if (want == SIA_U8) {
+    if (k->dtype != SIA_U8)
+      return fail(SIA_ERR_INVALID_ARGUMENT, "k/v must be uint8 (two codes a byte) for the int4 entry points");
+    if ((rc = prepare_i4_params(ks, vs, k, g, bt != nullptr, L))) return rc;
+  } else if (want == SIA_I8) {
     if (k->dtype != SIA_I8) return fail(SIA_ERR_INVALID_ARGUMENT, "k/v must be int8 for the int8 entry points");
     if ((rc = prepare_scales(ks, vs, k, bt != nullptr, L))) return rc;
   } else if (k->dtype != SIA_F16 && k->dtype != SIA_BF16 && k->dtype != SIA_F32) {
@@ -357,6 +387,7 @@ int decode_any(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, co
   // pages that do not hold whole 16-token tiles (page sizes 1-8, or any size
   // other than 16 * 2^k) go to the vector-ALU path with its per-token lookup
   const bool tiled_pages = bt == nullptr || (kTile << L.a.lg_tiles_per_page) == page_size;
+  if (k->dtype == SIA_U8) return dispatch_f32(L, g, k->dtype, out);
   if (q->dtype == SIA_F32 || k->dtype == SIA_F32 || !tiled_pages) return dispatch_f32(L, g, k->dtype, out);
   return dispatch(L, k->dtype);
 }
@@ -425,7 +456,7 @@ int sia_attention_flash_decode(const sia_tensor* q, const sia_tensor* k, const s
                                void* workspace, size_t workspace_bytes, const sia_decode_options* opts,
                                void* stream) {
   return decode_any(q, k, v, nullptr, nullptr, nullptr, kv_len, 0, sm_scale, out, workspace,
-                    workspace_bytes, opts, stream, false);
+                    workspace_bytes, opts, stream, 0);
 }
 
 int sia_attention_flash_decode_int8(const sia_tensor* q, const sia_tensor* k_int8, const sia_tensor* v_int8,
@@ -434,7 +465,7 @@ int sia_attention_flash_decode_int8(const sia_tensor* q, const sia_tensor* k_int
                                     void* workspace, size_t workspace_bytes, const sia_decode_options* opts,
                                     void* stream) {
   return decode_any(q, k_int8, v_int8, k_scale, v_scale, nullptr, kv_len, 0, sm_scale, out, workspace,
-                    workspace_bytes, opts, stream, true);
+                    workspace_bytes, opts, stream, SIA_I8);
 }
 
 int sia_gqa_int8_flash_decode(const sia_tensor* q, const sia_tensor* k_int8, const sia_tensor* v_int8,
@@ -442,7 +473,7 @@ int sia_gqa_int8_flash_decode(const sia_tensor* q, const sia_tensor* k_int8, con
                               float sm_scale, const sia_tensor* out, void* workspace, size_t workspace_bytes,
                               const sia_decode_options* opts, void* stream) {
   return decode_any(q, k_int8, v_int8, k_scale, v_scale, nullptr, kv_len, 0, sm_scale, out, workspace,
-                    workspace_bytes, opts, stream, true);
+                    workspace_bytes, opts, stream, SIA_I8);
 }
 
 int sia_paged_attention_flash_decode(const sia_tensor* q, const sia_tensor* k_pool, const sia_tensor* v_pool,
@@ -451,7 +482,7 @@ int sia_paged_attention_flash_decode(const sia_tensor* q, const sia_tensor* k_po
                                      size_t workspace_bytes, const sia_decode_options* opts, void* stream) {
   if (block_table == nullptr) return fail(SIA_ERR_INVALID_ARGUMENT, "block_table is NULL");
   return decode_any(q, k_pool, v_pool, nullptr, nullptr, block_table, kv_len, page_size, sm_scale, out,
-                    workspace, workspace_bytes, opts, stream, false);
+                    workspace, workspace_bytes, opts, stream, 0);
 }
 
 int sia_paged_gqa_int8_flash_decode_noalloc(const sia_tensor* q, const sia_tensor* k_pool, const sia_tensor* v_pool,
@@ -478,7 +509,7 @@ int sia_paged_gqa_int8_flash_decode_noalloc(const sia_tensor* q, const sia_tenso
   // nothing in the scratch needs to start at zero: every call writes the plan
   // and each partial slot before reading it
   return decode_any(q, k_pool, v_pool, k_scale_pool, v_scale_pool, block_table, kv_len, page_size, sm_scale, out,
-                    ws, kScratchBytes, opts, stream, true);
+                    ws, kScratchBytes, opts, stream, SIA_I8);
 }
 
 int sia_paged_gqa_int8_flash_decode(const sia_tensor* q, const sia_tensor* k_pool, const sia_tensor* v_pool,
@@ -488,7 +519,26 @@ int sia_paged_gqa_int8_flash_decode(const sia_tensor* q, const sia_tensor* k_poo
                                     size_t workspace_bytes, const sia_decode_options* opts, void* stream) {
   if (block_table == nullptr) return fail(SIA_ERR_INVALID_ARGUMENT, "block_table is NULL");
   return decode_any(q, k_pool, v_pool, k_scale_pool, v_scale_pool, block_table, kv_len, page_size, sm_scale,
-                    out, workspace, workspace_bytes, opts, stream, true);
+                    out, workspace, workspace_bytes, opts, stream, SIA_I8);
+}
+
+int sia_attention_flash_decode_int4(const sia_tensor* q, const sia_tensor* k_int4, const sia_tensor* v_int4,
+                                    const sia_tensor* k_scale, const sia_tensor* v_scale,
+                                    const sia_tensor* kv_len, float sm_scale, const sia_tensor* out,
+                                    void* workspace, size_t workspace_bytes, const sia_decode_options* opts,
+                                    void* stream) {
+  return decode_any(q, k_int4, v_int4, k_scale, v_scale, nullptr, kv_len, 0, sm_scale, out, workspace,
+                    workspace_bytes, opts, stream, SIA_U8);
+}
+
+int sia_paged_gqa_int4_flash_decode(const sia_tensor* q, const sia_tensor* k_pool, const sia_tensor* v_pool,
+                                    const sia_tensor* k_scale_pool, const sia_tensor* v_scale_pool,
+                                    const sia_tensor* block_table, const sia_tensor* kv_len, int32_t page_size,
+                                    float sm_scale, const sia_tensor* out, void* workspace,
+                                    size_t workspace_bytes, const sia_decode_options* opts, void* stream) {
+  if (block_table == nullptr) return fail(SIA_ERR_INVALID_ARGUMENT, "block_table is NULL");
+  return decode_any(q, k_pool, v_pool, k_scale_pool, v_scale_pool, block_table, kv_len, page_size, sm_scale,
+                    out, workspace, workspace_bytes, opts, stream, SIA_U8);
 }
 
 }  // extern "C"

@@ -1,8 +1,9 @@
-// extern "C" KV write-path entry points: validation and dispatch of kv_write.hip.
+// extern "C" entry points of KV writes and reads: validation and dispatch of kv_write.hip and kv_read.hip.
 #include <math.h>
 #include <string.h>
 
 #include "host_util.hpp"
+#include "int4.hpp"
 #include "kv_write.hpp"
 
 using namespace sia;
@@ -51,6 +52,51 @@ int check_scale(const sia_tensor* s, const sia_tensor* like, const char* name) {
   return SIA_OK;
 }
 
+bool head_dim_ok(int64_t D) { return D == 16 || D == 32 || D == 64 || D == 128 || D == 256; }
+
+// k and v descriptors that are read or written through one set of strides.
+int check_alike(const sia_tensor* k, const sia_tensor* v, const char* kn, const char* vn) {
+  if (v->dtype != k->dtype || v->ndim != k->ndim)
+    return fail(SIA_ERR_INVALID_ARGUMENT, "%s and %s must have one dtype and rank", kn, vn);
+  for (int d = 0; d < k->ndim; ++d)
+    if (v->shape[d] != k->shape[d] || v->stride[d] != k->stride[d])
+      return fail(SIA_ERR_INVALID_ARGUMENT, "%s and %s must have the same shape and strides", kn, vn);
+  return SIA_OK;
+}
+
+// start_pos (int32, 1 or B elements, on the device) into a.start.
+template <class A>
+int fill_start(const sia_tensor* start_pos, int64_t B, A& a) {
+  if (start_pos->data == nullptr || start_pos->dtype != SIA_I32 || start_pos->ndim > 1)
+    return fail(SIA_ERR_INVALID_ARGUMENT, "start_pos must be an int32 scalar, (1,) or (B,) tensor");
+  const int64_t n = start_pos->ndim == 0 ? 1 : start_pos->shape[0];
+  if (n != 1 && n != B) return fail(SIA_ERR_INVALID_ARGUMENT, "start_pos must have 1 or B elements");
+  if (n == B && B > 1 && start_pos->stride[0] != 1)
+    return fail(SIA_ERR_INVALID_ARGUMENT, "start_pos must be contiguous");
+  a.start = (const int32_t*)start_pos->data;
+  a.start_per_seq = (n == B && B > 1) ? 1 : 0;
+  return SIA_OK;
+}
+
+// block_table (B, max_blocks) int32 over a pool `t` (num_pages, H, page_size, *), into a's page fields.
+template <class A>
+int fill_table(const sia_tensor* block_table, const sia_tensor* t, int64_t B, int32_t page_size, A& a) {
+  if (block_table->data == nullptr || block_table->ndim != 2 || block_table->dtype != SIA_I32)
+    return fail(SIA_ERR_INVALID_ARGUMENT, "block_table must be a (B, max_blocks) int32 tensor");
+  if (block_table->shape[0] < B) return fail(SIA_ERR_INVALID_ARGUMENT, "block_table has fewer rows than the batch");
+  if (page_size <= 0 || t->shape[2] != page_size)
+    return fail(SIA_ERR_INVALID_ARGUMENT, "pool page dim %lld != page_size %d", (long long)t->shape[2], page_size);
+  const int64_t cap = block_table->shape[1] * (int64_t)page_size;
+  if (cap > 0x7fffffff) return fail(SIA_ERR_UNSUPPORTED, "block table capacity too large");
+  a.bt = (const int32_t*)block_table->data;
+  a.bt_sb = block_table->stride[0];
+  a.bt_sl = block_table->stride[1];
+  a.num_pages = t->shape[0];
+  a.page = page_size;
+  a.cap = (int32_t)cap;
+  return SIA_OK;
+}
+
 // Validates a KV write of k/v (B, H, T, D) and fills `a` (everything but the
 // RoPE fields); *dst_dtype receives the destination dtype.
 int setup_kv_write(const sia_tensor* k, const sia_tensor* v, const sia_tensor* k_dst, const sia_tensor* v_dst,
@@ -71,12 +117,12 @@ int setup_kv_write(const sia_tensor* k, const sia_tensor* v, const sia_tensor* k
       return fail(SIA_ERR_INVALID_ARGUMENT, "k and v must have the same strides");
   }
   const int64_t B = k->shape[0], H = k->shape[1], T = k->shape[2], D = k->shape[3];
-  if (D != 64 && D != 128 && D != 256 && D != 16 && D != 32)
+  if (!head_dim_ok(D))
     return fail(SIA_ERR_UNSUPPORTED, "head_dim %lld not supported (16, 32, 64, 128, 256)", (long long)D);
   if (k_dst == nullptr || k_dst->data == nullptr) return fail(SIA_ERR_INVALID_ARGUMENT, "k_dst is missing");
   const int dd = k_dst->dtype;
-  const bool int8 = dd == SIA_I8;
-  const int align = int8 ? 8 : 16;
+  const bool int8 = dd == SIA_I8, int4 = dd == SIA_U8;
+  const int align = int8 || int4 ? 8 : 16;
   if ((rc = check_rows(k_dst, "k_dst", align))) return rc;
   if (two) {
     if ((rc = check_rows(v_dst, "v_dst", align))) return rc;
@@ -87,9 +133,19 @@ int setup_kv_write(const sia_tensor* k, const sia_tensor* v, const sia_tensor* k
         bstride(v_dst, 2) != bstride(k_dst, 2))
       return fail(SIA_ERR_INVALID_ARGUMENT, "k_dst and v_dst must have the same strides");
   }
-  if (k_dst->shape[1] != H || k_dst->shape[3] != D)
-    return fail(SIA_ERR_INVALID_ARGUMENT, "destination must be (*, %lld, *, %lld)", (long long)H, (long long)D);
-  if (int8) {
+  const int64_t row = int4 ? i4_code_bytes(D) : D;
+  if (k_dst->shape[1] != H || k_dst->shape[3] != row)
+    return fail(SIA_ERR_INVALID_ARGUMENT, "destination must be (*, %lld, *, %lld)", (long long)H, (long long)row);
+  int lg_group = 0;
+  if (int4) {
+    if ((rc = check_i4_params(k_scale_dst, k_dst, D, "k_scale_dst", &lg_group))) return rc;
+    if (two) {
+      if (v_scale_dst == nullptr) return fail(SIA_ERR_INVALID_ARGUMENT, "v_scale_dst is required for an int4 destination");
+      if ((rc = check_alike(k_scale_dst, v_scale_dst, "k_scale_dst", "v_scale_dst")) ||
+          (rc = check_i4_params(v_scale_dst, k_dst, D, "v_scale_dst", &lg_group)))
+        return rc;
+    }
+  } else if (int8) {
     if ((rc = check_scale(k_scale_dst, k_dst, "k_scale_dst"))) return rc;
     if (two) {
       if ((rc = check_scale(v_scale_dst, k_dst, "v_scale_dst"))) return rc;
@@ -103,19 +159,7 @@ int setup_kv_write(const sia_tensor* k, const sia_tensor* v, const sia_tensor* k
 
   memset(&a, 0, sizeof(a));
   if (block_table != nullptr) {
-    if (block_table->data == nullptr || block_table->ndim != 2 || block_table->dtype != SIA_I32)
-      return fail(SIA_ERR_INVALID_ARGUMENT, "block_table must be a (B, max_blocks) int32 tensor");
-    if (block_table->shape[0] < B) return fail(SIA_ERR_INVALID_ARGUMENT, "block_table has fewer rows than the batch");
-    if (page_size <= 0 || k_dst->shape[2] != page_size)
-      return fail(SIA_ERR_INVALID_ARGUMENT, "pool page dim %lld != page_size %d", (long long)k_dst->shape[2], page_size);
-    const int64_t cap = block_table->shape[1] * (int64_t)page_size;
-    if (cap > 0x7fffffff) return fail(SIA_ERR_UNSUPPORTED, "block table capacity too large");
-    a.bt = (const int32_t*)block_table->data;
-    a.bt_sb = block_table->stride[0];
-    a.bt_sl = block_table->stride[1];
-    a.num_pages = k_dst->shape[0];
-    a.page = page_size;
-    a.cap = (int32_t)cap;
+    if ((rc = fill_table(block_table, k_dst, B, page_size, a))) return rc;
   } else {
     if (k_dst->shape[0] < B) return fail(SIA_ERR_INVALID_ARGUMENT, "cache batch dim smaller than the batch");
     if (k_dst->shape[2] > 0x7fffffff) return fail(SIA_ERR_UNSUPPORTED, "cache length too large");
@@ -123,14 +167,7 @@ int setup_kv_write(const sia_tensor* k, const sia_tensor* v, const sia_tensor* k
     a.page = 1;
   }
   if (start_pos != nullptr) {
-    if (start_pos->data == nullptr || start_pos->dtype != SIA_I32 || start_pos->ndim > 1)
-      return fail(SIA_ERR_INVALID_ARGUMENT, "start_pos must be an int32 scalar, (1,) or (B,) tensor");
-    const int64_t n = start_pos->ndim == 0 ? 1 : start_pos->shape[0];
-    if (n != 1 && n != B) return fail(SIA_ERR_INVALID_ARGUMENT, "start_pos must have 1 or B elements");
-    if (n == B && B > 1 && start_pos->stride[0] != 1)
-      return fail(SIA_ERR_INVALID_ARGUMENT, "start_pos must be contiguous");
-    a.start = (const int32_t*)start_pos->data;
-    a.start_per_seq = (n == B && B > 1) ? 1 : 0;
+    if ((rc = fill_start(start_pos, B, a))) return rc;
     a.start_host = start_pos_host;   // added to the device value
   } else {
     a.start_host = start_pos_host;
@@ -148,7 +185,7 @@ int setup_kv_write(const sia_tensor* k, const sia_tensor* v, const sia_tensor* k
   a.dst0 = (char*)k_dst->data;
   a.dst1 = two ? (char*)v_dst->data : nullptr;
   a.d_s0 = bstride(k_dst, 0); a.d_sh = bstride(k_dst, 1); a.d_sn = bstride(k_dst, 2);
-  if (int8) {
+  if (int8 || int4) {
     a.sc0 = (char*)k_scale_dst->data;
     a.sc1 = two ? (char*)v_scale_dst->data : nullptr;
     a.c_s0 = bstride(k_scale_dst, 0); a.c_sh = bstride(k_scale_dst, 1); a.c_sn = bstride(k_scale_dst, 2);
@@ -158,6 +195,7 @@ int setup_kv_write(const sia_tensor* k, const sia_tensor* v, const sia_tensor* k
   a.rows = B * H * T;
   a.ntensors = two ? 2 : 1;
   a.amax_floor = amax_floor(k->dtype);
+  a.lg_group = lg_group;
   *dst_dtype = dd;
   return SIA_OK;
 }
@@ -168,6 +206,35 @@ sia_tensor token_major_as_head_major(const sia_tensor* x) {
   y.shape[1] = x->shape[2]; y.stride[1] = x->stride[2];
   y.shape[2] = x->shape[1]; y.stride[2] = x->stride[1];
   return y;
+}
+
+// `t` with dims of size 1 put in front, up to `ndim` of them.
+sia_tensor lead_to(const sia_tensor& t, int ndim) {
+  sia_tensor y;
+  memset(&y, 0, sizeof(y));
+  y.data = t.data;
+  y.dtype = t.dtype;
+  y.ndim = ndim;
+  const int pad = ndim - t.ndim;
+  for (int d = 0; d < ndim; ++d) {
+    y.shape[d] = d < pad ? 1 : t.shape[d - pad];
+    y.stride[d] = d < pad ? 0 : t.stride[d - pad];
+  }
+  return y;
+}
+
+// The three tensors of an int4 (de)quantisation: x (..., D), codes (..., D / 2), params (..., 2 D / g).
+int check_i4_triple(const sia_tensor* x, const sia_tensor* codes, const sia_tensor* params, const char* xn) {
+  if (x == nullptr || codes == nullptr || params == nullptr)
+    return fail(SIA_ERR_INVALID_ARGUMENT, "%s, codes and params are required", xn);
+  if (x->ndim < 1 || x->ndim > 4) return fail(SIA_ERR_UNSUPPORTED, "%s must have 1 to 4 dims", xn);
+  if (codes->ndim != x->ndim || params->ndim != x->ndim)
+    return fail(SIA_ERR_INVALID_ARGUMENT, "codes and params must have the dims of %s", xn);
+  if (codes->dtype != SIA_U8) return fail(SIA_ERR_INVALID_ARGUMENT, "codes must be uint8");
+  for (int d = 0; d + 1 < x->ndim; ++d)
+    if (codes->shape[d] != x->shape[d] || params->shape[d] != x->shape[d])
+      return fail(SIA_ERR_INVALID_ARGUMENT, "codes and params must have the leading dims of %s", xn);
+  return SIA_OK;
 }
 
 }  // namespace
@@ -262,26 +329,101 @@ int sia_quantize_kv_int8(const sia_tensor* x, const sia_tensor* out_int8, const 
   for (int d = 0; d + 1 < x->ndim; ++d)
     if (out_scale->shape[d] != x->shape[d]) return fail(SIA_ERR_INVALID_ARGUMENT, "out_scale shape differs from x[:-1]");
   // view all three as 4-dim (leading dims of size 1)
-  sia_tensor xv, ov, sv;
-  memset(&xv, 0, sizeof(xv));
-  memset(&ov, 0, sizeof(ov));
-  memset(&sv, 0, sizeof(sv));
-  const int pad = 4 - x->ndim;
-  xv.data = x->data; xv.dtype = x->dtype; xv.ndim = 4;
-  ov.data = out_int8->data; ov.dtype = SIA_I8; ov.ndim = 4;
-  sv.data = out_scale->data; sv.dtype = out_scale->dtype; sv.ndim = 3;
-  for (int d = 0; d < 4; ++d) {
-    const int s = d - pad;
-    xv.shape[d] = s >= 0 ? x->shape[s] : 1;
-    xv.stride[d] = s >= 0 ? x->stride[s] : 0;
-    ov.shape[d] = s >= 0 ? out_int8->shape[s] : 1;
-    ov.stride[d] = s >= 0 ? out_int8->stride[s] : 0;
-    if (d < 3) {
-      sv.shape[d] = s >= 0 ? out_scale->shape[s] : 1;
-      sv.stride[d] = s >= 0 ? out_scale->stride[s] : 0;
+  const sia_tensor xv = lead_to(*x, 4), ov = lead_to(*out_int8, 4), sv = lead_to(*out_scale, 3);
+  return sia_kv_write(&xv, nullptr, &ov, nullptr, &sv, nullptr, nullptr, nullptr, 0, 0, stream);
+}
+
+int sia_quantize_kv_int4(const sia_tensor* x, const sia_tensor* codes, const sia_tensor* params, void* stream) {
+  int rc;
+  if ((rc = check_i4_triple(x, codes, params, "x"))) return rc;
+  const sia_tensor xv = lead_to(*x, 4), cv = lead_to(*codes, 4), pv = lead_to(*params, 4);
+  return sia_kv_write(&xv, nullptr, &cv, nullptr, &pv, nullptr, nullptr, nullptr, 0, 0, stream);
+}
+
+int sia_dequantize_kv_int4(const sia_tensor* codes, const sia_tensor* params, const sia_tensor* out, void* stream) {
+  int rc;
+  if ((rc = check_i4_triple(out, codes, params, "out"))) return rc;
+  const sia_tensor ov = lead_to(*out, 4), cv = lead_to(*codes, 4), pv = lead_to(*params, 4);
+  return sia_kv_read(&cv, nullptr, &pv, nullptr, nullptr, nullptr, 0, 0, &ov, nullptr, stream);
+}
+
+int sia_kv_read(const sia_tensor* k_src, const sia_tensor* v_src, const sia_tensor* k_scale, const sia_tensor* v_scale,
+                const sia_tensor* block_table, const sia_tensor* start_pos, int32_t start_pos_host, int32_t page_size,
+                const sia_tensor* k_out, const sia_tensor* v_out, void* stream) {
+  int rc;
+  if ((rc = check_rows(k_out, "k_out", 16))) return rc;
+  if (!src_dtype_ok(k_out->dtype))
+    return fail(SIA_ERR_UNSUPPORTED, "k_out dtype %s: expected float16, bfloat16 or float32", dtype_name(k_out->dtype));
+  const bool two = v_out != nullptr;
+  if (two != (v_src != nullptr)) return fail(SIA_ERR_INVALID_ARGUMENT, "v_src and v_out go together");
+  const int64_t B = k_out->shape[0], H = k_out->shape[1], T = k_out->shape[2], D = k_out->shape[3];
+  if (!head_dim_ok(D))
+    return fail(SIA_ERR_UNSUPPORTED, "head_dim %lld not supported (16, 32, 64, 128, 256)", (long long)D);
+  if (k_src == nullptr) return fail(SIA_ERR_INVALID_ARGUMENT, "k_src is missing");
+  const int sd = k_src->dtype;
+  const bool int8 = sd == SIA_I8, int4 = sd == SIA_U8;
+  if (!int8 && !int4 && !src_dtype_ok(sd))
+    return fail(SIA_ERR_UNSUPPORTED, "source dtype %s not supported", dtype_name(sd));
+  if ((rc = check_rows(k_src, "k_src", int8 || int4 ? 8 : 16))) return rc;
+  const int64_t row = int4 ? i4_code_bytes(D) : D;
+  if (k_src->shape[1] != H || k_src->shape[3] != row)
+    return fail(SIA_ERR_INVALID_ARGUMENT, "source must be (*, %lld, *, %lld)", (long long)H, (long long)row);
+  KvReadArgs a;
+  memset(&a, 0, sizeof(a));
+  if (int4) {
+    if ((rc = check_i4_params(k_scale, k_src, D, "k_scale", &a.lg_group))) return rc;
+  } else if (int8) {
+    if ((rc = check_scale(k_scale, k_src, "k_scale"))) return rc;
+    a.scale_f32 = k_scale->dtype == SIA_F32;
+  }
+  if (two) {
+    if ((rc = check_rows(v_src, "v_src", int8 || int4 ? 8 : 16)) || (rc = check_rows(v_out, "v_out", 16)) ||
+        (rc = check_alike(k_src, v_src, "k_src", "v_src")) || (rc = check_alike(k_out, v_out, "k_out", "v_out")))
+      return rc;
+    if (int8 || int4) {
+      if (v_scale == nullptr || v_scale->data == nullptr)
+        return fail(SIA_ERR_INVALID_ARGUMENT, "v_scale is required for a quantised source");
+      if ((rc = check_alike(k_scale, v_scale, "k_scale", "v_scale"))) return rc;
+      if ((uintptr_t)v_scale->data % (int4 ? 4 : elem_size(v_scale->dtype)))
+        return fail(SIA_ERR_INVALID_ARGUMENT, "v_scale misaligned");
     }
   }
-  return sia_kv_write(&xv, nullptr, &ov, nullptr, &sv, nullptr, nullptr, nullptr, 0, 0, stream);
+  if (block_table != nullptr) {
+    if ((rc = fill_table(block_table, k_src, B, page_size, a))) return rc;
+    a.dpage = make_fastdiv((uint32_t)a.page);
+  } else {
+    if (k_src->shape[0] < B) return fail(SIA_ERR_INVALID_ARGUMENT, "cache batch dim smaller than the batch");
+    if (k_src->shape[2] > 0x7fffffff) return fail(SIA_ERR_UNSUPPORTED, "cache length too large");
+    a.cap = (int32_t)k_src->shape[2];
+  }
+  a.start_host = start_pos_host;
+  if (start_pos != nullptr) {
+    if ((rc = fill_start(start_pos, B, a))) return rc;
+  } else if (start_pos_host < 0 || (int64_t)start_pos_host + T > a.cap) {
+    return fail(SIA_ERR_INVALID_ARGUMENT, "positions [%d, %lld) exceed the cache length %d", start_pos_host,
+                (long long)start_pos_host + T, a.cap);
+  }
+  if (B > 0x7fffffff || H > 0x7fffffff || T > 0x7fffffff || (double)B * H * T * (D / 8) + 255 > 2147483647.0)
+    return fail(SIA_ERR_UNSUPPORTED, "too many rows for one launch");
+  if (B <= 0 || H <= 0 || T <= 0) return SIA_OK;
+  if ((rc = device_ok())) return rc;
+  a.src0 = (const char*)k_src->data;
+  a.src1 = two ? (const char*)v_src->data : nullptr;
+  a.s_s0 = bstride(k_src, 0); a.s_sh = bstride(k_src, 1); a.s_sn = bstride(k_src, 2);
+  if (int8 || int4) {
+    a.sc0 = (const char*)k_scale->data;
+    a.sc1 = two ? (const char*)v_scale->data : nullptr;
+    a.c_s0 = bstride(k_scale, 0); a.c_sh = bstride(k_scale, 1); a.c_sn = bstride(k_scale, 2);
+  }
+  a.dst0 = (char*)k_out->data;
+  a.dst1 = two ? (char*)v_out->data : nullptr;
+  a.d_sb = bstride(k_out, 0); a.d_sh = bstride(k_out, 1); a.d_st = bstride(k_out, 2);
+  a.B = (int32_t)B; a.H = (int32_t)H; a.T = (int32_t)T; a.D = (int32_t)D;
+  a.dT = make_fastdiv((uint32_t)T);
+  a.dH = make_fastdiv((uint32_t)H);
+  a.ntensors = two ? 2 : 1;
+  a.rows = (uint32_t)(B * H * T);
+  return launch_kv_read(a, sd, k_out->dtype, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -67,7 +67,7 @@ struct DecodeArgs {
   char* out; int64_t o_sb, o_sh;
   const char* k; int64_t k_s0, k_sh, k_sn;           // s0: batch (contiguous) or page (paged)
   const char* v; int64_t v_s0, v_sh, v_sn;
-  const char* ks; int64_t ks_s0, ks_sh, ks_sn;       // int8 scales (nullptr otherwise)
+  const char* ks; int64_t ks_s0, ks_sh, ks_sn;       // int8 scales or int4 parameters (nullptr otherwise)
   const char* vs; int64_t vs_s0, vs_sh, vs_sn;
   const int32_t* bt; int64_t bt_sb, bt_sl;           // block table (element strides), nullptr = contiguous
   int64_t num_pages;

@@ -28,6 +28,7 @@ struct DecodeLaunch {
   void* ws;                 // the caller's workspace (the fp32 path lays it out itself)
   size_t ws_bytes;
   int page_size;            // paged pools: tokens per page (0: contiguous cache)
+  int lg_group;             // int4 only: log2 of the elements per parameter pair
 };
 
 inline size_t decode_lds_bytes(int D, int G16, int B, int NW) {

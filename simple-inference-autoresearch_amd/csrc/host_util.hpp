@@ -79,4 +79,32 @@ inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 // Byte stride of dimension d.
 inline int64_t bstride(const sia_tensor* t, int d) { return t->stride[d] * elem_size(t->dtype); }
 
+// Checks the fp16 parameters (steps and minima) of 4-bit rows of D elements:
+// shaped like the codes `like` (whatever rank) with a last dim of 2 D / g.
+// *lg_group receives log2 g; g is 32, 64 or 128, at most D, or 16 at head_dim 16.
+inline int check_i4_params(const sia_tensor* s, const sia_tensor* like, int64_t D, const char* name, int* lg_group) {
+  if (s == nullptr || s->data == nullptr)
+    return fail(SIA_ERR_INVALID_ARGUMENT, "%s is required for int4 K/V", name);
+  if (s->dtype != SIA_F16) return fail(SIA_ERR_INVALID_ARGUMENT, "%s must be float16 for int4 K/V", name);
+  if (s->ndim != like->ndim) return fail(SIA_ERR_INVALID_ARGUMENT, "%s must have %d dims", name, like->ndim);
+  const int last = s->ndim - 1;
+  for (int d = 0; d < last; ++d)
+    if (s->shape[d] != like->shape[d])
+      return fail(SIA_ERR_INVALID_ARGUMENT, "%s must have the K/V shape but for its last dim", name);
+  const int64_t n = s->shape[last];
+  if (n < 2 || n % 2 || 2 * D % n)
+    return fail(SIA_ERR_INVALID_ARGUMENT, "%s's last dim %lld is not twice the number of groups of a row of %lld", name,
+                (long long)n, (long long)D);
+  const int64_t g = 2 * D / n;
+  if (g != 32 && g != 64 && g != 128 && !(g == 16 && D == 16))
+    return fail(SIA_ERR_UNSUPPORTED, "%s: groups of %lld elements (32, 64 or 128; 16 at head_dim 16)", name, (long long)g);
+  if (s->stride[last] != 1) return fail(SIA_ERR_INVALID_ARGUMENT, "%s must be contiguous along its last dim", name);
+  if ((uintptr_t)s->data % 4) return fail(SIA_ERR_INVALID_ARGUMENT, "%s must be 4-byte aligned", name);
+  for (int d = 0; d < last; ++d)
+    if (s->shape[d] > 1 && s->stride[d] % 2)
+      return fail(SIA_ERR_INVALID_ARGUMENT, "%s strides must be multiples of 4 bytes", name);
+  *lg_group = __builtin_ctz((unsigned)g);
+  return SIA_OK;
+}
+
 }  // namespace sia

@@ -1,6 +1,6 @@
 // KV write path for gfx950: store new K/V tokens into a contiguous cache or a
-// paged pool, quantising to int8 with per-token-per-head scales on the way
-// when the destination is int8.
+// paged pool, quantising on the way to int8 with per-token-per-head scales or
+// to 4 bits with a step and a minimum per group (int4.hpp).
 //
 // Semantics follow the reference engine:
 //  * quantize_kv_int8 (model/kv_cache.py:58-67): amax = max |x| over head_dim,
@@ -28,53 +28,12 @@
 // capacity, page id outside the pool) are skipped: the kernel never writes
 // outside the buffers it was given.
 #include "host_util.hpp"
+#include "int4.hpp"
+#include "kv_rows.hpp"
 #include "kv_write.hpp"
 #include "sia_common.hpp"
 
 namespace sia {
-
-template <class T>
-__device__ __forceinline__ void load8(const char* p, float* x);
-template <>
-__device__ __forceinline__ void load8<F16>(const char* p, float* x) {
-  const u32x4 w = *(const u32x4*)p;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { x[2 * i] = lo_f32(F16{}, w[i]); x[2 * i + 1] = hi_f32(F16{}, w[i]); }
-}
-template <>
-__device__ __forceinline__ void load8<BF16>(const char* p, float* x) {
-  const u32x4 w = *(const u32x4*)p;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { x[2 * i] = lo_f32(BF16{}, w[i]); x[2 * i + 1] = hi_f32(BF16{}, w[i]); }
-}
-template <>
-__device__ __forceinline__ void load8<F32>(const char* p, float* x) {
-  const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 16);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
-}
-
-template <class T>
-__device__ __forceinline__ void store8(char* p, const float* x);
-template <>
-__device__ __forceinline__ void store8<F16>(char* p, const float* x) {
-  u32x4 w;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = pack2(F16{}, x[2 * i], x[2 * i + 1]);
-  *(u32x4*)p = w;
-}
-template <>
-__device__ __forceinline__ void store8<BF16>(char* p, const float* x) {
-  u32x4 w;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = pack2(BF16{}, x[2 * i], x[2 * i + 1]);
-  *(u32x4*)p = w;
-}
-template <>
-__device__ __forceinline__ void store8<F32>(char* p, const float* x) {
-  *(f32x4*)p = f32x4{x[0], x[1], x[2], x[3]};
-  *(f32x4*)(p + 16) = f32x4{x[4], x[5], x[6], x[7]};
-}
 
 // N (4 or 8) consecutive table values of dtype C from element j0 of `row`
 // (a 16-byte aligned chunk: the host requires aligned tables).
@@ -163,6 +122,45 @@ __device__ __forceinline__ float div_by_scale(float x, float s, float inv) {
 __device__ __forceinline__ float group_max(float x, int width) {
   for (int o = width >> 1; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
   return x;
+}
+
+// This lane's 8 elements of a row as 4-bit codes (one word), and in `sm` its
+// group's parameters (s low, m high); see int4.hpp.  `gl` lanes (a power of
+// two, at most 16) hold a group.  Every lane of the wave calls this.
+__device__ __forceinline__ uint32_t quantise8_i4(float (&x)[8], int gl, uint32_t& sm) {
+#pragma clang fp contract(off)
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    bad |= !(fabsf(x[i]) <= 3.402823466e38f);
+    x[i] = __builtin_amdgcn_fmed3f(x[i], -kF16Max, kF16Max);
+  }
+  float lo = x[0], hi = x[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    lo = fminf(lo, x[i]);
+    hi = fmaxf(hi, x[i]);
+  }
+  for (int o = gl >> 1; o > 0; o >>= 1) {
+    lo = fminf(lo, __shfl_xor(lo, o));
+    hi = fmaxf(hi, __shfl_xor(hi, o));
+  }
+  const int lane = threadIdx.x & 63;
+  const uint64_t group = ((1ull << gl) - 1ull) << (lane & ~(gl - 1));
+  const bool poison = (__ballot(bad) & group) != 0;
+  const float m = (float)(_Float16)lo;
+  const float step = fmaxf(__fdiv_rn(hi - m, 15.0f), 0.0f);
+  const uint32_t sbits = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(step, lo)) & 0xffffu;
+  const float s = lo_f32(F16{}, sbits);
+  const float inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;    // (s = 0: every code is 0)
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float n = __builtin_amdgcn_fmed3f(__builtin_rintf(div_by_scale(x[i] - m, s, inv)), 0.0f, 15.0f);
+    w |= (uint32_t)n << (4 * i);
+  }
+  sm = poison ? 0x7e007e00u : sbits | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) << 16);
+  return poison ? 0u : w;
 }
 
 // The q part of a RoPE write: one work-group per token (b, t); a work item is
@@ -280,7 +278,15 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const KvWriteArgs a) {
         for (int i = 0; i < 8; ++i) x[i] = to_src<S>(x[i]);
       }
     }
-    if constexpr (std::is_same<DT, I8>::value) {
+    if constexpr (std::is_same<DT, I4>::value) {
+      uint32_t sm;
+      const uint32_t w = quantise8_i4(x, 1 << (a.lg_group - 3), sm);
+      if (store) {
+        *(uint32_t*)(dst + dst_row + 4 * i4_place(part, a.D)) = w;
+        const int first = part & ((1 << (a.lg_group - 3)) - 1);
+        if (first == 0) *(uint32_t*)(sdst + sc_row + 4 * (part >> (a.lg_group - 3))) = sm;
+      }
+    } else if constexpr (std::is_same<DT, I8>::value) {
       float m = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
@@ -321,6 +327,7 @@ static int launch_dst(const KvWriteArgs& a, int dst_dtype, hipStream_t stream) {
     case SIA_BF16: hipLaunchKernelGGL((kv_write_kernel<S, BF16, C, ROPE>), grid, dim3(256), 0, stream, a); break;
     case SIA_F32: hipLaunchKernelGGL((kv_write_kernel<S, F32, C, ROPE>), grid, dim3(256), 0, stream, a); break;
     case SIA_I8: hipLaunchKernelGGL((kv_write_kernel<S, I8, C, ROPE>), grid, dim3(256), 0, stream, a); break;
+    case SIA_U8: hipLaunchKernelGGL((kv_write_kernel<S, I4, C, ROPE>), grid, dim3(256), 0, stream, a); break;
     default: return fail(SIA_ERR_UNSUPPORTED, "destination dtype %s not supported", dtype_name(dst_dtype));
   }
   const hipError_t e = hipGetLastError();

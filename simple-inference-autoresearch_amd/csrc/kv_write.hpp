@@ -1,8 +1,10 @@
-// Host/device description of one KV write (see kv_write.hip).
+// Host/device description of KV writes and reads (kv_write.hip, kv_read.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include "sia_common.hpp"
 
 namespace sia {
 
@@ -11,7 +13,7 @@ struct KvWriteArgs {
   int64_t s_sb, s_sh, s_st;               // source byte strides (batch, head, token); head_dim contiguous
   char* dst0; char* dst1;                 // destinations: cache (B', H, S, D) or pool (pages, H, page, D)
   int64_t d_s0, d_sh, d_sn;               // destination byte strides
-  char* sc0; char* sc1;                   // int8 scale destinations (same indexing without head_dim)
+  char* sc0; char* sc1;                   // int8 scale / int4 parameter destinations (same indexing without head_dim)
   int64_t c_s0, c_sh, c_sn;               // scale byte strides
   const int32_t* bt; int64_t bt_sb, bt_sl;   // block table (element strides); nullptr = contiguous cache
   int64_t num_pages;
@@ -23,6 +25,7 @@ struct KvWriteArgs {
   int32_t ntensors;
   int32_t scale_f32;
   float amax_floor;                       // 1e-8 rounded to the source dtype
+  int32_t lg_group;                       // int4 destinations: log2 of the elements per (step, minimum) pair
   // rotary embedding of K (and q) on the way in; rope == 0 leaves the rows as they are
   int32_t rope;                           // 0 none, 1 split-half pairs (i, i + D/2), 2 interleaved (2i, 2i + 1)
   const char* cs; const char* sn;         // cos / sin tables (Tc, >= D/2), read at row `position`
@@ -40,5 +43,29 @@ struct KvWriteArgs {
 };
 
 int launch_kv_write(const KvWriteArgs& a, int src_dtype, int dst_dtype, hipStream_t stream);
+
+// Host/device description of one KV read (see kv_read.hip).
+struct KvReadArgs {
+  const char* src0; const char* src1;     // K and V: cache (B', H, S, D) or pool (pages, H, page, D)
+  int64_t s_s0, s_sh, s_sn;               // source byte strides
+  const char* sc0; const char* sc1;       // int8 scales / int4 parameters (nullptr otherwise)
+  int64_t c_s0, c_sh, c_sn;               // their byte strides
+  const int32_t* bt; int64_t bt_sb, bt_sl;   // block table (element strides); nullptr = contiguous cache
+  int64_t num_pages;
+  FastDiv dpage; int32_t page;            // tokens per page (paged)
+  int32_t cap;                            // positions the source holds (S, or max_blocks * page)
+  const int32_t* start; int32_t start_per_seq; int32_t start_host;   // first position: start_host + start[b]
+  char* dst0; char* dst1;                 // outputs (B, H, T, D)
+  int64_t d_sb, d_sh, d_st;               // output byte strides
+  int32_t B, H, T, D;
+  FastDiv dT, dH;                         // divisions by T and H
+  int32_t ntensors;
+  int32_t scale_f32;
+  int32_t lg_group;
+  int32_t log2_width;                     // log2 of the threads per row
+  uint32_t rows;                          // B * H * T
+};
+
+int launch_kv_read(const KvReadArgs& a, int src_dtype, int dst_dtype, hipStream_t stream);
 
 }  // namespace sia

@@ -12,6 +12,8 @@ attention_flash_decode_int8        kernels/flash_decode_int8_kernel.py:121-167
 paged_attention_flash_decode       kernels/paged_flash_decode_kernel.py:107-152
 gqa_int8_flash_decode              kernels/paged_flash_decode_int8_gqa_kernel.py:100-124
 paged_gqa_int8_flash_decode        (new: paged pool + int8 + GQA, BASELINE configs 3/5)
+attention_flash_decode_int4        (new: contiguous cache held in 4 bits)
+paged_gqa_int4_flash_decode        (new: paged pool held in 4 bits)
 =================================  =================================================
 
 Differences that only widen the reference's contract:
@@ -91,7 +93,7 @@ def _kv_len_tensor(kv_len, device: torch.device) -> torch.Tensor:
 
 
 # decode kinds of the extension's decode op (one per C entry point)
-CONTIG, CONTIG_INT8, GQA_INT8, PAGED, PAGED_INT8 = range(5)
+CONTIG, CONTIG_INT8, GQA_INT8, PAGED, PAGED_INT8, CONTIG_INT4, PAGED_INT4 = range(7)
 
 
 def _run(kind: int, q: torch.Tensor, k, v, k_scale, v_scale, block_table, kv_len, page_size: int,
@@ -209,3 +211,36 @@ def paged_gqa_int8_flash_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: t
     scale = (1.0 / (D ** 0.5)) if sm_scale is None else float(sm_scale)
     kl = _kv_len_tensor(kv_len, q.device)
     return _run(PAGED_INT8, q, k_pool, v_pool, k_scale_pool, v_scale_pool, block_table, kl, page_size, scale)
+
+
+def attention_flash_decode_int4(q: torch.Tensor, k_int4: torch.Tensor, v_int4: torch.Tensor,
+                                k_scale: torch.Tensor, v_scale: torch.Tensor, kv_len,
+                                sm_scale: float | None = None) -> torch.Tensor:
+    """Decode attention over a cache held in 4 bits (the format of :func:`~.kv_cache.quantize_kv_int4`).
+
+    k_int4, v_int4: (B, Hkv, S, D/2) uint8 codes; k_scale, v_scale: (B, Hkv, S,
+    2D/g) fp16 steps and minima of groups of g elements; kv_len int32, (1,)/()
+    shared or (B,) per sequence.  q (B, Hq, 1, D) fp16, bf16 or fp32; returns
+    (B, 1, Hq, D) in q's dtype.
+    """
+    scale = _common(q, k_int4, sm_scale)
+    kl = _kv_len_tensor(kv_len, q.device)
+    return _run(CONTIG_INT4, q, k_int4, v_int4, k_scale, v_scale, None, kl, 0, scale)
+
+
+def paged_gqa_int4_flash_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                                k_scale_pool: torch.Tensor, v_scale_pool: torch.Tensor,
+                                block_table: torch.Tensor, kv_len, page_size: int,
+                                sm_scale: float | None = None) -> torch.Tensor:
+    """Paged decode attention over pools held in 4 bits.
+
+    k_pool, v_pool: (num_blocks, Hkv, page_size, D/2) uint8 codes; k_scale_pool,
+    v_scale_pool: (num_blocks, Hkv, page_size, 2D/g) fp16; block_table (B,
+    max_blocks) int32; kv_len (1,)/() or (B,) int32.
+    """
+    P = k_pool.shape[2]
+    if P != page_size:
+        raise AssertionError(f"k_pool page dim {P} != page_size {page_size}")
+    scale = _common(q, k_pool, sm_scale)
+    kl = _kv_len_tensor(kv_len, q.device)
+    return _run(PAGED_INT4, q, k_pool, v_pool, k_scale_pool, v_scale_pool, block_table, kl, page_size, scale)

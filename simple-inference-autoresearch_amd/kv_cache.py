@@ -1,4 +1,4 @@
-"""Contiguous KV cache and the INT8-KV format, with the reference's interface.
+"""Contiguous KV cache and the INT8 and 4-bit KV formats, with the reference's interface.
 
 Drop-in for ``model/kv_cache.py`` of the reference engine:
 
@@ -13,6 +13,15 @@ Drop-in for ``model/kv_cache.py`` of the reference engine:
 * :meth:`KVCache.write_decode` -- the CUDA-graph decode write of
   ``ops/attention.py:217-228`` (``quantize_kv_int8`` + four ``index_copy_`` at
   ``ctx.pos_index``) as one launch that reads the position on the device.
+
+Without a counterpart in the reference:
+
+* :func:`quantize_kv_int4` / :func:`dequantize_kv_int4` -- K/V in 4 bits with a
+  step and a minimum per group of elements, and the values back;
+  ``KVCache(kv_dtype="int4")`` holds its pools that way.
+* :func:`kv_read` -- cached tokens of any format back as plain tensors, and
+  :meth:`KVCache.read`, with which a quantised prefix can be attended to by the
+  next chunk of a prompt.
 
 :func:`kv_write` is the general entry point both caches use.
 """
@@ -35,10 +44,53 @@ def kv_write(k: torch.Tensor, v: torch.Tensor | None, k_dst: torch.Tensor, v_dst
     Without ``block_table`` the destinations are contiguous ``(B', H, S, D)``
     views; with it they are paged pools ``(num_pages, H, page_size, D)``.
     An int8 destination is quantised per token and head (scales written to
+    ``k_scale_dst`` / ``v_scale_dst``), a uint8 one, ``(..., D/2)``, in 4 bits
+    as :func:`quantize_kv_int4` does (parameters ``(..., 2D/g)`` to
     ``k_scale_dst`` / ``v_scale_dst``); other destinations receive a cast copy.
     """
     _lib.gpu_ops().kv_write(k, v, k_dst, v_dst, k_scale_dst, v_scale_dst, block_table, start_pos,
                             int(start_offset), int(page_size))
+
+
+def kv_read(k_src: torch.Tensor, v_src: torch.Tensor | None, length: int, k_scale: torch.Tensor | None = None,
+            v_scale: torch.Tensor | None = None, block_table: torch.Tensor | None = None,
+            start_pos: torch.Tensor | None = None, start_offset: int = 0, page_size: int = 0,
+            dtype: torch.dtype | None = None, out=None):
+    """``length`` cached tokens of every sequence as plain ``(B, H, length, D)`` tensors (``sia_kv_read``).
+
+    The cache is contiguous ``(B, H, S, D)`` or, with ``block_table (B,
+    max_blocks)``, a pool ``(num_pages, H, page_size, D)``: 16-bit, fp32, int8
+    with scales, or uint8 codes ``(..., D/2)`` with int4 parameters.  Token
+    ``t`` of sequence ``b`` is position ``start_offset + start_pos[b] + t``, as
+    in :func:`kv_write`; without ``start_pos`` every position must lie inside
+    the cache, with it positions outside read as zeros (so do page ids outside
+    the pool).  ``dtype`` defaults to the cache's, or to bfloat16 for a
+    quantised one.  ``out=(k, v)`` writes into the caller's tensors instead (any
+    strides, 16-byte aligned rows).  Returns ``(k, v)``; ``v`` is None when
+    ``v_src`` is.
+    """
+    ops = _lib.gpu_ops()
+    length = int(length)
+    if k_src.dim() != 4:
+        raise ValueError("k_src must have 4 dims")
+    if length < 0:
+        raise ValueError("length must not be negative")
+    quantised = k_src.dtype in (torch.int8, torch.uint8)
+    D = k_src.shape[3] * (2 if k_src.dtype == torch.uint8 else 1)
+    B = block_table.shape[0] if block_table is not None else k_src.shape[0]
+    shape = (B, k_src.shape[1], length, D)
+    if out is None:
+        dt = dtype or (torch.bfloat16 if quantised else k_src.dtype)
+        k = torch.empty(shape, dtype=dt, device=k_src.device)
+        v = torch.empty(shape, dtype=dt, device=k_src.device) if v_src is not None else None
+    else:
+        k, v = out
+        if dtype not in (None, k.dtype):
+            raise ValueError("dtype differs from out's")
+        if tuple(k.shape) != shape or (v is None) != (v_src is None):
+            raise ValueError(f"out must be a (k, v) pair of shape {shape}, v None exactly where v_src is")
+    ops.kv_read(k_src, v_src, k_scale, v_scale, block_table, start_pos, int(start_offset), int(page_size), k, v)
+    return k, v
 
 
 def rope_kv_write(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor | None, cos: torch.Tensor,
@@ -77,6 +129,43 @@ def quantize_kv_int8(x: torch.Tensor, scale_dtype: torch.dtype = torch.float16):
     return ops.quantize_kv_int8(src, scale_dtype == torch.float32)
 
 
+def quantize_kv_int4(x: torch.Tensor, group_size: int = 64):
+    """K or V ``(..., D)`` in 4 bits -> codes ``(..., D/2)`` uint8, parameters ``(..., 2D/g)`` fp16.
+
+    Groups of ``g = min(group_size, D)`` consecutive elements (``group_size``
+    32, 64 or 128) share a minimum ``m`` and a step ``s``; a code ``n`` stands
+    for ``m + n s``.  With lo, hi the group's extremes clamped to +-65504:
+    ``m = fp16(lo)``, ``s = fp16(max(0, (hi - m) / 15))`` rounded towards zero
+    (so ``m + 15 s <= hi``), ``n = round((x - m) / s)`` half to even within 0
+    and 15, 0 where ``s`` is 0.  A group with a NaN or an infinity reads back as NaN.
+    The parameters alternate, ``[s0, m0, s1, m1, ...]``; the order of the codes
+    is that of ``include/sia_attention.h``, which every function here shares.
+    """
+    ops = _lib.gpu_ops()
+    g = int4_group(x.shape[-1], group_size)
+    src = x if x.stride(-1) == 1 and all((s * x.element_size()) % 16 == 0 for s in x.stride()[:-1]) \
+        and x.data_ptr() % 16 == 0 else x.contiguous()
+    return ops.quantize_kv_int4(src, g)
+
+
+def dequantize_kv_int4(codes: torch.Tensor, params: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values ``(..., D)`` that codes ``(..., D/2)`` and parameters ``(..., 2D/g)`` stand for, rounded once."""
+    return _lib.gpu_ops().dequantize_kv_int4(codes, params, dtype)
+
+
+def int4_group(head_dim: int, group_size: int) -> int:
+    """Elements per group of a 4-bit row: ``group_size``, at most the row."""
+    if group_size not in (32, 64, 128):
+        raise ValueError("group_size must be 32, 64 or 128")
+    return min(group_size, head_dim)
+
+
+def int4_pools(rows: tuple, head_dim: int, group: int, device):
+    """Zeroed codes and parameters of 4-bit rows ``(*rows, head_dim)``."""
+    return (torch.zeros(*rows, head_dim // 2, dtype=torch.uint8, device=device),
+            torch.zeros(*rows, 2 * head_dim // group, dtype=torch.float16, device=device))
+
+
 def _int32_positions(pos: torch.Tensor) -> torch.Tensor:
     """Device positions as int32 (the reference's ctx.pos_index is int64)."""
     if pos.dtype == torch.int32:
@@ -93,7 +182,12 @@ class KVCache:
     INT8_SEQ_THRESHOLD = 256
 
     def __init__(self, n_layers: int, max_batch: int, max_seq_len: int, n_heads_kv: int, head_dim: int,
-                 dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda"):
+                 dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda",
+                 kv_dtype: torch.dtype | str | None = None, group_size: int = 64):
+        """``kv_dtype``: None for the reference's rule (int8 above the threshold), ``torch.int8``, or ``"int4"``
+        for 4-bit pools with a step and a minimum per ``group_size`` elements."""
+        if kv_dtype not in (None, torch.int8, "int4"):
+            raise ValueError('kv_dtype must be None, torch.int8 or "int4"')
         self.n_layers = n_layers
         self.max_batch = max_batch
         self.max_seq_len = max_seq_len
@@ -101,9 +195,14 @@ class KVCache:
         self.head_dim = head_dim
         self.dtype = dtype
         self.device = torch.device(device)
-        self.is_int8 = max_seq_len > KVCache.INT8_SEQ_THRESHOLD
+        self.is_int4 = kv_dtype == "int4"
+        self.is_int8 = kv_dtype == torch.int8 or (kv_dtype is None and max_seq_len > KVCache.INT8_SEQ_THRESHOLD)
+        self.group_size = int4_group(head_dim, group_size) if self.is_int4 else None
         shape = (n_layers, max_batch, n_heads_kv, max_seq_len, head_dim)
-        if self.is_int8:
+        if self.is_int4:
+            self.k_cache, self.k_scale = int4_pools(shape[:-1], head_dim, self.group_size, self.device)
+            self.v_cache, self.v_scale = int4_pools(shape[:-1], head_dim, self.group_size, self.device)
+        elif self.is_int8:
             self.k_cache = torch.zeros(shape, dtype=torch.int8, device=self.device)
             self.v_cache = torch.zeros(shape, dtype=torch.int8, device=self.device)
             sshape = (n_layers, max_batch, n_heads_kv, max_seq_len)
@@ -117,17 +216,22 @@ class KVCache:
     def _layer(self, layer_idx: int, B: int):
         kc = self.k_cache[layer_idx, :B]
         vc = self.v_cache[layer_idx, :B]
-        ks = self.k_scale[layer_idx, :B] if self.is_int8 else None
-        vs = self.v_scale[layer_idx, :B] if self.is_int8 else None
+        ks = self.k_scale[layer_idx, :B] if self.is_quantized else None
+        vs = self.v_scale[layer_idx, :B] if self.is_quantized else None
         return kc, vc, ks, vs
+
+    @property
+    def is_quantized(self) -> bool:
+        """int8 or 4-bit pools, with scales or parameters in ``k_scale`` / ``v_scale``."""
+        return self.is_int8 or self.is_int4
 
     def update(self, layer_idx: int, start_pos: int, k: torch.Tensor, v: torch.Tensor):
         """Write K/V ``(B, Hkv, T, D)`` at ``[start_pos, start_pos + T)``.
 
         Returns what ``model/kv_cache.py:133-184`` returns: the cached prefix
         views ``(B, Hkv, start_pos + T, D)`` for a 16-bit cache, and the new
-        ``k, v`` themselves for an int8 cache (whose prefix is read by the int8
-        decode kernels instead).
+        ``k, v`` themselves for an int8 or 4-bit cache (whose prefix is read by
+        the decode kernels, or back with :meth:`read`).
         """
         B, H, T, D = k.shape
         end = start_pos + T
@@ -137,7 +241,7 @@ class KVCache:
         assert end <= self.max_seq_len, f"sequence overflow: start_pos+T={end} > max_seq_len={self.max_seq_len}"
         kc, vc, ks, vs = self._layer(layer_idx, B)
         kv_write(k, v, kc, vc, ks, vs, start_offset=start_pos)
-        if self.is_int8:
+        if self.is_quantized:
             return k, v
         return self.k_cache[layer_idx, :B, :, :end, :], self.v_cache[layer_idx, :B, :, :end, :]
 
@@ -163,9 +267,20 @@ class KVCache:
         sequence's position ``pos_index`` on the device, so no per-step table
         row copy is needed.
         """
-        ks, vs = (self.k_scale, self.v_scale) if self.is_int8 else (None, None)
+        ks, vs = (self.k_scale, self.v_scale) if self.is_quantized else (None, None)
         return _lib.gpu_ops().rope_kv_write_layer(q, k, v, cos, sin, self.k_cache, self.v_cache, ks, vs, layer_idx,
                                                   None, _int32_positions(pos_index), 0, 0, bool(interleaved))
+
+    def read(self, layer_idx: int, B: int, length: int, start_pos: int = 0, dtype: torch.dtype | None = None,
+             out=None):
+        """Cached K/V of positions ``[start_pos, start_pos + length)``, ``(B, Hkv, length, D)`` each (:func:`kv_read`).
+
+        ``dtype`` defaults to the cache's ``dtype``.
+        """
+        assert B <= self.max_batch, f"batch {B} > max_batch {self.max_batch}"
+        kc, vc, ks, vs = self._layer(layer_idx, B)
+        return kv_read(kc, vc, length, ks, vs, start_offset=start_pos,
+                       dtype=dtype if dtype is not None or out is not None else self.dtype, out=out)
 
     def reset(self) -> None:
         """Logical reset between independent sequences (nothing to clear, as in the reference)."""

@@ -12,6 +12,9 @@ all widening the contract:
 * ``kv_dtype=torch.int8`` stores int8 pools with fp32 per-token-per-head scale
   pools ``(L, num_blocks, Hkv, block_size)`` (the format of the paged INT8-KV
   GQA decode kernel); writes quantise on the fly.
+* ``kv_dtype="int4"`` stores 4-bit pools ``(L, num_blocks, Hkv, block_size,
+  D/2)`` with fp16 parameter pools ``(..., 2D/g)`` (:func:`~.kv_cache.quantize_kv_int4`).
+* :meth:`read` gives cached tokens back as plain tensors, through the block table.
 * The decode-step write that the reference documents but never implements
   (``slot_for``, ``model/paged_kv_cache.py:29-30``) is :meth:`write_decode`:
   the slot is derived on the device from ``seq_lens`` through the block table,
@@ -26,15 +29,16 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .decode import PAGED, PAGED_INT8, _common, _run_layer
-from .kv_cache import kv_write
+from .decode import PAGED, PAGED_INT4, PAGED_INT8, _common, _run_layer
+from .kv_cache import int4_group, int4_pools, kv_read, kv_write
 
 
 class PagedKVCache:
     BACKEND = "paged"
 
     def __init__(self, n_layers, max_batch, max_seq_len, n_heads_kv, head_dim, block_size=16,
-                 dtype=torch.bfloat16, device="cuda", kv_dtype: torch.dtype | None = None):
+                 dtype=torch.bfloat16, device="cuda", kv_dtype: torch.dtype | str | None = None,
+                 group_size: int = 64):
         self.n_layers = n_layers
         self.max_batch = max_batch
         self.max_seq_len = max_seq_len
@@ -44,21 +48,27 @@ class PagedKVCache:
         self.dtype = dtype
         self.device = torch.device(device)
         self.kv_dtype = dtype if kv_dtype is None else kv_dtype
-        if self.kv_dtype not in (torch.float16, torch.bfloat16, torch.int8):
-            raise ValueError("kv_dtype must be float16, bfloat16 or int8")
+        if self.kv_dtype not in (torch.float16, torch.bfloat16, torch.int8, "int4"):
+            raise ValueError('kv_dtype must be float16, bfloat16, int8 or "int4"')
         self.is_int8 = self.kv_dtype == torch.int8
+        self.is_int4 = self.kv_dtype == "int4"
+        self.group_size = int4_group(head_dim, group_size) if self.is_int4 else None
 
         self.max_blocks_per_seq = (max_seq_len + block_size - 1) // block_size
         # one full max_seq_len per request, as the reference sizes it
         self.num_blocks = max_batch * self.max_blocks_per_seq
         shape = (n_layers, self.num_blocks, n_heads_kv, block_size, head_dim)
-        self.k_pool = torch.zeros(shape, dtype=self.kv_dtype, device=self.device)
-        self.v_pool = torch.zeros(shape, dtype=self.kv_dtype, device=self.device)
+        if self.is_int4:
+            self.k_pool, self.k_scale_pool = int4_pools(shape[:-1], head_dim, self.group_size, self.device)
+            self.v_pool, self.v_scale_pool = int4_pools(shape[:-1], head_dim, self.group_size, self.device)
+        else:
+            self.k_pool = torch.zeros(shape, dtype=self.kv_dtype, device=self.device)
+            self.v_pool = torch.zeros(shape, dtype=self.kv_dtype, device=self.device)
         if self.is_int8:
             sshape = (n_layers, self.num_blocks, n_heads_kv, block_size)
             self.k_scale_pool = torch.zeros(sshape, dtype=torch.float32, device=self.device)
             self.v_scale_pool = torch.zeros(sshape, dtype=torch.float32, device=self.device)
-        else:
+        elif not self.is_int4:
             self.k_scale_pool = self.v_scale_pool = None
 
         self.block_tables = torch.zeros(max_batch, self.max_blocks_per_seq, dtype=torch.int32, device=self.device)
@@ -87,9 +97,9 @@ class PagedKVCache:
 
     # -- views ----------------------------------------------------------------------
     def layer(self, layer_idx: int):
-        """(k_pool, v_pool, k_scale_pool, v_scale_pool) of one layer (scales None unless int8)."""
-        ks = self.k_scale_pool[layer_idx] if self.is_int8 else None
-        vs = self.v_scale_pool[layer_idx] if self.is_int8 else None
+        """(k_pool, v_pool, k_scale_pool, v_scale_pool) of one layer (scales None unless quantised)."""
+        ks = self.k_scale_pool[layer_idx] if self.k_scale_pool is not None else None
+        vs = self.v_scale_pool[layer_idx] if self.v_scale_pool is not None else None
         return self.k_pool[layer_idx], self.v_pool[layer_idx], ks, vs
 
     # -- writes ---------------------------------------------------------------------
@@ -124,17 +134,30 @@ class PagedKVCache:
         rotated by that row of the full ``cos``/``sin`` tables, so requests at
         different positions share one launch.
         """
-        ks, vs = (self.k_scale_pool, self.v_scale_pool) if self.is_int8 else (None, None)
-        return _lib.gpu_ops().rope_kv_write_layer(q, k, v, cos, sin, self.k_pool, self.v_pool, ks, vs, layer_idx,
+        return _lib.gpu_ops().rope_kv_write_layer(q, k, v, cos, sin, self.k_pool, self.v_pool, self.k_scale_pool,
+                                                  self.v_scale_pool, layer_idx,
                                                   self.block_tables, self.seq_lens, -1, self.block_size,
                                                   bool(interleaved))
 
     def decode_attention(self, layer_idx: int, q: torch.Tensor, sm_scale: float | None = None) -> torch.Tensor:
         """Decode attention of ``q (B, Hq, 1, D)`` over each request's ``seq_lens[b]`` cached tokens."""
         scale = _common(q, self.k_pool, sm_scale)
-        ks, vs = (self.k_scale_pool, self.v_scale_pool) if self.is_int8 else (None, None)
-        return _run_layer(PAGED_INT8 if self.is_int8 else PAGED, q, self.k_pool, self.v_pool, ks, vs, layer_idx,
+        kind = PAGED_INT4 if self.is_int4 else PAGED_INT8 if self.is_int8 else PAGED
+        return _run_layer(kind, q, self.k_pool, self.v_pool, self.k_scale_pool, self.v_scale_pool, layer_idx,
                           self.block_tables, self.seq_lens, self.block_size, scale)
+
+    # -- reads ----------------------------------------------------------------------
+    def read(self, layer_idx: int, B: int, length: int, start_pos: int = 0, dtype: torch.dtype | None = None,
+             out=None):
+        """Cached K/V of positions ``[start_pos, start_pos + length)`` of requests ``[0, B)``, through the block table.
+
+        ``(B, Hkv, length, D)`` each, in ``dtype`` (default: the cache's ``dtype``).
+        """
+        assert B <= self.max_batch
+        kp, vp, ks, vs = self.layer(layer_idx)
+        return kv_read(kp, vp, length, ks, vs, block_table=self.block_tables[:B], start_offset=start_pos,
+                       page_size=self.block_size,
+                       dtype=dtype if dtype is not None or out is not None else self.dtype, out=out)
 
     def __repr__(self):
         gb = 2 * self.k_pool.numel() * self.k_pool.element_size() / 1e9

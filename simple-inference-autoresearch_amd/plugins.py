@@ -36,18 +36,25 @@ ATTENTION_NAME = "sia"
 
 
 def llama_cache_builder(config, *, max_batch: int, max_seq_len: int, dtype: torch.dtype,
-                        device: torch.device | str) -> KVCache:
-    """The llama plugin's cache hook (``model/llama_plugin.py:22-38``) on this library's KVCache."""
+                        device: torch.device | str, kv_dtype: torch.dtype | str | None = None,
+                        group_size: int = 64) -> KVCache:
+    """The llama plugin's cache hook (``model/llama_plugin.py:22-38``) on this library's KVCache.
+
+    ``kv_dtype="int4"`` holds K/V in 4 bits with parameters per ``group_size`` elements.
+    """
     return KVCache(n_layers=config.num_hidden_layers, max_batch=max_batch, max_seq_len=max_seq_len,
-                   n_heads_kv=config.num_key_value_heads, head_dim=config.head_dim, dtype=dtype, device=device)
+                   n_heads_kv=config.num_key_value_heads, head_dim=config.head_dim, dtype=dtype, device=device,
+                   kv_dtype=kv_dtype, group_size=group_size)
 
 
 def llama_paged_cache_builder(config, *, max_batch: int, max_seq_len: int, dtype: torch.dtype,
                               device: torch.device | str, block_size: int = 16,
-                              kv_dtype: torch.dtype | None = None) -> PagedKVCache:
-    """Same hook, building a paged cache (``kv_dtype=torch.int8`` for int8 pools with fp32 scales)."""
+                              kv_dtype: torch.dtype | str | None = None, group_size: int = 64) -> PagedKVCache:
+    """Same hook, building a paged cache (``kv_dtype=torch.int8`` for int8 pools with fp32 scales, ``"int4"`` for
+    4-bit pools with fp16 parameters per ``group_size`` elements)."""
     return PagedKVCache(config.num_hidden_layers, max_batch, max_seq_len, config.num_key_value_heads,
-                        config.head_dim, block_size=block_size, dtype=dtype, device=device, kv_dtype=kv_dtype)
+                        config.head_dim, block_size=block_size, dtype=dtype, device=device, kv_dtype=kv_dtype,
+                        group_size=group_size)
 
 
 # ------------------------------------------------ transformers attention hook

@@ -173,7 +173,7 @@ size_t decode_ws_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int dev) {
   return n;
 }
 
-enum DecodeKind { kContig = 0, kContigInt8 = 1, kGqaInt8 = 2, kPaged = 3, kPagedInt8 = 4 };
+enum DecodeKind { kContig = 0, kContigInt8 = 1, kGqaInt8 = 2, kPaged = 3, kPagedInt8 = 4, kContigInt4 = 5, kPagedInt4 = 6 };
 
 Tensor decode_call(int64_t kind, const Tensor& q, const sia_tensor& dk, const sia_tensor& dv, const sia_tensor* dks,
                    const sia_tensor* dvs, const sia_tensor* dbt, const sia_tensor& dl, int64_t page_size,
@@ -253,6 +253,13 @@ Tensor decode_call(int64_t kind, const Tensor& q, const sia_tensor& dk, const si
       break;
     case kPagedInt8:
       rc = sia_paged_gqa_int8_flash_decode(&dq, &dk, &dv, dks, dvs, dbt, &dl, (int32_t)page_size, sc, &dout,
+                                           ws.data_ptr(), ws_bytes, po, s);
+      break;
+    case kContigInt4:
+      rc = sia_attention_flash_decode_int4(&dq, &dk, &dv, dks, dvs, &dl, sc, &dout, ws.data_ptr(), ws_bytes, po, s);
+      break;
+    case kPagedInt4:
+      rc = sia_paged_gqa_int4_flash_decode(&dq, &dk, &dv, dks, dvs, dbt, &dl, (int32_t)page_size, sc, &dout,
                                            ws.data_ptr(), ws_bytes, po, s);
       break;
     default:
@@ -336,6 +343,50 @@ std::tuple<Tensor, Tensor> quantize_kv_int8(const Tensor& x, bool scale_f32) {
   const sia_tensor dxi = desc(xi, dev, "out"), ds = desc(scale, dev, "scale");
   check(sia_quantize_kv_int8(&dx, &dxi, &ds, stream_of(dev)));
   return {xi, scale};
+}
+
+// x (..., D) -> codes (..., D / 2) uint8 and parameters (..., 2 D / group) fp16.
+std::tuple<Tensor, Tensor> quantize_kv_int4(const Tensor& x, int64_t group) {
+  const at::Device dev = gpu_of(x, "x");
+  const c10::DeviceGuard guard(dev);
+  if (x.dim() < 1) throw py::value_error("x must have at least one dim");
+  const int64_t D = x.size(-1);
+  if (group < 1 || D % 2 || D % group) throw py::value_error("head_dim must be a multiple of the group size");
+  std::vector<int64_t> cs(x.sizes().begin(), x.sizes().end()), ps = cs;
+  cs.back() = D / 2;
+  ps.back() = 2 * D / group;
+  Tensor codes = at::empty(cs, x.options().dtype(at::kByte));
+  Tensor params = at::empty(ps, x.options().dtype(at::kHalf));
+  if (x.numel() == 0) return {codes, params};
+  const sia_tensor dx = desc(x, dev, "x"), dc = desc(codes, dev, "codes"), dp = desc(params, dev, "params");
+  check(sia_quantize_kv_int4(&dx, &dc, &dp, stream_of(dev)));
+  return {codes, params};
+}
+
+Tensor dequantize_kv_int4(const Tensor& codes, const Tensor& params, at::ScalarType dtype) {
+  const at::Device dev = gpu_of(codes, "codes");
+  const c10::DeviceGuard guard(dev);
+  if (codes.dim() < 1) throw py::value_error("codes must have at least one dim");
+  std::vector<int64_t> os(codes.sizes().begin(), codes.sizes().end());
+  os.back() *= 2;
+  Tensor out = at::empty(os, codes.options().dtype(dtype));
+  if (out.numel() == 0) return out;
+  const sia_tensor dc = desc(codes, dev, "codes"), dp = desc(params, dev, "params"), dout = desc(out, dev, "out");
+  check(sia_dequantize_kv_int4(&dc, &dp, &dout, stream_of(dev)));
+  return out;
+}
+
+// Positions [start, start + T) of a cache or pool into k_out / v_out (B, H, T, D).
+void kv_read(const Tensor& k_src, const OptT& v_src, const OptT& k_scale, const OptT& v_scale, const OptT& block_table,
+             const OptT& start_pos, int64_t start_offset, int64_t page_size, const Tensor& k_out, const OptT& v_out) {
+  const at::Device dev = gpu_of(k_src, "k_src");
+  const c10::DeviceGuard guard(dev);
+  if (k_out.numel() == 0 && k_out.dim() == 4) return;   // no tokens to read
+  const sia_tensor dk = desc(k_src, dev, "k_src"), dko = desc(k_out, dev, "k_out");
+  const OptDesc dv(v_src, dev, "v_src"), dks(k_scale, dev, "k_scale"), dvs(v_scale, dev, "v_scale"),
+      dbt(block_table, dev, "block_table"), dsp(start_pos, dev, "start_pos"), dvo(v_out, dev, "v_out");
+  check(sia_kv_read(&dk, dv.ptr(), dks.ptr(), dvs.ptr(), dbt.ptr(), dsp.ptr(), (int32_t)start_offset,
+                    (int32_t)page_size, &dko, dvo.ptr(), stream_of(dev)));
 }
 
 void kv_write(const Tensor& k, const OptT& v, const Tensor& k_dst, const OptT& v_dst, const OptT& k_scale_dst,
@@ -445,6 +496,9 @@ PYBIND11_MODULE(_sia_ops, m) {
   m.def("prefill", &prefill);
   m.def("prefill_rope", &prefill_rope);
   m.def("quantize_kv_int8", &quantize_kv_int8);
+  m.def("quantize_kv_int4", &quantize_kv_int4);
+  m.def("dequantize_kv_int4", &dequantize_kv_int4);
+  m.def("kv_read", &kv_read);
   m.def("kv_write", &kv_write);
   m.def("rope_kv_write", &rope_kv_write);
   m.def("rope_kv_write_layer", &rope_kv_write_layer);

@@ -90,6 +90,8 @@ EXTRA_FLAGS = {
     "decode_f16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "decode_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "decode_i8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "decode_i4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "decode_i4_d128.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attn_f32_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

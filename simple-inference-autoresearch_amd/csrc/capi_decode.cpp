@@ -350,6 +350,7 @@ int dispatch(DecodeLaunch& L, int kv_dtype) {
     case SIA_F16: return launch_decode_f16(L);
     case SIA_BF16: return launch_decode_bf16(L);
     case SIA_I8: return launch_decode_i8(L);
+    case SIA_U8: return launch_decode_i4(L);
     default: return fail(SIA_ERR_UNSUPPORTED, "k/v dtype %s not supported", dtype_name(kv_dtype));
   }
 }
@@ -387,8 +388,8 @@ int decode_any(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, co
   // pages that do not hold whole 16-token tiles (page sizes 1-8, or any size
   // other than 16 * 2^k) go to the vector-ALU path with its per-token lookup
   const bool tiled_pages = bt == nullptr || (kTile << L.a.lg_tiles_per_page) == page_size;
-  if (k->dtype == SIA_U8) return dispatch_f32(L, g, k->dtype, out);
-  if (q->dtype == SIA_F32 || k->dtype == SIA_F32 || !tiled_pages) return dispatch_f32(L, g, k->dtype, out);
+  // (int4 at head_dim 16 and 32 too: a row there is a fraction of a k-step)
+  if (q->dtype == SIA_F32 || k->dtype == SIA_F32 || !tiled_pages || (k->dtype == SIA_U8 && g.D < 64)) return dispatch_f32(L, g, k->dtype, out);
   return dispatch(L, k->dtype);
 }
 

@@ -123,6 +123,17 @@ int launch_decode_q(DecodeLaunch& L) {
   return fail(SIA_ERR_UNSUPPORTED, "query dtype must be float16 or bfloat16");
 }
 
+// int4 K/V with groups of G elements at head_dim D (64, 128, 256).
+template <int D, int G>
+int launch_decode_i4_typed(DecodeLaunch& L) {
+  if (L.q_dtype == SIA_F16) return launch_decode_typed<D, I4G<G>, F16, F16>(L);
+  if (L.q_dtype == SIA_BF16) return launch_decode_typed<D, I4G<G>, BF16, F16>(L);
+  return fail(SIA_ERR_UNSUPPORTED, "query dtype must be float16 or bfloat16");
+}
+int launch_decode_i4(DecodeLaunch& L);       // decode_i4.hip
+int launch_decode_i4_128(DecodeLaunch& L);   // decode_i4_d128.hip
+int launch_decode_i4_256(DecodeLaunch& L);   // decode_i4_d256.hip
+
 // Entry points implemented by decode_f16.hip / decode_bf16.hip / decode_i8.hip.
 int launch_decode_f16(DecodeLaunch& L);
 int launch_decode_bf16(DecodeLaunch& L);

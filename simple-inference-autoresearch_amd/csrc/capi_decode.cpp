@@ -66,9 +66,11 @@ int geometry(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, Geometry& g) {
 // Otherwise it keeps wide items: a page holds every KV head's 16 tokens side
 // by side and the waves of a wide item read them together; narrower items
 // that still leave a split ran config 2's main kernel 2-2.5 us (7%) slower.
-void item_units(Geometry& g, bool paged) {
+// int4 counts two work-groups per CU in place of one: a batch of 64 x 8 KV heads
+// takes items of one unit, and no piece of a sequence is left to merge.
+void item_units(Geometry& g, bool paged, bool int4) {
   const int nw = decode_waves(g.D);
-  const int cus = device_info().cus > 0 ? device_info().cus : 256;
+  const int cus = (device_info().cus > 0 ? device_info().cus : 256) * (int4 ? 2 : 1);
   auto items = [&](int iu) { return (int64_t)g.B * ((g.U + iu - 1) / iu); };
   g.IU = g.U < nw ? g.U : nw;
   int iu = g.IU;
@@ -154,6 +156,10 @@ int prepare_kv(const sia_tensor* k, const sia_tensor* v, const Geometry& g, bool
   for (int d = 0; d < 3; ++d)
     if (bstride(k, d) % align || bstride(v, d) % align)
       return fail(SIA_ERR_INVALID_ARGUMENT, "k/v strides must be multiples of %d bytes", align);
+  if (int4)   // (one layout, as in sia_kv_write and sia_kv_read: the kernel computes a tile's offset once for both)
+    for (int d = 0; d < 3; ++d)
+      if (k->shape[d] > 1 && k->stride[d] != v->stride[d])
+        return fail(SIA_ERR_UNSUPPORTED, "int4 k and v must have the same strides");
   DecodeArgs& a = L.a;
   a.k = (const char*)k->data; a.k_s0 = bstride(k, 0); a.k_sh = bstride(k, 1); a.k_sn = bstride(k, 2);
   a.v = (const char*)v->data; a.v_s0 = bstride(v, 0); a.v_sh = bstride(v, 1); a.v_sn = bstride(v, 2);
@@ -218,6 +224,9 @@ int prepare_i4_params(const sia_tensor* ks, const sia_tensor* vs, const sia_tens
   if ((rc = check_i4_params(ks, k, g.D, "k_scale", &L.lg_group))) return rc;
   if ((rc = check_i4_params(vs, k, g.D, "v_scale", &lgv))) return rc;
   if (lgv != L.lg_group) return fail(SIA_ERR_INVALID_ARGUMENT, "k_scale and v_scale have different group sizes");
+  for (int d = 0; d < 3; ++d)
+    if (ks->shape[d] > 1 && ks->stride[d] != vs->stride[d])
+      return fail(SIA_ERR_UNSUPPORTED, "int4 k_scale and v_scale must have the same strides");
   DecodeArgs& a = L.a;
   a.ks = (const char*)ks->data; a.ks_s0 = bstride(ks, 0); a.ks_sh = bstride(ks, 1); a.ks_sn = bstride(ks, 2);
   a.vs = (const char*)vs->data; a.vs_s0 = bstride(vs, 0); a.vs_sh = bstride(vs, 1); a.vs_sn = bstride(vs, 2);
@@ -229,6 +238,9 @@ int prepare_i4_params(const sia_tensor* ks, const sia_tensor* vs, const sia_tens
       return fail(SIA_ERR_UNSUPPORTED, "k_scale/v_scale page stride too large");
     a.ks_pg = (uint32_t)a.ks_s0; a.vs_pg = (uint32_t)a.vs_s0;
   }
+  // a tile's offsets and its buffer range are 32-bit
+  if (a.k_sn * kTile + 256 > 0xfffffff0LL || a.ks_sn * kTile + 256 > 0xfffffff0LL)
+    return fail(SIA_ERR_UNSUPPORTED, "int4 token stride too large");
   return SIA_OK;
 }
 
@@ -365,7 +377,7 @@ int decode_any(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, co
   int rc;
   if (k == nullptr) return fail(SIA_ERR_INVALID_ARGUMENT, "k is NULL");
   if ((rc = prepare_common(q, kv_len, out, (int)k->shape[1], sm_scale, g, L))) return rc;
-  item_units(g, bt != nullptr);
+  item_units(g, bt != nullptr, k->dtype == SIA_U8);
   L.a.IU = g.IU;
   L.a.UB = g.UB;
   if ((rc = prepare_kv(k, v, g, bt != nullptr, page_size, L))) return rc;

@@ -238,31 +238,6 @@ __device__ __forceinline__ float scale_of(const Scales<ST, SV>& s, int i) {
   else return SV ? ((i & 1) ? hi_f32(F16{}, s.w[i >> 1]) : lo_f32(F16{}, s.w[i >> 1])) : lo_f32(F16{}, s.w[i]);
 }
 
-// 4-bit K/V with a step and a minimum per G elements (int4.hpp).
-template <int G>
-struct I4G { static constexpr int group = G; };
-template <class KV> struct IsInt4 { static constexpr bool value = false; };
-template <int G> struct IsInt4<I4G<G>> { static constexpr bool value = true; };
-
-// Bytes of n consecutive elements.
-template <class KV>
-constexpr int kv_bytes(int n) {
-  if constexpr (IsInt4<KV>::value) return n / 2;
-  else return n * KV::bytes;
-}
-
-// int4 parameters of a lane (words: step low, minimum high): for K all groups
-// of its 4 tokens, for V the groups that its share of a row lies in.
-template <int D, class KV>
-struct I4Params { };
-template <int D, int G>
-struct I4Params<D, I4G<G>> {
-  static constexpr int NK = D / G;                        // groups of a row
-  static constexpr int NV = D == 256 && G == 32 ? 2 : 1;  // groups of a lane's V share (see v_word)
-  Raw<4 * NK> k[4];
-  Raw<4 * NV> v[4];
-};
-
 // One 16-token tile's operands as held by one lane.
 template <int D, class KV, class ST, bool SV>
 struct Tile {
@@ -272,22 +247,18 @@ struct Tile {
   // lanes of a row read 64 contiguous bytes per load instruction.  (A lane
   // owning a contiguous quarter of the row instead made every 16-bit load
   // instruction touch 64 cache lines at 16 bytes each.)
-  static constexpr int KB = kv_bytes<KV>(D / 4);
+  static constexpr int KB = (D / 4) * KV::bytes;
   static constexpr int KSTRIDE = 64;                                      // bytes between a lane's K pieces
-  static constexpr int VB = kv_bytes<KV>(D / 16);    // V bytes per lane per token (see kVSplit)
+  static constexpr int VB = (D / 16) * KV::bytes;    // V bytes per lane per token (see kVSplit)
   static constexpr bool kInt8 = std::is_same<KV, I8>::value;
-  static constexpr bool kInt4 = IsInt4<KV>::value;
-  // int4: 16 bytes of K hold one word of each of four consecutive k-steps
-  // (int4.hpp; 8 bytes and two at D = 64), and V is D/32 bytes of codes.
   // V of one token: elements [lane16*D/16, +D/16), or, when a lane's share is
   // more than 16 bytes (16-bit V at D = 256), 16-byte pieces 256 bytes apart,
   // elements [128 p + 8 lane16, +8) for piece p, so that one load instruction
   // reads whole 128-byte lines of the row.
-  static constexpr bool kVSplit = !kInt8 && !kInt4 && VB > 16;
+  static constexpr bool kVSplit = !kInt8 && VB > 16;
   Raw<KB> k;
   Raw<VB> v[4];                                      // tokens 4*grp + i
   Scales<ST, SV> ks, vs;                             // int8 scales of tokens 4*grp + i
-  I4Params<D, KV> par;                               // int4 parameters of tokens 4*grp + i
 };
 
 // This lane's byte offsets inside one tile (constant): K of token lane16
@@ -313,7 +284,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const char* p) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, -1, kRawBufferFlags);
 }
 
-// BYTES at rsrc + off (BYTES a multiple of 16, or 8 or 4); 16-byte pieces
+// BYTES at rsrc + off (BYTES a multiple of 16, or 8, 4 or 2); 16-byte pieces
 // STRIDE bytes apart.
 template <int BYTES, int STRIDE = 16>
 __device__ __forceinline__ void load_raw_buf(Raw<BYTES>& r, __amdgpu_buffer_rsrc_t rs, uint32_t off) {
@@ -364,21 +335,6 @@ __device__ __forceinline__ void load_tile(const DecodeArgs& a, const TilePtr& t,
     if (FULL || 4 * grp + i < valid) load_raw_buf<C::VB, C::kVSplit ? 256 : 16>(c.v[i], rv, o.v[i]);
     else zero_raw<C::VB>(c.v[i]);
   }
-  if constexpr (C::kInt4) {
-    // (a token's parameters in one load; 4-byte alignment is enough for any width)
-    const __amdgpu_buffer_rsrc_t rks = tile_rsrc(t.ks), rvs = tile_rsrc(t.vs);
-    using PT = I4Params<D, KV>;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (FULL || 4 * grp + i < valid) {
-        load_raw_buf<4 * PT::NK>(c.par.k[i], rks, o.ks + i * a.ks_tok);
-        load_raw_buf<4 * PT::NV>(c.par.v[i], rvs, o.vs + i * a.vs_tok);
-      } else {
-        zero_raw<4 * PT::NK>(c.par.k[i]);
-        zero_raw<4 * PT::NV>(c.par.v[i]);
-      }
-    }
-  }
   if constexpr (C::kInt8) {
     const __amdgpu_buffer_rsrc_t rks = tile_rsrc(t.ks), rvs = tile_rsrc(t.vs);
     if constexpr (FULL && SV && std::is_same<ST, F32>::value) {
@@ -417,17 +373,7 @@ __device__ __forceinline__ void load_tile(const DecodeArgs& a, const TilePtr& t,
 template <int D, class KV, class ST, bool SV>
 __device__ __forceinline__ u32x4 k_operand(const Tile<D, KV, ST, SV>& c, int j) {
   u32x4 r;
-  if constexpr (IsInt4<KV>::value) {
-    // code pairs (0, 4), (1, 5), (2, 6), (3, 7) as fp16 denormals: n 2^-24
-    // from bits 0-3 of a half, n 2^-20 from bits 4-7, which the query's odd
-    // elements make up for (prep_q).  The matrix cores multiply denormals
-    // exactly, so five instructions serve 8 codes.
-    const uint32_t w = c.k.w[j], w8 = w >> 8;
-    r[0] = w & 0x000f000fu;
-    r[1] = w & 0x00f000f0u;
-    r[2] = w8 & 0x000f000fu;
-    r[3] = w8 & 0x00f000f0u;
-  } else if constexpr (std::is_same<KV, I8>::value) {
+  if constexpr (std::is_same<KV, I8>::value) {
     const uint32_t w0 = c.k.w[2 * j] ^ 0x80808080u;
     const uint32_t w1 = c.k.w[2 * j + 1] ^ 0x80808080u;
     r[0] = i8pair_to_f16x2(w0, 0x04010400u);
@@ -443,48 +389,12 @@ __device__ __forceinline__ u32x4 k_operand(const Tile<D, KV, ST, SV>& c, int j) 
   return r;
 }
 
-// int4 V: the halves of words of codes and the parameter pairs of tokens (t, t + 1).
-struct I4Pair {
-  uint32_t x, x8;    // 4 codes of each token: as loaded, and shifted down by 8 bits
-  f16x2 s, m;
-};
-// Codes e & 3 of a pair as values m + n s, rounded once to fp16 (n exactly:
-// 0x6400 | n is 1024 + n, 0x5400 | n << 4 is 64 + n).
-__device__ __forceinline__ uint32_t i4_pair(const I4Pair& p, int e) {
-  const uint32_t c = (e & 2) ? p.x8 : p.x;
-  f16x2 n;
-  if (e & 1) {
-    const f16x2 bias = {(_Float16)-64.0f, (_Float16)-64.0f};
-    n = __builtin_bit_cast(f16x2, (c & 0x00f000f0u) | 0x54005400u) + bias;
-  } else {
-    const f16x2 bias = {(_Float16)-1024.0f, (_Float16)-1024.0f};
-    n = __builtin_bit_cast(f16x2, (c & 0x000f000fu) | 0x64006400u) + bias;
-  }
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n, p.s, p.m));
-}
-// Half h of a lane's V codes (4 of them; word h / 2 of a token's share) of tokens t and t + 1.
-template <int D, class KV, class ST, bool SV>
-__device__ __forceinline__ I4Pair i4_half(const Tile<D, KV, ST, SV>& c, int t, int h) {
-  using PT = I4Params<D, KV>;
-  const int gv = PT::NV == 2 ? h >> 1 : 0;
-  I4Pair p;
-  p.x = gather16(c.v[t].w[h >> 1], c.v[t + 1].w[h >> 1], h & 1);
-  p.x8 = p.x >> 8;
-  const uint32_t a = c.par.v[t].w[gv], b = c.par.v[t + 1].w[gv];
-  p.s = __builtin_bit_cast(f16x2, gather16(a, b, 0));
-  p.m = __builtin_bit_cast(f16x2, gather16(a, b, 1));
-  return p;
-}
-
 // V^T operand (A of O^T += V^T P^T, 16x16x16) for d-tile e: element e of the
 // lane's D/16-wide slice for tokens (4g, 4g+1) and (4g+2, 4g+3).
 template <int D, class KV, class ST, bool SV>
 __device__ __forceinline__ u32x2 v_operand(const Tile<D, KV, ST, SV>& c, int e) {
   u32x2 r;
-  if constexpr (IsInt4<KV>::value) {
-    r[0] = i4_pair(i4_half(c, 0, e >> 2), e);
-    r[1] = i4_pair(i4_half(c, 2, e >> 2), e);
-  } else if constexpr (std::is_same<KV, I8>::value) {
+  if constexpr (std::is_same<KV, I8>::value) {
     r[0] = i8gather_to_f16x2(c.v[0].w[e >> 2], c.v[1].w[e >> 2], e & 3);
     r[1] = i8gather_to_f16x2(c.v[2].w[e >> 2], c.v[3].w[e >> 2], e & 3);
   } else {
@@ -518,8 +428,7 @@ struct WaveState {
 
 template <int D, class KV, class QT, class ST, bool FULL, bool SV>
 __device__ __forceinline__ void compute_tile(const Tile<D, KV, ST, SV>& c, const u32x4* qop, const u32x4* qop_lo,
-                                             const float* qsum, float qmul, int tile, int ntok, int grp,
-                                             WaveState<D>& st) {
+                                             float qmul, int tile, int ntok, int grp, WaveState<D>& st) {
   using MT = typename MmaOf<KV>::T;
   constexpr int KSTEPS = D / 32;
   constexpr int E = D / 16;
@@ -531,30 +440,7 @@ __device__ __forceinline__ void compute_tile(const Tile<D, KV, ST, SV>& c, const
   constexpr bool kPSplit = !kInt8 && std::is_same<MT, BF16>::value;
 
   float s[4];
-  if constexpr (IsInt4<KV>::value) {
-    // sum_i q_i (m + n_i s) = s sum_i q_i n_i + m sum_i q_i, group by group:
-    // the products of the codes are exact, s and m are applied in fp32 (qsum
-    // holds the query's sums, in the scale of the products)
-    constexpr int NK = D / KV::group, PER = KV::group / 32;
-    f32x4 gacc[NK];
-#pragma unroll
-    for (int gi = 0; gi < NK; ++gi) {
-      gacc[gi] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = PER * gi; j < PER * (gi + 1); ++j) gacc[gi] = mfma16x16x32(MT{}, k_operand(c, j), qop[j], gacc[gi]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float t = 0.f;
-#pragma unroll
-      for (int gi = 0; gi < NK; ++gi) {
-        const uint32_t sm = c.par.k[i].w[gi];
-        t = __builtin_fmaf(hi_f32(F16{}, sm), qsum[gi], t);
-        t = __builtin_fmaf(lo_f32(F16{}, sm), gacc[gi][i], t);
-      }
-      s[i] = t * qmul;
-    }
-  } else if constexpr (kInt8) {
+  if constexpr (kInt8) {
     // int8 K against the three int8 query terms (q = step * (hi + mid/254 +
     // lo/254^2), hi and mid in qop, lo in qop_lo): exact integer dot
     // products, no conversion of K
@@ -664,11 +550,8 @@ __device__ __forceinline__ QRaw<D> load_q_raw(const DecodeArgs& a, int b, int hq
 
 // Q operand for a unit from its raw row.  Returns the per-lane score
 // multiplier (sm_scale*log2e, times the query's scale step).
-// int4 K: qsum[g] receives 2^-24 times the sum of group g's elements, as the
-// products carry that factor, and the multiplier makes up for it.
 template <int D, class KV, class QT>
-__device__ __forceinline__ float prep_q(const DecodeArgs& a, const QRaw<D>& raw, u32x4* qop, u32x4* qop_lo,
-                                        float* qsum) {
+__device__ __forceinline__ float prep_q(const DecodeArgs& a, const QRaw<D>& raw, u32x4* qop, u32x4* qop_lo) {
   using MT = typename MmaOf<KV>::T;
   constexpr int KSTEPS = D / 32;
   constexpr int PER = D / 4;
@@ -733,25 +616,6 @@ __device__ __forceinline__ float prep_q(const DecodeArgs& a, const QRaw<D>& raw,
     for (int i = 0; i < PER; ++i) qf[i] = ldexpf(qf[i], sh);
     mul = ldexpf(mul, -sh);
   }
-  if constexpr (IsInt4<KV>::value) {
-    constexpr int PER_G = KV::group / 32;
-#pragma unroll
-    for (int gi = 0; gi < D / KV::group; ++gi) {
-      float t = 0.f;
-#pragma unroll
-      for (int i = 8 * PER_G * gi; i < 8 * PER_G * (gi + 1); ++i) t += qf[i];
-      qsum[gi] = wave_sum_xor16_32(t) * 0x1p-24f;
-    }
-    // the order and the powers of two of k_operand's pairs
-#pragma unroll
-    for (int j = 0; j < KSTEPS; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float f = (i & 1) ? 0.0625f : 1.0f;
-        qop[j][i] = pack2(MT{}, qf[8 * j + i] * f, qf[8 * j + i + 4] * f);
-      }
-    return mul * 0x1p24f;
-  }
 #pragma unroll
   for (int j = 0; j < KSTEPS; ++j) {
 #pragma unroll
@@ -766,6 +630,12 @@ __device__ __forceinline__ float prep_q(const DecodeArgs& a, const QRaw<D>& raw,
   return mul;
 }
 
+}  // namespace sia
+
+#include "decode_i4.hpp"
+
+namespace sia {
+
 // Head-dim index of accumulator element (e, i) of a lane in row group g: the
 // PV product's d-tile e holds, in output row 4 g + i, the element that lane
 // 4 g + i loaded as element e of its V share (see Tile).
@@ -773,12 +643,11 @@ template <int D, class KV>
 __device__ __forceinline__ int out_d(int g, int i, int e) {
   if constexpr (IsInt4<KV>::value) {
     // lane l = 4 g + i holds the half word at place l / 2 (D = 64), the word at
-    // place l (128) or the words at places 2 l and 2 l + 1 (256)
+    // place l (128) or the words at places 2 l and 2 l + 1 (256); see int4.hpp
     if constexpr (D == 64) return 32 * (i >> 1) + 8 * g + 4 * (i & 1) + e;
     else if constexpr (D == 128) return 32 * i + 8 * g + e;
     else return 128 * (g >> 1) + 64 * (i & 1) + 32 * (e >> 3) + 16 * (g & 1) + 8 * (i >> 1) + (e & 7);
-  }
-  if constexpr (Tile<D, KV, F32, false>::kVSplit) return 128 * (e >> 3) + 32 * g + 8 * i + (e & 7);
+  } else if constexpr (Tile<D, KV, F32, false>::kVSplit) return 128 * (e >> 3) + 32 * g + 8 * i + (e & 7);
   else return g * (D / 4) + i * (D / 16) + e;
 }
 
@@ -789,6 +658,12 @@ __device__ __forceinline__ int out_d(int g, int i, int e) {
 template <int D, class KV, bool SV>
 struct DecodeWaves {
   static constexpr int value = D <= 64 && (!std::is_same<KV, I8>::value || SV) ? 4 : (D <= 128 ? 2 : 1);
+};
+// int4 holds one tile instead of two and fits twice as many waves, but for the
+// four parameter pairs per token of head_dim 128 in groups of 32, which spill.
+template <int D, int G, bool SV>
+struct DecodeWaves<D, I4G<G>, SV> {
+  static constexpr int value = D <= 128 ? 4 : 2;
 };
 
 // Geometry of one item inside a work-group of NW waves (all uniform): it
@@ -830,9 +705,13 @@ void decode_main(const DecodeArgs a) {
   constexpr int E = D / 16;
   constexpr int KSTEPS = D / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  // LDS: [acc: NW*G16*D f32][m: NW*G16][l: NW*G16][red: 2*NW+2 ints][pre: B+1 ints][lens: B ints, B <= kLensInLds]
+  // LDS: [acc: NW*G16*D f32, int4: the waves' rings][m: NW*G16][l: NW*G16][red: 2*NW+2 ints][pre: B+1 ints][lens: B ints, B <= kLensInLds]
   float* l_acc = (float*)smem;
-  float* l_m = l_acc + NW * a.G16 * D;
+  // floats between the waves' parts of l_acc
+  int acc_wave;
+  if constexpr (IsInt4<KV>::value) acc_wave = i4_wave_lds<D, KV>(a.G16) / 4;
+  else acc_wave = a.G16 * D;
+  float* l_m = l_acc + NW * acc_wave;
   float* l_l = l_m + NW * a.G16;
   int* red = (int*)(l_l + NW * a.G16);
   int* pre = red + 2 * NW + 2;
@@ -893,15 +772,16 @@ void decode_main(const DecodeArgs a) {
   const int lane = threadIdx.x & 63;
   const int wave = uniform(threadIdx.x >> 6);
   const int lane16 = lane & 15, grp = lane >> 4;
-  using TileT = Tile<D, KV, ST, SV>;
-  LaneOff lo;
-  lo.k = lane16 * a.k_tok + (uint32_t)(grp * (TileT::kInt4 && D == 64 ? 8 : 16));
+  constexpr bool kInt4 = IsInt4<KV>::value;
+  using TileT = std::conditional_t<kInt4, I4Tile<D, KV>, Tile<D, KV, ST, SV>>;
+  std::conditional_t<kInt4, int, LaneOff> lo;
+  if constexpr (!kInt4) {
+    lo.k = lane16 * a.k_tok + (uint32_t)(grp * 16);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) lo.v[i] = (4 * grp + i) * a.v_tok + (uint32_t)(lane16 * (TileT::kVSplit ? 16 : TileT::VB));
-  lo.ks = 4 * grp * a.ks_tok;
-  lo.vs = 4 * grp * a.vs_tok;
-  if constexpr (TileT::kInt4)   // the (first) group of the lane's V share
-    lo.vs += 4 * (uint32_t)((8 * i4_word((int)(lane16 * TileT::VB) / 4, D)) / KV::group);
+    for (int i = 0; i < 4; ++i) lo.v[i] = (4 * grp + i) * a.v_tok + (uint32_t)(lane16 * (TileT::kVSplit ? 16 : TileT::VB));
+    lo.ks = 4 * grp * a.ks_tok;
+    lo.vs = 4 * grp * a.vs_tok;
+  }
   const int uin = wave >> a.lgP;         // unit slot of this wave inside an item
   const int phase = wave & (shape.P - 1);
 
@@ -959,7 +839,7 @@ void decode_main(const DecodeArgs a) {
   // to), so that a segment change waits for its first tile only.
   // (Not where its registers do not fit: head_dim 64, two groups per CU in 128
   // registers, and int8 with scattered scales.)
-  constexpr bool kNext = D > 64 && (!TileT::kInt8 || SV);
+  constexpr bool kNext = D > 64 && (!TileT::kInt8 || SV) && !kInt4;
   QRaw<D> q_next;
   int pg_next = 0, seg_next = -1;
   bool first_seg = true;
@@ -1009,14 +889,21 @@ void decode_main(const DecodeArgs a) {
       // already in flight), unless the previous segment loaded them already.
       QRaw<D> qraw;
       int pg0;
-      constexpr bool kPartFirst = D > 64 && !(D == 256 && QSplit<KV, QT>::value);   // (see below)
+      constexpr bool kPartFirst = D > 64 && !(D == 256 && QSplit<KV, QT>::value) && !kInt4;   // (see below)
+      // int4: lane l holds the page id of the wave's tile k0 + l, 64 tiles by one load
+      auto page_window = [&](int k0) {
+        const int t = t_first + max(0, min(k0 + lane, nt - 1)) * P;
+        return btrow[(int64_t)(min(t, cap_tiles - 1) >> a.lg_tiles_per_page) * bt_step];
+      };
+      int pgw = 0;
+      if constexpr (kInt4) pgw = page_window(0);
       int pgl = kPartFirst && nt > nfull ? page_id(nfull) : 0;
       if (kNext && x == seg_next) {
         qraw = q_next;
         pg0 = pg_next;
       } else {
         qraw = load_q_raw<D, KV>(a, b, hq, live, grp);
-        pg0 = page_id(0);
+        pg0 = kInt4 ? 0 : page_id(0);
       }
       // the next segment of the share, if this wave has a unit there: its
       // query row and first page id (issued behind this segment's first tile)
@@ -1049,9 +936,16 @@ void decode_main(const DecodeArgs a) {
         TilePtr tp;
         const uint32_t pg = (uint32_t)phys < npages ? (uint32_t)phys : 0u;   // never read outside the pool
         const uint32_t off = (uint32_t)((t & tpp_mask) * kTile);
+        if constexpr (kInt4) {       // (one layout for K and V)
+          const uint64_t o = uniform64((uint64_t)pg * a.k_pg + (uint64_t)off * a.k_tok);
+          const uint64_t os = uniform64((uint64_t)pg * a.ks_pg + (uint64_t)off * a.ks_tok);
+          tp.k = kb + o; tp.v = vb + o;
+          tp.ks = ksb + os; tp.vs = vsb + os;
+          return tp;
+        }
         tp.k = kb + uniform64((uint64_t)pg * a.k_pg + (uint64_t)off * a.k_tok);
         tp.v = vb + uniform64((uint64_t)pg * a.v_pg + (uint64_t)off * a.v_tok);
-        if constexpr (TileT::kInt8 || TileT::kInt4) {
+        if constexpr (TileT::kInt8) {
           tp.ks = ksb + uniform64((uint64_t)pg * a.ks_pg + (uint64_t)off * a.ks_tok);
           tp.vs = vsb + uniform64((uint64_t)pg * a.vs_pg + (uint64_t)off * a.vs_tok);
         } else {
@@ -1059,8 +953,60 @@ void decode_main(const DecodeArgs a) {
         }
         return tp;
       };
+      if constexpr (kInt4) {
+        // Tiles through the wave's ring in LDS (see decode_i4.hpp), kStages - 1 of
+        // them in flight.
+        if (nt > 0) {
+          using R = I4Ring<D, KV>;
+          const I4Lane<D, KV> il(a, lane);
+          const I4Const ic;
+          I4Query<D, KV> qi;
+          char* ring = smem + wave * i4_wave_lds<D, KV>(a.G16);
+          auto left = [&](int k) { return k < nt ? ntok - (t_first + k * P) * kTile : 0; };   // live tokens of tile k
+          auto issue = [&](int k, int stage) {
+            const int kn = min(k, nt - 1);
+            const TilePtr tp = tile_ptr(t_first + kn * P, __builtin_amdgcn_readlane(pgw, kn & 63));
+            i4_issue<D, KV>(a, tp, il, left(k), ring + stage * R::kStage);
+          };
+#pragma unroll
+          for (int k = 0; k < R::kStages - 1; ++k) issue(k, k);
+          i4_prep_q<D, KV, QT>(a, qraw, grp, qi);
+          int at = 0;                                    // stage of tile k
+          for (int k = 0; k < nt; ++k) {
+            const int kn = k + R::kStages - 1;
+            if ((kn & 63) == 0 && kn < nt) {
+              pgw = page_window(kn);
+              asm volatile("" ::"v"(pgw));               // (waited for here, not by every round at its readlane)
+            }
+            issue(kn, at == 0 ? R::kStages - 1 : at - 1);
+            i4_wait<(R::kStages - 1) * R::kTransfers>();
+            const char* stage = ring + at * R::kStage;
+            I4Tile<D, KV> c;
+            float s[4], p[4];
+            i4_read_k<D, KV>(stage, il, c);
+            i4_scores<D, KV>(c, qi, s);
+            i4_read_v<D, KV>(stage, il, c);
+            if (k >= nfull) {
+              // the sequence's partial last tile (uniform).  Its dead tokens
+              // weigh 0; their parameters are cleared too, so that the result
+              // never depends on what a dropped read leaves behind.
+              const int live_tok = left(k);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (4 * grp + i >= live_tok) {
+                  s[i] = -INFINITY;
+#pragma unroll
+                  for (int g2 = 0; g2 < I4Tile<D, KV>::NV; ++g2) c.vp[i].w[g2] = 0u;
+                }
+            }
+            i4_softmax<D>(s, qi.mul, st, p);
+            i4_pv<D, KV>(c, ic, p, st);
+            at = at + 1 == R::kStages ? 0 : at + 1;
+          }
+          i4_wait<0>();                                  // (the empty transfers too: the merge reuses the ring)
+        }
+      } else {
       u32x4 qop[KSTEPS], qop_lo[KSTEPS];
-      float qsum[8];               // (int4: one per group)
       float qmul = 0.f;
       // The sequence's partial last tile, if it is this wave's, is loaded and
       // computed first (its order is free), while the first full tile is in
@@ -1078,7 +1024,7 @@ void decode_main(const DecodeArgs a) {
                                            ntok - (t_first + nfull * P) * kTile, last, lane16, grp);
       };
       auto compute_part = [&](const TileT& last) {
-        compute_tile<D, KV, QT, ST, false>(last, qop, qop_lo, qsum, qmul, t_first + nfull * P, ntok, grp, st);
+        compute_tile<D, KV, QT, ST, false>(last, qop, qop_lo, qmul, t_first + nfull * P, ntok, grp, st);
       };
       const bool part = nt > nfull;
       std::conditional_t<kPartFirst, TileT, int> first;     // (the partial tile, where it is taken first)
@@ -1105,7 +1051,7 @@ void decode_main(const DecodeArgs a) {
         load_tile<D, KV, ST, true, SV>(a, tile_ptr(t_first, pg0), lo, 16, bufA, lane16, grp);
         prefetch_next();
         // the query's conversion overlaps the first tile's flight
-        qmul = prep_q<D, KV, QT>(a, qraw, qop, qop_lo, qsum);
+        qmul = prep_q<D, KV, QT>(a, qraw, qop, qop_lo);
         if constexpr (kPartFirst) {
           if (part) compute_part(first);
         }
@@ -1125,9 +1071,9 @@ void decode_main(const DecodeArgs a) {
           const int pg1 = __builtin_amdgcn_readlane(pgv, 0), pg2 = __builtin_amdgcn_readlane(pgv, 1);
           load_tile<D, KV, ST, true, SV>(a, tile_ptr(t_first + (k + 1) * P, pg1), lo, 16, bufB, lane16, grp);
           pgv = page_pair(k + 3);
-          compute_tile<D, KV, QT, ST, true>(bufA, qop, qop_lo, qsum, qmul, 0, ntok, grp, st);
+          compute_tile<D, KV, QT, ST, true>(bufA, qop, qop_lo, qmul, 0, ntok, grp, st);
           load_tile<D, KV, ST, true, SV>(a, tile_ptr(t_first + (k + 2) * P, pg2), lo, 16, bufA, lane16, grp);
-          compute_tile<D, KV, QT, ST, true>(bufB, qop, qop_lo, qsum, qmul, 0, ntok, grp, st);
+          compute_tile<D, KV, QT, ST, true>(bufB, qop, qop_lo, qmul, 0, ntok, grp, st);
         }
         if constexpr (NW == 8) {
           __builtin_amdgcn_s_setprio(0);
@@ -1139,14 +1085,14 @@ void decode_main(const DecodeArgs a) {
         if (k + 1 < nfull) {
           load_tile<D, KV, ST, true, SV>(a, tile_ptr(t_first + (k + 1) * P, __builtin_amdgcn_readlane(pgv, 0)), lo,
                                          16, bufB, lane16, grp);
-          compute_tile<D, KV, QT, ST, true>(bufA, qop, qop_lo, qsum, qmul, 0, ntok, grp, st);
-          compute_tile<D, KV, QT, ST, true>(bufB, qop, qop_lo, qsum, qmul, 0, ntok, grp, st);
+          compute_tile<D, KV, QT, ST, true>(bufA, qop, qop_lo, qmul, 0, ntok, grp, st);
+          compute_tile<D, KV, QT, ST, true>(bufB, qop, qop_lo, qmul, 0, ntok, grp, st);
         } else {
-          compute_tile<D, KV, QT, ST, true>(bufA, qop, qop_lo, qsum, qmul, 0, ntok, grp, st);
+          compute_tile<D, KV, QT, ST, true>(bufA, qop, qop_lo, qmul, 0, ntok, grp, st);
         }
       } else {
         prefetch_next();
-        qmul = prep_q<D, KV, QT>(a, qraw, qop, qop_lo, qsum);
+        qmul = prep_q<D, KV, QT>(a, qraw, qop, qop_lo);
         if constexpr (kPartFirst) {
           if (part) compute_part(first);
         }
@@ -1157,6 +1103,7 @@ void decode_main(const DecodeArgs a) {
           load_part(last);
           compute_part(last);
         }
+      }
       }
     }
 
@@ -1199,7 +1146,7 @@ void decode_main(const DecodeArgs a) {
       // states read one after the other and three runtime divisions each, took
       // 3.4 us of a 10.7 us group at one sequence of 1000 tokens.)
       if (live) {
-        float* dst = l_acc + (wave * a.G16 + lane16) * D;
+        float* dst = l_acc + wave * acc_wave + lane16 * D;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1223,10 +1170,10 @@ void decode_main(const DecodeArgs a) {
           fDL x[PB];
 #pragma unroll
           for (int p2 = 0; p2 < PB; ++p2) {
-            const int ws = min(p0 + p2, w1) * a.G16 + cc;
+            const int wn = min(p0 + p2, w1), ws = wn * a.G16 + cc;
             mw[p2] = l_m[ws];
             lw[p2] = l_l[ws];
-            x[p2] = *(const fDL*)(l_acc + ws * D + DL * lane);
+            x[p2] = *(const fDL*)(l_acc + wn * acc_wave + cc * D + DL * lane);
           }
           float mb = M;
 #pragma unroll

@@ -31,8 +31,9 @@ struct DecodeLaunch {
   int lg_group;             // int4 only: log2 of the elements per parameter pair
 };
 
-inline size_t decode_lds_bytes(int D, int G16, int B, int NW) {
-  return (size_t)NW * G16 * D * 4 + (size_t)2 * NW * G16 * 4 + (size_t)(2 * NW + 2) * 4 +
+// wave_bytes: what a wave has of it by itself (its merge state; int4: its ring, which the merge reuses)
+inline size_t decode_lds_bytes(size_t wave_bytes, int G16, int B, int NW) {
+  return (size_t)NW * wave_bytes + (size_t)2 * NW * G16 * 4 + (size_t)(2 * NW + 2) * 4 +
          (size_t)(B + 1) * 4 + (B <= kLensInLds ? (size_t)B * 4 : 0);
 }
 
@@ -59,7 +60,9 @@ int launch_decode_typed(DecodeLaunch& L) {
   L.a.dHq = make_fastdiv((uint32_t)L.a.Hq);
   L.a.dG = make_fastdiv((uint32_t)L.a.G);
   L.a.dIU = make_fastdiv((uint32_t)L.a.IU);
-  const size_t lds = decode_lds_bytes(D, L.a.G16, L.a.B, NW);
+  size_t wave_bytes = (size_t)L.a.G16 * D * 4;
+  if constexpr (IsInt4<KV>::value) wave_bytes = (size_t)i4_wave_lds<D, KV>(L.a.G16);
+  const size_t lds = decode_lds_bytes(wave_bytes, L.a.G16, L.a.B, NW);
   const int occ = kernel_occupancy((const void*)kmain, NW * 64, lds);
   if (occ <= 0) return fail(SIA_ERR_LAUNCH, "decode kernel does not fit on a CU (LDS %zu B)", lds);
   L.a.cus = device_info().cus;

@@ -32,6 +32,18 @@
 namespace sia {
 
 struct I4 { static constexpr int code = SIA_U8; };
+// The same with groups of G elements known to the compiler (the matrix kernels).
+template <int G>
+struct I4G { static constexpr int group = G; };
+template <class KV> struct IsInt4 { static constexpr bool value = false; };
+template <int G> struct IsInt4<I4G<G>> { static constexpr bool value = true; };
+
+// Bytes of n consecutive elements.
+template <class KV>
+constexpr int kv_bytes(int n) {
+  if constexpr (IsInt4<KV>::value) return n / 2;
+  else return n * KV::bytes;
+}
 
 constexpr float kF16Max = 65504.0f;
 

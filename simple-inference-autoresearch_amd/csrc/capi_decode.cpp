@@ -66,16 +66,21 @@ int geometry(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, Geometry& g) {
 // Otherwise it keeps wide items: a page holds every KV head's 16 tokens side
 // by side and the waves of a wide item read them together; narrower items
 // that still leave a split ran config 2's main kernel 2-2.5 us (7%) slower.
-// int4 counts two work-groups per CU in place of one: a batch of 64 x 8 KV heads
-// takes items of one unit, and no piece of a sequence is left to merge.
-void item_units(Geometry& g, bool paged, bool int4) {
+//
+// int4 goes by the lengths instead, paged or not.  One shared length: the
+// halved IU (8 x 3000 tokens 16.7 us against 17.8, one sequence of 8192 13.9
+// against 18.3; 32/8 heads, D 128).  Lengths of their own: wide items, since
+// each of the many segments of a narrow split starts its ring anew (64 requests
+// of 100-8000 tokens 69.8 us at 8 units, 79.8 at 4, 90.1 at 2, 134.4 at 1; 16 of
+// up to 4096, 16/16 heads, D 64, 24.5, 33.9, 49.7, 76.9).
+void item_units(Geometry& g, bool paged, bool int4, bool ragged) {
   const int nw = decode_waves(g.D);
-  const int cus = (device_info().cus > 0 ? device_info().cus : 256) * (int4 ? 2 : 1);
+  const int cus = device_info().cus > 0 ? device_info().cus : 256;
   auto items = [&](int iu) { return (int64_t)g.B * ((g.U + iu - 1) / iu); };
   g.IU = g.U < nw ? g.U : nw;
   int iu = g.IU;
   while (iu % 2 == 0 && items(iu) < cus) iu /= 2;
-  if (!paged || items(iu) >= cus || g.B <= 4) g.IU = iu;
+  if (int4 ? !ragged : !paged || items(iu) >= cus || g.B <= 4) g.IU = iu;
   g.UB = (g.U + g.IU - 1) / g.IU;
 }
 
@@ -377,7 +382,7 @@ int decode_any(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, co
   int rc;
   if (k == nullptr) return fail(SIA_ERR_INVALID_ARGUMENT, "k is NULL");
   if ((rc = prepare_common(q, kv_len, out, (int)k->shape[1], sm_scale, g, L))) return rc;
-  item_units(g, bt != nullptr, k->dtype == SIA_U8);
+  item_units(g, bt != nullptr, k->dtype == SIA_U8, L.a.kv_per_seq != 0);
   L.a.IU = g.IU;
   L.a.UB = g.UB;
   if ((rc = prepare_kv(k, v, g, bt != nullptr, page_size, L))) return rc;

@@ -33,14 +33,25 @@ struct I4Tile {
   static constexpr int NM = NK < 4 ? NK : 4;              // groups per lane of the minima's operand
   static constexpr int KB = D / 8;                        // K bytes per lane: 4 lanes a token
   static constexpr int VB = D / 32;                       // V bytes per lane and token: 16 lanes a token
-  Raw<KB> k;               // token lane16: word j belongs to k-step j (int4.hpp)
-  Raw<4 * NM> km;          // token lane16: parameters of groups [4 (grp / 2), +4) (NK = 8), or of all
-  Raw<4 * NK> kp[4];       // tokens 4 grp + i: parameters of every group (step low, minimum high)
-  Raw<VB> v[4];            // tokens 4 grp + i: codes of the lane's share
-  Raw<4 * NV> vp[4];       // tokens 4 grp + i: parameters of its groups
+};
+template <int D, class KV>
+struct I4K {
+  using C = I4Tile<D, KV>;
+  Raw<C::KB> k;            // token lane16: word j belongs to k-step j (int4.hpp)
+  Raw<4 * C::NM> m;        // token lane16: parameters of groups [4 (grp / 2), +4) (NK = 8), or of all
+};
+template <int D, class KV>
+struct I4KP {
+  Raw<4 * I4Tile<D, KV>::NK> t[4];   // tokens 4 grp + i: parameters of every group (step low, minimum high)
+};
+template <int D, class KV>
+struct I4V {
+  using C = I4Tile<D, KV>;
+  Raw<C::VB> v[4];         // tokens 4 grp + i: codes of the lane's share
+  Raw<4 * C::NV> p[4];     // tokens 4 grp + i: parameters of its groups
 };
 
-// The ring of one wave: kStages tiles, each K codes, V codes, K parameters, V
+// The ring of one wave: kStages pairs of tiles, a tile K codes, V codes, K parameters, V
 // parameters.  Rows of codes are cut into 16-byte pieces, one lane of a
 // transfer each:
 //  * K rows in token order, the pieces of row r exchanged by r (piece c at
@@ -57,10 +68,11 @@ struct I4Ring {
   static constexpr int KI = D == 256 ? 2 : 1;             // transfers (of 64 pieces) per tensor
   static constexpr int PI = NK == 8 ? 2 : 1;              // transfers (of 64 words) of its parameters
   static constexpr int kV = 1024 * KI, kKP = 2 * kV, kVP = kKP + 256 * PI;
-  static constexpr int kStage = kVP + 256 * PI;
-  static constexpr int kStages = 3;
+  static constexpr int kTileBytes = kVP + 256 * PI;
+  static constexpr int kStage = 2 * kTileBytes;
+  static constexpr int kStages = D == 256 ? 2 : 3;
   static constexpr int kBytes = kStage * kStages;
-  static constexpr int kTransfers = 2 * (KI + PI);        // of a tile
+  static constexpr int kTransfers = 4 * (KI + PI);        // of a stage
   static __device__ __forceinline__ int swizzle(int r) {
     return D == 64 ? (r >> 3) & 1 : D == 128 ? (r >> 2) & 3 : (r >> 1) & 7;
   }
@@ -168,42 +180,53 @@ __device__ __forceinline__ void i4_read(Raw<BYTES>& r, const char* p) {
   }
 }
 template <int D, class KV>
-__device__ __forceinline__ void i4_read_k(const char* stage, const I4Lane<D, KV>& o, I4Tile<D, KV>& c) {
+__device__ __forceinline__ void i4_read_k(const char* tile, const I4Lane<D, KV>& o, I4K<D, KV>& c) {
   using C = I4Tile<D, KV>;
   if constexpr (D == 256) {     // pieces grp and grp + 4
-    const u32x4 x = *(const u32x4*)(stage + o.rk), y = *(const u32x4*)(stage + (o.rk ^ 64));
+    const u32x4 x = *(const u32x4*)(tile + o.rk), y = *(const u32x4*)(tile + (o.rk ^ 64));
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       c.k.w[j] = x[j];
       c.k.w[4 + j] = y[j];
     }
   } else {
-    i4_read<C::KB>(c.k, stage + o.rk);
+    i4_read<C::KB>(c.k, tile + o.rk);
   }
-  if constexpr (C::NK > 1) i4_read<4 * C::NM>(c.km, stage + o.rkm);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) i4_read<4 * C::NK>(c.kp[i], stage + o.rkp + 4 * C::NK * i);
+  if constexpr (C::NK > 1) i4_read<4 * C::NM>(c.m, tile + o.rkm);
 }
 template <int D, class KV>
-__device__ __forceinline__ void i4_read_v(const char* stage, const I4Lane<D, KV>& o, I4Tile<D, KV>& c) {
+__device__ __forceinline__ void i4_read_kp(const char* tile, const I4Lane<D, KV>& o, I4KP<D, KV>& c) {
   using C = I4Tile<D, KV>;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) i4_read<C::VB>(c.v[i], stage + o.rv + 64 * C::VB * i);
+  for (int i = 0; i < 4; ++i) i4_read<4 * C::NK>(c.t[i], tile + o.rkp + 4 * C::NK * i);
+}
+template <int D, class KV>
+__device__ __forceinline__ void i4_read_v(const char* tile, const I4Lane<D, KV>& o, I4V<D, KV>& c) {
+  using C = I4Tile<D, KV>;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) i4_read<4 * C::NV>(c.vp[i], stage + o.rvp + 4 * C::NK * i);
+  for (int i = 0; i < 4; ++i) i4_read<C::VB>(c.v[i], tile + o.rv + 64 * C::VB * i);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) i4_read<4 * C::NV>(c.p[i], tile + o.rvp + 4 * C::NK * i);
 }
 
 // The query of a unit: its MFMA operands, its sums over the groups and the
 // multiplier of a score.
+//
+// HALF: at most 8 heads, so the 16 columns hold them twice, and column c + 8
+// is head c for the second tile of a pair.  With the query zero in the other
+// tile's columns (op[0], op[1]), both tiles accumulate into one result, and the
+// softmax of a pair costs what that of one tile did.  (Head_dim 256 has no
+// registers for two operands and selects between two results.)
 template <int D, class KV>
 struct I4Query {
-  u32x4 op[D / 32];
-  u32x2 sums;     // NK > 1: operand of the minima's product, 2^-24 times the sums in two fp16 parts
+  static constexpr int N = KV::half && D <= 128 ? 2 : 1;
+  u32x4 op[N][D / 32];
+  u32x2 sums[N];  // NK > 1: operand of the minima's product, 2^-24 times the sums in two fp16 parts
   float sum;      // NK = 1: 2^-24 times the sum
   float mul;
 };
 template <int D, class KV, class QT>
-__device__ __forceinline__ void i4_prep_q(const DecodeArgs& a, QRaw<D>& raw, int grp, I4Query<D, KV>& q) {
+__device__ __forceinline__ void i4_prep_q(const DecodeArgs& a, QRaw<D>& raw, int lane16, int grp, I4Query<D, KV>& q) {
   constexpr int NK = I4Tile<D, KV>::NK, STEPS = D / 32, PER = STEPS / NK;
   // a power of two brings max |q| into [2^13, 2^14): fp16 operands without
   // overflow that lose bits only below 2^-24 of the maximum
@@ -236,7 +259,7 @@ __device__ __forceinline__ void i4_prep_q(const DecodeArgs& a, QRaw<D>& raw, int
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float f = (i & 1) ? 0.0625f : 1.0f;
-      q.op[j][i] = pack2(F16{}, x[i] * f, x[i + 4] * f);
+      q.op[0][j][i] = pack2(F16{}, x[i] * f, x[i + 4] * f);
     }
   }
 #pragma unroll
@@ -255,53 +278,105 @@ __device__ __forceinline__ void i4_prep_q(const DecodeArgs& a, QRaw<D>& raw, int
       const float hi = (float)(_Float16)f;
       x[i] = (grp & 1) ? f - hi : hi;
     }
-    q.sums = u32x2{pack2(F16{}, x[0], x[1]), pack2(F16{}, x[2], x[3])};
+    q.sums[0] = u32x2{pack2(F16{}, x[0], x[1]), pack2(F16{}, x[2], x[3])};
+  }
+  if constexpr (I4Query<D, KV>::N == 2) {
+    const uint32_t first = lane16 < 8 ? ~0u : 0u;
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) {
+      q.op[1][j] = q.op[0][j] & ~first;
+      q.op[0][j] &= first;
+    }
+    if constexpr (NK > 1) {
+      q.sums[1] = q.sums[0] & ~first;
+      q.sums[0] &= first;
+    }
   }
 }
 
-// Scores of tokens 4 grp + i for head lane16, before the multiplier.
+// acc + K Q over group g's k-steps of one tile.
 template <int D, class KV>
-__device__ __forceinline__ void i4_scores(const I4Tile<D, KV>& c, const I4Query<D, KV>& q, float (&s)[4]) {
-  constexpr int NK = I4Tile<D, KV>::NK, PER = KV::group / 32;
-  f32x4 t = {0.f, 0.f, 0.f, 0.f};
-  if constexpr (NK > 1) {
-    constexpr int NM = I4Tile<D, KV>::NM;
-    const u32x2 ma = {gather16(c.km.w[0], c.km.w[1], 1), NM == 4 ? gather16(c.km.w[NM - 2], c.km.w[NM - 1], 1) : 0u};
-    t = mfma16x16x16(F16{}, ma, q.sums, t);
-  }
+__device__ __forceinline__ f32x4 i4_qk(const I4K<D, KV>& c, const u32x4* op, int g, f32x4 acc) {
+  constexpr int PER = KV::group / 32;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) s[i] = NK == 1 ? hi_f32(F16{}, c.kp[i].w[0]) * q.sum : t[i];
+  for (int j = PER * g; j < PER * (g + 1); ++j) {
+    // codes (0, 4), (1, 5), (2, 6), (3, 7)
+    const uint32_t w = c.k.w[j], w8 = w >> 8;
+    const u32x4 ka = {w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u};
+    acc = mfma16x16x32(F16{}, ka, op[j], acc);
+  }
+  return acc;
+}
+// acc + the minima's product of one tile.
+template <int D, class KV>
+__device__ __forceinline__ f32x4 i4_qm(const I4K<D, KV>& c, u32x2 sums, f32x4 acc) {
+  constexpr int NM = I4Tile<D, KV>::NM;
+  const u32x2 ma = {gather16(c.m.w[0], c.m.w[NM > 1 ? 1 : 0], 1),
+                    NM == 4 ? gather16(c.m.w[NM == 4 ? 2 : 0], c.m.w[NM == 4 ? 3 : 0], 1) : 0u};
+  return mfma16x16x16(F16{}, ma, sums, acc);
+}
+// Scores of tokens 4 grp + i, before the multiplier: HALF, of the tile whose
+// columns the lane is in (kp: that tile's parameters), else of tile `t`.
+template <int D, class KV>
+__device__ __forceinline__ void i4_scores(const I4K<D, KV>* c, int t, const I4KP<D, KV>& kp, const I4Query<D, KV>& q,
+                                          int lane16, float (&s)[4]) {
+  constexpr int NK = I4Tile<D, KV>::NK;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  // x(tile, operand, start): one tile's product added to `start`
+  auto both = [&](auto&& x) -> f32x4 {
+    if constexpr (!KV::half) return x(t, 0, zero);
+    else if constexpr (I4Query<D, KV>::N == 2) return x(1, 1, x(0, 0, zero));
+    else {
+      const f32x4 u = x(0, 0, zero), v = x(1, 0, zero);
+      return lane16 < 8 ? u : v;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[i] = 0.f;
+  if constexpr (NK > 1) {
+    const f32x4 z = both([&](int ti, int qi, f32x4 acc) { return i4_qm<D, KV>(c[ti], q.sums[qi], acc); });
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = z[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = hi_f32(F16{}, kp.t[i].w[0]) * q.sum;
+  }
 #pragma unroll
   for (int g = 0; g < NK; ++g) {
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const f32x4 acc = both([&](int ti, int qi, f32x4 a0) { return i4_qk<D, KV>(c[ti], q.op[qi], g, a0); });
 #pragma unroll
-    for (int j = PER * g; j < PER * (g + 1); ++j) {
-      // codes (0, 4), (1, 5), (2, 6), (3, 7)
-      const uint32_t w = c.k.w[j], w8 = w >> 8;
-      const u32x4 ka = {w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u};
-      acc = mfma16x16x32(F16{}, ka, q.op[j], acc);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(lo_f32(F16{}, c.kp[i].w[g]), acc[i], s[i]);
+    for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(lo_f32(F16{}, kp.t[i].w[g]), acc[i], s[i]);
   }
 }
 
-// Online softmax of a tile's scores: weights p (the running maximum moves
-// lazily, as in compute_tile).
-template <int D>
-__device__ __forceinline__ void i4_softmax(const float (&s)[4], float mul, WaveState<D>& st, float (&p)[4]) {
-  const float lmax = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])) * mul;
+// Online softmax of NS x 4 scores per lane: weights p (the running maximum
+// moves lazily, as in compute_tile).  A score of -inf weighs 0, also before any
+// other was seen.
+template <int D, int NS>
+__device__ __forceinline__ void i4_softmax(const float (&s)[NS][4], float mul, bool masked, WaveState<D>& st,
+                                           float (&p)[NS][4]) {
+  float lmax = -INFINITY;
+#pragma unroll
+  for (int n = 0; n < NS; ++n) lmax = fmaxf(lmax, fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3])));
+  lmax *= mul;
   if (__any(lmax > st.m + kLazyMax)) {
     const float m_new = fmaxf(st.m, wave_max_xor16_32(lmax));
-    const float alpha = fast_exp2(st.m - m_new);
+    const float alpha = fast_exp2(st.m - (m_new == -INFINITY ? 0.f : m_new));
     st.m = m_new;
     st.l *= alpha;
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) st.acc[e] *= alpha;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) p[i] = fast_exp2(__builtin_fmaf(s[i], mul, -st.m));
-  st.l += (p[0] + p[1]) + (p[2] + p[3]);
+  for (int n = 0; n < NS; ++n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[n][i] = fast_exp2(__builtin_fmaf(s[n][i], mul, -st.m));
+    if (masked) {                  // (uniform)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[n][i] = s[n][i] == -INFINITY ? 0.f : p[n][i];
+    }
+    st.l += (p[n][0] + p[n][1]) + (p[n][2] + p[n][3]);
+  }
 }
 
 // Constants of the conversion, in registers: v_and_or_b32 takes no literal
@@ -317,39 +392,116 @@ struct I4Const {
   }
 };
 
-// O^T += V^T P^T.  d-tile e takes code e of every lane's share, for tokens
-// (4 grp, 4 grp + 1) and (4 grp + 2, 4 grp + 3).
+// O^T += V^T P^T over a pair of tiles.  d-tile e takes code e of every lane's
+// share, for tokens (4 grp, 4 grp + 1) and (4 grp + 2, 4 grp + 3) of either
+// tile.  pop: P in the same order, zero (HALF) in the other tile's columns.
 template <int D, class KV>
-__device__ __forceinline__ void i4_pv(const I4Tile<D, KV>& c, const I4Const& ic, const float (&p)[4],
-                                      WaveState<D>& st) {
+__device__ __forceinline__ void i4_pv(const I4V<D, KV>* c, const I4Const& ic, u32x4 pop, WaveState<D>& st) {
   using C = I4Tile<D, KV>;
-  const u32x2 pop = {pack2(F16{}, p[0], p[1]), pack2(F16{}, p[2], p[3])};
 #pragma unroll
   for (int h = 0; h < D / 64; ++h) {        // 4 codes of each token
     const int gv = C::NV == 2 ? h >> 1 : 0;
-    uint32_t x[2], x8[2];
-    f16x2 s[2], m[2];
+    uint32_t x[4], x8[4];
+    f16x2 s[4], m[4];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      x[t] = gather16(c.v[2 * t].w[h >> 1], c.v[2 * t + 1].w[h >> 1], h & 1);
+    for (int t = 0; t < 4; ++t) {
+      const I4V<D, KV>& v = c[t >> 1];
+      const int k = 2 * (t & 1);
+      x[t] = gather16(v.v[k].w[h >> 1], v.v[k + 1].w[h >> 1], h & 1);
       x8[t] = x[t] >> 8;
-      s[t] = __builtin_bit_cast(f16x2, gather16(c.vp[2 * t].w[gv], c.vp[2 * t + 1].w[gv], 0));
-      m[t] = __builtin_bit_cast(f16x2, gather16(c.vp[2 * t].w[gv], c.vp[2 * t + 1].w[gv], 1));
+      s[t] = __builtin_bit_cast(f16x2, gather16(v.p[k].w[gv], v.p[k + 1].w[gv], 0));
+      m[t] = __builtin_bit_cast(f16x2, gather16(v.p[k].w[gv], v.p[k + 1].w[gv], 1));
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      u32x2 va;
+      u32x4 va;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < 4; ++t) {
         const uint32_t w = e & 2 ? x8[t] : x[t];
         const _Float16 b = e & 1 ? (_Float16)-64.0f : (_Float16)-1024.0f;
         const uint32_t biased = e & 1 ? ((w & ic.hi) | ic.bhi) : ((w & ic.lo) | ic.blo);
         const f16x2 n = __builtin_bit_cast(f16x2, biased) + f16x2{b, b};
         va[t] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n, s[t], m[t]));
       }
-      st.acc[4 * h + e] = mfma16x16x16(F16{}, va, pop, st.acc[4 * h + e]);
+      st.acc[4 * h + e] = mfma16x16x32(F16{}, va, pop, st.acc[4 * h + e]);
     }
   }
+}
+
+// One pair of tiles: left0, left1 live tokens.
+template <int D, class KV>
+__device__ __forceinline__ void i4_pair(const char* stage, const I4Lane<D, KV>& o, const I4Const& ic,
+                                        const I4Query<D, KV>& q, int left0, int left1, int lane16, int grp,
+                                        WaveState<D>& st) {
+  using R = I4Ring<D, KV>;
+  constexpr int NS = KV::half ? 1 : 2;
+  const bool masked = left0 < kTile || left1 < kTile;
+  float s[NS][4], p[NS][4];
+  {
+    I4K<D, KV> k[2];
+    i4_read_k<D, KV>(stage, o, k[0]);
+    i4_read_k<D, KV>(stage + R::kTileBytes, o, k[1]);
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      I4KP<D, KV> kp;
+      i4_read_kp<D, KV>(stage + (KV::half ? (lane16 < 8 ? 0 : R::kTileBytes) : n * R::kTileBytes), o, kp);
+      i4_scores<D, KV>(k, n, kp, q, lane16, s[n]);
+    }
+  }
+  I4V<D, KV> v[2];
+  i4_read_v<D, KV>(stage, o, v[0]);
+  i4_read_v<D, KV>(stage + R::kTileBytes, o, v[1]);
+  if (masked) {
+    // (uniform) the wave's last pair.  Dead tokens weigh 0; their parameters
+    // are cleared too, so that the result never depends on what a dropped
+    // transfer leaves behind.
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int live = KV::half ? (lane16 < 8 ? left0 : left1) : n == 0 ? left0 : left1;
+        if (4 * grp + i >= live) s[n][i] = -INFINITY;
+      }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (4 * grp + i >= (t == 0 ? left0 : left1)) {
+#pragma unroll
+          for (int g = 0; g < I4Tile<D, KV>::NV; ++g) v[t].p[i].w[g] = 0u;
+        }
+  }
+  i4_softmax<D, NS>(s, q.mul, masked, st, p);
+  u32x4 pop;
+  if constexpr (KV::half) {
+    const u32x2 w = {pack2(F16{}, p[0][0], p[0][1]), pack2(F16{}, p[0][2], p[0][3])};
+    const uint32_t first = lane16 < 8 ? ~0u : 0u;
+    pop = u32x4{w[0] & first, w[1] & first, w[0] & ~first, w[1] & ~first};
+  } else {
+    pop = u32x4{pack2(F16{}, p[0][0], p[0][1]), pack2(F16{}, p[0][2], p[0][3]),
+                pack2(F16{}, p[NS - 1][0], p[NS - 1][1]), pack2(F16{}, p[NS - 1][2], p[NS - 1][3])};
+  }
+  i4_pv<D, KV>(v, ic, pop, st);
+}
+
+// HALF: the two tiles' states of a head, columns c and c + 8, added up.
+template <int D>
+__device__ __forceinline__ void i4_join(WaveState<D>& st) {
+  auto other = [](float x) {      // of lane16 ^ 8: a rotation by 8 inside each row of 16 lanes
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xf, 0xf, false));
+  };
+  const float m = fmaxf(st.m, other(st.m));
+  const float w = fast_exp2(st.m - (m == -INFINITY ? 0.f : m));
+  st.m = m;
+  st.l *= w;
+  st.l += other(st.l);
+#pragma unroll
+  for (int e = 0; e < D / 16; ++e)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = st.acc[e][i] * w;
+      st.acc[e][i] = x + other(x);
+    }
 }
 
 }  // namespace sia

@@ -659,11 +659,10 @@ template <int D, class KV, bool SV>
 struct DecodeWaves {
   static constexpr int value = D <= 64 && (!std::is_same<KV, I8>::value || SV) ? 4 : (D <= 128 ? 2 : 1);
 };
-// int4 holds one tile instead of two and fits twice as many waves, but for the
-// four parameter pairs per token of head_dim 128 in groups of 32, which spill.
-template <int D, int G, bool SV>
-struct DecodeWaves<D, I4G<G>, SV> {
-  static constexpr int value = D <= 128 ? 4 : 2;
+// int4: 15 KB of ring per wave leave 8 waves to a CU.
+template <int D, int G, bool HALF, bool SV>
+struct DecodeWaves<D, I4G<G, HALF>, SV> {
+  static constexpr int value = 2;
 };
 
 // Geometry of one item inside a work-group of NW waves (all uniform): it
@@ -707,11 +706,12 @@ void decode_main(const DecodeArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   // LDS: [acc: NW*G16*D f32, int4: the waves' rings][m: NW*G16][l: NW*G16][red: 2*NW+2 ints][pre: B+1 ints][lens: B ints, B <= kLensInLds]
   float* l_acc = (float*)smem;
-  // floats between the waves' parts of l_acc
-  int acc_wave;
-  if constexpr (IsInt4<KV>::value) acc_wave = i4_wave_lds<D, KV>(a.G16) / 4;
-  else acc_wave = a.G16 * D;
-  float* l_m = l_acc + NW * acc_wave;
+  // merge state of head column c of wave w (int4: inside the wave's ring)
+  auto acc_at = [&](int w, int c) {
+    if constexpr (IsInt4<KV>::value) return w * (i4_wave_lds<D, KV>(a.G16) / 4) + c * D;
+    else return (w * a.G16 + c) * D;
+  };
+  float* l_m = l_acc + acc_at(NW, 0);
   float* l_l = l_m + NW * a.G16;
   int* red = (int*)(l_l + NW * a.G16);
   int* pre = red + 2 * NW + 2;
@@ -902,8 +902,14 @@ void decode_main(const DecodeArgs a) {
         qraw = q_next;
         pg0 = pg_next;
       } else {
-        qraw = load_q_raw<D, KV>(a, b, hq, live, grp);
-        pg0 = kInt4 ? 0 : page_id(0);
+        if constexpr (i4_half<KV>()) {   // column c + 8 holds head c's query too
+          const int qc = lane16 & 7;
+          qraw = load_q_raw<D, KV>(a, b, qc < nh ? hkv * a.G + 16 * hg + qc : 0, qc < nh, grp);
+        } else {
+          qraw = load_q_raw<D, KV>(a, b, hq, live, grp);
+        }
+        if constexpr (kInt4) pg0 = 0;
+        else pg0 = page_id(0);
       }
       // the next segment of the share, if this wave has a unit there: its
       // query row and first page id (issued behind this segment's first tile)
@@ -954,56 +960,41 @@ void decode_main(const DecodeArgs a) {
         return tp;
       };
       if constexpr (kInt4) {
-        // Tiles through the wave's ring in LDS (see decode_i4.hpp), kStages - 1 of
-        // them in flight.
+        // Pairs of tiles through the wave's ring in LDS (see decode_i4.hpp),
+        // kStages - 1 of them in flight.
         if (nt > 0) {
           using R = I4Ring<D, KV>;
           const I4Lane<D, KV> il(a, lane);
           const I4Const ic;
           I4Query<D, KV> qi;
           char* ring = smem + wave * i4_wave_lds<D, KV>(a.G16);
+          const int np = (nt + 1) >> 1;
           auto left = [&](int k) { return k < nt ? ntok - (t_first + k * P) * kTile : 0; };   // live tokens of tile k
-          auto issue = [&](int k, int stage) {
-            const int kn = min(k, nt - 1);
-            const TilePtr tp = tile_ptr(t_first + kn * P, __builtin_amdgcn_readlane(pgw, kn & 63));
-            i4_issue<D, KV>(a, tp, il, left(k), ring + stage * R::kStage);
+          auto issue = [&](int pair, int stage) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int k = 2 * pair + i, kn = min(k, nt - 1);
+              const TilePtr tp = tile_ptr(t_first + kn * P, __builtin_amdgcn_readlane(pgw, kn & 63));
+              i4_issue<D, KV>(a, tp, il, left(k), ring + stage * R::kStage + i * R::kTileBytes);
+            }
           };
 #pragma unroll
           for (int k = 0; k < R::kStages - 1; ++k) issue(k, k);
-          i4_prep_q<D, KV, QT>(a, qraw, grp, qi);
-          int at = 0;                                    // stage of tile k
-          for (int k = 0; k < nt; ++k) {
+          i4_prep_q<D, KV, QT>(a, qraw, lane16, grp, qi);
+          int at = 0;                                    // stage of pair k
+          for (int k = 0; k < np; ++k) {
             const int kn = k + R::kStages - 1;
-            if ((kn & 63) == 0 && kn < nt) {
-              pgw = page_window(kn);
+            if ((kn & 31) == 0 && kn < np) {
+              pgw = page_window(2 * kn);
               asm volatile("" ::"v"(pgw));               // (waited for here, not by every round at its readlane)
             }
             issue(kn, at == 0 ? R::kStages - 1 : at - 1);
             i4_wait<(R::kStages - 1) * R::kTransfers>();
-            const char* stage = ring + at * R::kStage;
-            I4Tile<D, KV> c;
-            float s[4], p[4];
-            i4_read_k<D, KV>(stage, il, c);
-            i4_scores<D, KV>(c, qi, s);
-            i4_read_v<D, KV>(stage, il, c);
-            if (k >= nfull) {
-              // the sequence's partial last tile (uniform).  Its dead tokens
-              // weigh 0; their parameters are cleared too, so that the result
-              // never depends on what a dropped read leaves behind.
-              const int live_tok = left(k);
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (4 * grp + i >= live_tok) {
-                  s[i] = -INFINITY;
-#pragma unroll
-                  for (int g2 = 0; g2 < I4Tile<D, KV>::NV; ++g2) c.vp[i].w[g2] = 0u;
-                }
-            }
-            i4_softmax<D>(s, qi.mul, st, p);
-            i4_pv<D, KV>(c, ic, p, st);
+            i4_pair<D, KV>(ring + at * R::kStage, il, ic, qi, left(2 * k), left(2 * k + 1), lane16, grp, st);
             at = at + 1 == R::kStages ? 0 : at + 1;
           }
           i4_wait<0>();                                  // (the empty transfers too: the merge reuses the ring)
+          if constexpr (i4_half<KV>()) i4_join<D>(st);
         }
       } else {
       u32x4 qop[KSTEPS], qop_lo[KSTEPS];
@@ -1146,7 +1137,7 @@ void decode_main(const DecodeArgs a) {
       // states read one after the other and three runtime divisions each, took
       // 3.4 us of a 10.7 us group at one sequence of 1000 tokens.)
       if (live) {
-        float* dst = l_acc + wave * acc_wave + lane16 * D;
+        float* dst = l_acc + acc_at(wave, lane16);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1170,10 +1161,11 @@ void decode_main(const DecodeArgs a) {
           fDL x[PB];
 #pragma unroll
           for (int p2 = 0; p2 < PB; ++p2) {
-            const int wn = min(p0 + p2, w1), ws = wn * a.G16 + cc;
+            const int ws = min(p0 + p2, w1) * a.G16 + cc;
             mw[p2] = l_m[ws];
             lw[p2] = l_l[ws];
-            x[p2] = *(const fDL*)(l_acc + wn * acc_wave + cc * D + DL * lane);
+            if constexpr (IsInt4<KV>::value) x[p2] = *(const fDL*)(l_acc + acc_at(min(p0 + p2, w1), cc) + DL * lane);
+            else x[p2] = *(const fDL*)(l_acc + ws * D + DL * lane);
           }
           float mb = M;
 #pragma unroll

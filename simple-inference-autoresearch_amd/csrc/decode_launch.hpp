@@ -129,8 +129,11 @@ int launch_decode_q(DecodeLaunch& L) {
 // int4 K/V with groups of G elements at head_dim D (64, 128, 256).
 template <int D, int G>
 int launch_decode_i4_typed(DecodeLaunch& L) {
-  if (L.q_dtype == SIA_F16) return launch_decode_typed<D, I4G<G>, F16, F16>(L);
-  if (L.q_dtype == SIA_BF16) return launch_decode_typed<D, I4G<G>, BF16, F16>(L);
+  const bool half = L.a.G <= 8;
+  if (L.q_dtype == SIA_F16)
+    return half ? launch_decode_typed<D, I4G<G, true>, F16, F16>(L) : launch_decode_typed<D, I4G<G, false>, F16, F16>(L);
+  if (L.q_dtype == SIA_BF16)
+    return half ? launch_decode_typed<D, I4G<G, true>, BF16, F16>(L) : launch_decode_typed<D, I4G<G, false>, BF16, F16>(L);
   return fail(SIA_ERR_UNSUPPORTED, "query dtype must be float16 or bfloat16");
 }
 int launch_decode_i4(DecodeLaunch& L);       // decode_i4.hip

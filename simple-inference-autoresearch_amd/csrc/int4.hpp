@@ -32,11 +32,17 @@
 namespace sia {
 
 struct I4 { static constexpr int code = SIA_U8; };
-// The same with groups of G elements known to the compiler (the matrix kernels).
-template <int G>
-struct I4G { static constexpr int group = G; };
+// The same with groups of G elements known to the compiler (the matrix
+// kernels); HALF: at most 8 query heads share a KV head (decode_i4.hpp).
+template <int G, bool HALF>
+struct I4G { static constexpr int group = G; static constexpr bool half = HALF; };
 template <class KV> struct IsInt4 { static constexpr bool value = false; };
-template <int G> struct IsInt4<I4G<G>> { static constexpr bool value = true; };
+template <int G, bool HALF> struct IsInt4<I4G<G, HALF>> { static constexpr bool value = true; };
+template <class KV>
+constexpr bool i4_half() {
+  if constexpr (IsInt4<KV>::value) return KV::half;
+  else return false;
+}
 
 // Bytes of n consecutive elements.
 template <class KV>

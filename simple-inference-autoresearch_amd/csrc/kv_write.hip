@@ -1,6 +1,6 @@
 // KV write path for gfx950: store new K/V tokens into a contiguous cache or a
-// paged pool, quantising on the way to int8 with per-token-per-head scales or
-// to 4 bits with a step and a minimum per group (int4.hpp).
+// paged pool, quantising to int8 with per-token-per-head scales on the way
+// when the destination is int8 (4 bits: kv_write_i4.hip).
 //
 // Semantics follow the reference engine:
 //  * quantize_kv_int8 (model/kv_cache.py:58-67): amax = max |x| over head_dim,
@@ -28,46 +28,11 @@
 // capacity, page id outside the pool) are skipped: the kernel never writes
 // outside the buffers it was given.
 #include "host_util.hpp"
-#include "int4.hpp"
 #include "kv_rows.hpp"
 #include "kv_write.hpp"
 #include "sia_common.hpp"
 
 namespace sia {
-
-// N (4 or 8) consecutive table values of dtype C from element j0 of `row`
-// (a 16-byte aligned chunk: the host requires aligned tables).
-template <class C, int N>
-__device__ __forceinline__ void tab_n(const char* row, int j0, float* c) {
-  if constexpr (std::is_same<C, F32>::value) {
-    const f32x4 a = *(const f32x4*)(row + j0 * 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = a[i];
-    if constexpr (N == 8) {
-      const f32x4 b = *(const f32x4*)(row + j0 * 4 + 16);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) c[4 + i] = b[i];
-    }
-  } else {
-    uint32_t w[N / 2];
-    if constexpr (N == 8) {
-      const u32x4 v = *(const u32x4*)(row + j0 * 2);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = v[i];
-    } else {
-      const u32x2 v = *(const u32x2*)(row + j0 * 2);
-      w[0] = v[0]; w[1] = v[1];
-    }
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i) { c[2 * i] = lo_f32(C{}, w[i]); c[2 * i + 1] = hi_f32(C{}, w[i]); }
-  }
-}
-
-// Round a float to the source dtype (the rotated row is stored in that dtype
-// before it is quantised or cast, as a separate RoPE pass would store it).
-template <class S> __device__ __forceinline__ float to_src(float x) { return x; }
-template <> __device__ __forceinline__ float to_src<F16>(float x) { return (float)(_Float16)x; }
-template <> __device__ __forceinline__ float to_src<BF16>(float x) { return (float)(__bf16)x; }
 
 // Rotate this lane's 8 elements of a K row (lane `part` of the row's `width`
 // lanes holds elements [8 part, 8 part + 8)) by table row `pos` (already
@@ -104,115 +69,10 @@ __device__ __forceinline__ void rope8(float (&x)[8], int part, int width, const 
   }
 }
 
-// x / s correctly rounded, from inv = RN(1/s): q0 = RN(x inv) is within one
-// ulp of x/s, r = x - q0 s is exact under an FMA, and RN(q0 + r inv) is the
-// correctly rounded quotient (Markstein's correction step) while the scale
-// stays a normal number, which the amax floor guarantees.  Three VALU
-// operations per element instead of a full division; checked against the
-// correctly rounded division for every bf16 and fp16 (x, amax) pair and for
-// sampled fp32 pairs (tests/test_quant_division.py).
-__device__ __forceinline__ float div_by_scale(float x, float s, float inv) {
-#pragma clang fp contract(off)
-  const float q0 = x * inv;
-  const float r = __builtin_fmaf(-q0, s, x);
-  return __builtin_fmaf(r, inv, q0);
-}
-
 // Max over the `width` lanes of a row group (width = D/8 <= 32, power of two).
 __device__ __forceinline__ float group_max(float x, int width) {
   for (int o = width >> 1; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
   return x;
-}
-
-// This lane's 8 elements of a row as 4-bit codes (one word), and in `sm` its
-// group's parameters (s low, m high); see int4.hpp.  `gl` lanes (a power of
-// two, at most 16) hold a group.  Every lane of the wave calls this.
-__device__ __forceinline__ uint32_t quantise8_i4(float (&x)[8], int gl, uint32_t& sm) {
-#pragma clang fp contract(off)
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    bad |= !(fabsf(x[i]) <= 3.402823466e38f);
-    x[i] = __builtin_amdgcn_fmed3f(x[i], -kF16Max, kF16Max);
-  }
-  float lo = x[0], hi = x[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-  }
-  for (int o = gl >> 1; o > 0; o >>= 1) {
-    lo = fminf(lo, __shfl_xor(lo, o));
-    hi = fmaxf(hi, __shfl_xor(hi, o));
-  }
-  const int lane = threadIdx.x & 63;
-  const uint64_t group = ((1ull << gl) - 1ull) << (lane & ~(gl - 1));
-  const bool poison = (__ballot(bad) & group) != 0;
-  const float m = (float)(_Float16)lo;
-  const float step = fmaxf(__fdiv_rn(hi - m, 15.0f), 0.0f);
-  const uint32_t sbits = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(step, lo)) & 0xffffu;
-  const float s = lo_f32(F16{}, sbits);
-  const float inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;    // (s = 0: every code is 0)
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float n = __builtin_amdgcn_fmed3f(__builtin_rintf(div_by_scale(x[i] - m, s, inv)), 0.0f, 15.0f);
-    w |= (uint32_t)n << (4 * i);
-  }
-  sm = poison ? 0x7e007e00u : sbits | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) << 16);
-  return poison ? 0u : w;
-}
-
-// The q part of a RoPE write: one work-group per token (b, t); a work item is
-// 8 pairs of one query head, read and written with 16-byte accesses (both
-// halves of a split-half pair, or 16 consecutive elements of interleaved
-// pairs, in the same thread).  A token whose position lies outside the table
-// is written as zeros.  Loads are unconditional (a position outside the
-// table reads row 0 and the result is then zeroed), so no branch sits
-// between a load and its use.
-template <class S, class C, int ROPE>
-__device__ __forceinline__ void rope_q_token(const KvWriteArgs& a, uint32_t token) {
-  constexpr int ES = S::bytes;
-  const uint32_t b = token / (uint32_t)a.T, t = token - b * (uint32_t)a.T;
-  const int pos = (int)t + a.start_host + (a.start ? a.start[a.start_per_seq ? b : 0] : 0);
-  const bool tab_ok = pos >= 0 && pos < a.Tc;
-  const int half = a.D >> 1;
-  const int per_head = half >> 3;
-  const int items = a.Hq * per_head;
-  const char* qrow = a.q + (int64_t)b * a.q_sb + (int64_t)t * a.q_st;
-  char* orow = a.qo + (int64_t)b * a.qo_sb + (int64_t)t * a.qo_st;
-  const char* crow = a.cs + (int64_t)(tab_ok ? pos : 0) * a.tab_rs;
-  const char* srow = a.sn + (int64_t)(tab_ok ? pos : 0) * a.tab_rs;
-  for (int it = threadIdx.x; it < items; it += 256) {
-    const int h = it / per_head;
-    const int i0 = (it - h * per_head) * 8;
-    const char* src = qrow + (int64_t)h * a.q_sh;
-    char* dst = orow + (int64_t)h * a.qo_sh;
-    float c[8], s[8], x0[8], x1[8];
-    // split-half: x0 = elements [i0, i0+8), x1 = [i0+half, ...); interleaved: 16 consecutive
-    const int o0 = ROPE == 1 ? i0 : 2 * i0;
-    const int o1 = ROPE == 1 ? i0 + half : 2 * i0 + 8;
-    load8<S>(src + o0 * ES, x0);
-    load8<S>(src + o1 * ES, x1);
-    tab_n<C, 8>(crow, i0, c);
-    tab_n<C, 8>(srow, i0, s);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      c[i] = tab_ok ? c[i] : 0.f;
-      s[i] = tab_ok ? s[i] : 0.f;
-    }
-    if constexpr (ROPE == 1) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) rope_rotate(x0[i], x1[i], c[i], s[i], x0[i], x1[i]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) rope_rotate(x0[2 * j], x0[2 * j + 1], c[j], s[j], x0[2 * j], x0[2 * j + 1]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) rope_rotate(x1[2 * j], x1[2 * j + 1], c[4 + j], s[4 + j], x1[2 * j], x1[2 * j + 1]);
-    }
-    store8<S>(dst + o0 * ES, x0);
-    store8<S>(dst + o1 * ES, x1);
-  }
 }
 
 // K/V part: rows are (b, kv head, token).  Loads are unconditional: a row past
@@ -278,15 +138,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const KvWriteArgs a) {
         for (int i = 0; i < 8; ++i) x[i] = to_src<S>(x[i]);
       }
     }
-    if constexpr (std::is_same<DT, I4>::value) {
-      uint32_t sm;
-      const uint32_t w = quantise8_i4(x, 1 << (a.lg_group - 3), sm);
-      if (store) {
-        *(uint32_t*)(dst + dst_row + 4 * i4_place(part, a.D)) = w;
-        const int first = part & ((1 << (a.lg_group - 3)) - 1);
-        if (first == 0) *(uint32_t*)(sdst + sc_row + 4 * (part >> (a.lg_group - 3))) = sm;
-      }
-    } else if constexpr (std::is_same<DT, I8>::value) {
+    if constexpr (std::is_same<DT, I8>::value) {
       float m = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
@@ -327,7 +179,6 @@ static int launch_dst(const KvWriteArgs& a, int dst_dtype, hipStream_t stream) {
     case SIA_BF16: hipLaunchKernelGGL((kv_write_kernel<S, BF16, C, ROPE>), grid, dim3(256), 0, stream, a); break;
     case SIA_F32: hipLaunchKernelGGL((kv_write_kernel<S, F32, C, ROPE>), grid, dim3(256), 0, stream, a); break;
     case SIA_I8: hipLaunchKernelGGL((kv_write_kernel<S, I8, C, ROPE>), grid, dim3(256), 0, stream, a); break;
-    case SIA_U8: hipLaunchKernelGGL((kv_write_kernel<S, I4, C, ROPE>), grid, dim3(256), 0, stream, a); break;
     default: return fail(SIA_ERR_UNSUPPORTED, "destination dtype %s not supported", dtype_name(dst_dtype));
   }
   const hipError_t e = hipGetLastError();
@@ -354,6 +205,7 @@ static int launch_src(const KvWriteArgs& a, int dst_dtype, hipStream_t stream) {
 }
 
 int launch_kv_write(const KvWriteArgs& a_in, int src_dtype, int dst_dtype, hipStream_t stream) {
+  if (dst_dtype == SIA_U8) return launch_kv_write_i4(a_in, src_dtype, stream);
   KvWriteArgs a = a_in;
   const int width = a.D / 8;
   if (a.rows * width + 255 > 0x7fffffff || (int64_t)a.B * a.T > 0x7fffffff)

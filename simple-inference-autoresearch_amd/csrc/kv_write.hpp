@@ -25,7 +25,6 @@ struct KvWriteArgs {
   int32_t ntensors;
   int32_t scale_f32;
   float amax_floor;                       // 1e-8 rounded to the source dtype
-  int32_t lg_group;                       // int4 destinations: log2 of the elements per (step, minimum) pair
   // rotary embedding of K (and q) on the way in; rope == 0 leaves the rows as they are
   int32_t rope;                           // 0 none, 1 split-half pairs (i, i + D/2), 2 interleaved (2i, 2i + 1)
   const char* cs; const char* sn;         // cos / sin tables (Tc, >= D/2), read at row `position`
@@ -40,9 +39,14 @@ struct KvWriteArgs {
   uint32_t kv_blocks;                     // work-groups of the K/V part; the q part (one per token) follows
   int32_t log2_width;                     // log2(D / 8): lanes per row
   int32_t h_fast;                         // rows ordered (b, t, h) instead of (b, h, t)
+  // int4 destinations (kv_write_i4.hip)
+  int32_t lg_group;                       // log2 of the elements per (step, minimum) pair
+  int32_t lg_chunk;                       // rows ordered (b, t >> lg_chunk, h, the low bits of t)
+  FastDiv dH, dchunks, dpage;             // divisions by H, by the chunks of T and by the page size
 };
 
 int launch_kv_write(const KvWriteArgs& a, int src_dtype, int dst_dtype, hipStream_t stream);
+int launch_kv_write_i4(const KvWriteArgs& a, int src_dtype, hipStream_t stream);
 
 // Host/device description of one KV read (see kv_read.hip).
 struct KvReadArgs {

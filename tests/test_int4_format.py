@@ -151,3 +151,26 @@ def test_python_refusals():
     assert c.k_cache.shape == (2, 3, 4, 20, 64) and c.v_scale.shape == (2, 3, 4, 20, 8) and c.is_quantized
     p = pkg.PagedKVCache(2, 3, 40, 4, 16, device="cpu", kv_dtype="int4")
     assert p.k_pool.shape == (2, 9, 4, 16, 8) and p.k_scale_pool.shape == (2, 9, 4, 16, 2)
+
+
+def test_reciprocal_of_every_step():
+    """1 / s from a reciprocal within one ulp (v_rcp_f32) and one Newton step under FMAs is correctly rounded, and x / s
+    from it (three more instructions) too, for every positive fp16 s: the write kernel's arithmetic."""
+    f, d = np.float32, np.float64
+    s = np.arange(1, 0x7C00, dtype=np.uint16).view(np.float16).astype(f)
+    want = (d(1) / s.astype(d)).astype(f)
+    for off in (-1, 0, 1):
+        r = (want.view(np.int32) + off).view(f)
+        # (an fp32 product of two fp32 numbers is exact in fp64, and so are the sums here up to one fp64 rounding, far
+        # below the fp32 rounding that follows)
+        e = (d(1) - s.astype(d) * r.astype(d)).astype(f)
+        inv = (e.astype(d) * r.astype(d) + r.astype(d)).astype(f)
+        np.testing.assert_array_equal(inv, want)
+    rng = np.random.default_rng(0)
+    for _ in range(20):
+        x = (rng.standard_normal(s.size) * s * 8).astype(f)
+        x[::3] = (s[::3] * (rng.integers(0, 16, x[::3].size) + 0.5)).astype(f)          # ties
+        q0 = (x.astype(d) * want.astype(d)).astype(f)
+        r = (x.astype(d) - q0.astype(d) * s.astype(d)).astype(f)
+        q = (r.astype(d) * want.astype(d) + q0.astype(d)).astype(f)
+        np.testing.assert_array_equal(q, (x.astype(d) / s.astype(d)).astype(f))

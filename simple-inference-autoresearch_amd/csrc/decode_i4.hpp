@@ -116,10 +116,9 @@ struct I4Lane {
 };
 
 // A tile is transferred through buffer descriptors that end behind its last
-// live token: the range check drops the reads behind it (they fill zeros) and,
-// for a tile without live tokens (behind a wave's last one), all of them, so
-// every round of the loop issues the same number of transfers and its wait is
-// a constant.
+// live token: the range check drops the reads behind it (they fill zeros), and
+// all of them for the second tile of a pair that has none, so every pair is
+// the same number of transfers and every wait a constant.
 __device__ __forceinline__ uint32_t i4_range(uint32_t tok, int row, int valid) {
   const uint32_t n = (uint32_t)(min(valid, kTile) - 1) * tok + (uint32_t)row;
   return valid > 0 ? n : 0u;

@@ -716,6 +716,13 @@ void decode_main(const DecodeArgs a) {
   int* red = (int*)(l_l + NW * a.G16);
   int* pre = red + 2 * NW + 2;
 
+  // Every line of the arguments is asked for at once: they lie in host memory,
+  // and the compiler reads a field where it is first needed, one round trip
+  // each.
+  if constexpr (IsInt4<KV>::value) {
+    asm volatile("" ::"s"(a.q), "s"(a.k), "s"(a.v), "s"(a.ks), "s"(a.vs), "s"(a.bt), "s"(a.kv_len), "s"(a.dHG.m),
+                 "s"(a.ws_acc), "s"(a.k_pg), "s"(a.cus));
+  }
   const ItemShape shape = item_shape<NW>(a);
   // The work line (every work-group computes the same prefix) and its
   // stream-K split: group g takes an equal contiguous share, so groups finish
@@ -892,6 +899,7 @@ void decode_main(const DecodeArgs a) {
       constexpr bool kPartFirst = D > 64 && !(D == 256 && QSplit<KV, QT>::value) && !kInt4;   // (see below)
       // int4: lane l holds the page id of the wave's tile k0 + l, 64 tiles by one load
       auto page_window = [&](int k0) {
+        if (!paged) return 0;      // (nothing to wait for)
         const int t = t_first + max(0, min(k0 + lane, nt - 1)) * P;
         return btrow[(int64_t)(min(t, cap_tiles - 1) >> a.lg_tiles_per_page) * bt_step];
       };
@@ -978,8 +986,10 @@ void decode_main(const DecodeArgs a) {
               i4_issue<D, KV>(a, tp, il, left(k), ring + stage * R::kStage + i * R::kTileBytes);
             }
           };
+          issue(0, 0);
 #pragma unroll
-          for (int k = 0; k < R::kStages - 1; ++k) issue(k, k);
+          for (int k = 1; k < R::kStages - 1; ++k)
+            if (k < np) issue(k, k);
           i4_prep_q<D, KV, QT>(a, qraw, lane16, grp, qi);
           int at = 0;                                    // stage of pair k
           for (int k = 0; k < np; ++k) {
@@ -988,12 +998,17 @@ void decode_main(const DecodeArgs a) {
               pgw = page_window(2 * kn);
               asm volatile("" ::"v"(pgw));               // (waited for here, not by every round at its readlane)
             }
-            issue(kn, at == 0 ? R::kStages - 1 : at - 1);
-            i4_wait<(R::kStages - 1) * R::kTransfers>();
+            if (kn < np) {
+              issue(kn, at == 0 ? R::kStages - 1 : at - 1);
+              i4_wait<(R::kStages - 1) * R::kTransfers>();
+            } else if (R::kStages > 2 && k + 1 < np) {   // (one pair behind this one)
+              i4_wait<R::kTransfers>();
+            } else {
+              i4_wait<0>();
+            }
             i4_pair<D, KV>(ring + at * R::kStage, il, ic, qi, left(2 * k), left(2 * k + 1), lane16, grp, st);
             at = at + 1 == R::kStages ? 0 : at + 1;
           }
-          i4_wait<0>();                                  // (the empty transfers too: the merge reuses the ring)
           if constexpr (i4_half<KV>()) i4_join<D>(st);
         }
       } else {
@@ -1138,10 +1153,19 @@ void decode_main(const DecodeArgs a) {
       // 3.4 us of a 10.7 us group at one sequence of 1000 tokens.)
       if (live) {
         float* dst = l_acc + acc_at(wave, lane16);
+        if constexpr (kInt4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int e = 0; e < E; ++e) dst[out_d<D, KV>(grp, i, e)] = st.acc[e][i] * unscale;
+            for (int e = 0; e < E; e += 4)
+              *(f32x4*)(dst + out_d<D, KV>(grp, i, e)) =
+                  f32x4{st.acc[e][i], st.acc[e + 1][i], st.acc[e + 2][i], st.acc[e + 3][i]};
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < E; ++e) dst[out_d<D, KV>(grp, i, e)] = st.acc[e][i] * unscale;
+        }
       }
       if (lane16 < a.G16 && grp == 0) {
         l_m[wave * a.G16 + lane16] = live ? st.m : -INFINITY;

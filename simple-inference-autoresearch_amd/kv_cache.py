@@ -69,28 +69,9 @@ def kv_read(k_src: torch.Tensor, v_src: torch.Tensor | None, length: int, k_scal
     strides, 16-byte aligned rows).  Returns ``(k, v)``; ``v`` is None when
     ``v_src`` is.
     """
-    ops = _lib.gpu_ops()
-    length = int(length)
-    if k_src.dim() != 4:
-        raise ValueError("k_src must have 4 dims")
-    if length < 0:
-        raise ValueError("length must not be negative")
-    quantised = k_src.dtype in (torch.int8, torch.uint8)
-    D = k_src.shape[3] * (2 if k_src.dtype == torch.uint8 else 1)
-    B = block_table.shape[0] if block_table is not None else k_src.shape[0]
-    shape = (B, k_src.shape[1], length, D)
-    if out is None:
-        dt = dtype or (torch.bfloat16 if quantised else k_src.dtype)
-        k = torch.empty(shape, dtype=dt, device=k_src.device)
-        v = torch.empty(shape, dtype=dt, device=k_src.device) if v_src is not None else None
-    else:
-        k, v = out
-        if dtype not in (None, k.dtype):
-            raise ValueError("dtype differs from out's")
-        if tuple(k.shape) != shape or (v is None) != (v_src is None):
-            raise ValueError(f"out must be a (k, v) pair of shape {shape}, v None exactly where v_src is")
-    ops.kv_read(k_src, v_src, k_scale, v_scale, block_table, start_pos, int(start_offset), int(page_size), k, v)
-    return k, v
+    ko, vo = (None, None) if out is None else out
+    return _lib.gpu_ops().kv_read(k_src, v_src, length, k_scale, v_scale, block_table, start_pos, start_offset,
+                                  page_size, dtype, ko, vo)
 
 
 def rope_kv_write(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor | None, cos: torch.Tensor,

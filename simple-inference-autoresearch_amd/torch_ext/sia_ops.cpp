@@ -376,17 +376,43 @@ Tensor dequantize_kv_int4(const Tensor& codes, const Tensor& params, at::ScalarT
   return out;
 }
 
-// Positions [start, start + T) of a cache or pool into k_out / v_out (B, H, T, D).
-void kv_read(const Tensor& k_src, const OptT& v_src, const OptT& k_scale, const OptT& v_scale, const OptT& block_table,
-             const OptT& start_pos, int64_t start_offset, int64_t page_size, const Tensor& k_out, const OptT& v_out) {
+// Positions [start, start + length) of a cache or pool as (B, H, length, D)
+// tensors of `dtype`, or into the caller's k_out / v_out.
+std::tuple<Tensor, OptT> kv_read(const Tensor& k_src, const OptT& v_src, int64_t length, const OptT& k_scale,
+                                 const OptT& v_scale, const OptT& block_table, const OptT& start_pos,
+                                 int64_t start_offset, int64_t page_size, std::optional<at::ScalarType> dtype,
+                                 const OptT& k_out, const OptT& v_out) {
   const at::Device dev = gpu_of(k_src, "k_src");
   const c10::DeviceGuard guard(dev);
-  if (k_out.numel() == 0 && k_out.dim() == 4) return;   // no tokens to read
-  const sia_tensor dk = desc(k_src, dev, "k_src"), dko = desc(k_out, dev, "k_out");
+  if (k_src.dim() != 4) throw py::value_error("k_src must have 4 dims");
+  if (length < 0) throw py::value_error("length must not be negative");
+  const at::ScalarType st = k_src.scalar_type();
+  const bool int4 = st == at::kByte, quantised = int4 || st == at::kChar;
+  if (block_table.has_value() && block_table->dim() != 2)
+    throw py::value_error("block_table must be a (B, max_blocks) int32 tensor");
+  const int64_t B = block_table.has_value() ? block_table->size(0) : k_src.size(0);
+  const int64_t D = k_src.size(3) * (int4 ? 2 : 1);
+  const std::vector<int64_t> shape = {B, k_src.size(1), length, D};
+  Tensor k;
+  OptT v;
+  if (k_out.has_value()) {
+    k = *k_out;
+    v = v_out;
+    if (dtype.has_value() && *dtype != k.scalar_type()) throw py::value_error("dtype differs from out's");
+    if (k.sizes() != shape || v.has_value() != v_src.has_value() || (v.has_value() && v->sizes() != shape))
+      throw py::value_error("out must be a (k, v) pair of shape (B, H, length, D), v None exactly where v_src is");
+  } else {
+    const auto opts = k_src.options().dtype(dtype.has_value() ? *dtype : quantised ? at::kBFloat16 : st);
+    k = at::empty(shape, opts);
+    if (v_src.has_value()) v = at::empty(shape, opts);
+  }
+  if (k.numel() == 0) return {k, v};   // no tokens to read
+  const sia_tensor dk = desc(k_src, dev, "k_src"), dko = desc(k, dev, "k_out");
   const OptDesc dv(v_src, dev, "v_src"), dks(k_scale, dev, "k_scale"), dvs(v_scale, dev, "v_scale"),
-      dbt(block_table, dev, "block_table"), dsp(start_pos, dev, "start_pos"), dvo(v_out, dev, "v_out");
+      dbt(block_table, dev, "block_table"), dsp(start_pos, dev, "start_pos"), dvo(v, dev, "v_out");
   check(sia_kv_read(&dk, dv.ptr(), dks.ptr(), dvs.ptr(), dbt.ptr(), dsp.ptr(), (int32_t)start_offset,
                     (int32_t)page_size, &dko, dvo.ptr(), stream_of(dev)));
+  return {k, v};
 }
 
 void kv_write(const Tensor& k, const OptT& v, const Tensor& k_dst, const OptT& v_dst, const OptT& k_scale_dst,

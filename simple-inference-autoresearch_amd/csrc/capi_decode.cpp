@@ -271,9 +271,9 @@ int prepare_workspace(void* ws, size_t bytes, const Geometry& g, const sia_decod
     L.begin_event = (hipEvent_t)opts->main_begin_event;
     L.end_event = (hipEvent_t)opts->main_end_event;
   }
-  // the work line (B x (tiles + the split's segment charge, at most 4) x unit
-  // blocks) is indexed with 32-bit integers
-  if ((int64_t)g.B * ((L.a.cap_tokens + kTile - 1) / kTile + 4) * g.UB > 0x7fffffffLL)
+  // the work line (B x (tiles + the split's segment charge, at most 4, int4 8)
+  // x unit blocks) is indexed with 32-bit integers
+  if ((int64_t)g.B * (((int64_t)L.a.cap_tokens + kTile - 1) / kTile + (L.lg_group > 0 ? 8 : 4)) * g.UB > 0x7fffffffLL)
     return fail(SIA_ERR_UNSUPPORTED, "batch x cache capacity too large (more than 2^31 tiles of work)");
   const size_t pb = plan_bytes(g.B);
   const size_t ib = item_bytes(g);
@@ -406,7 +406,8 @@ int decode_any(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, co
   // other than 16 * 2^k) go to the vector-ALU path with its per-token lookup
   const bool tiled_pages = bt == nullptr || (kTile << L.a.lg_tiles_per_page) == page_size;
   // (int4 at head_dim 16 and 32 too: a row there is a fraction of a k-step)
-  if (q->dtype == SIA_F32 || k->dtype == SIA_F32 || !tiled_pages || (k->dtype == SIA_U8 && g.D < 64)) return dispatch_f32(L, g, k->dtype, out);
+  if (q->dtype == SIA_F32 || k->dtype == SIA_F32 || !tiled_pages || (k->dtype == SIA_U8 && g.D < 64))
+    return dispatch_f32(L, g, k->dtype, out);
   return dispatch(L, k->dtype);
 }
 

@@ -49,9 +49,12 @@ int launch_decode_typed(DecodeLaunch& L) {
   // The split charges every segment start this many virtual tiles: starting
   // a segment costs about four dependent memory round trips (its length and
   // query, its first page id, its first tile), about two tiles of streaming
-  // time for 16-bit K/V and three for int8.  Equal lengths keep their shares
-  // aligned to sequence boundaries whatever the charge.
-  L.a.seg_pen = std::is_same<KV, I8>::value ? 3 : 2;
+  // time for 16-bit K/V, three for int8 and six for 4 bits (16 sequences of
+  // 256 to 4096 tokens, 32/8 heads: head_dim 64 16.9 us against 19.5 with two
+  // and 17.5 with twelve, head_dim 128 22.5 against 24.9 and 22.8).  Equal
+  // lengths keep their shares aligned to sequence boundaries whatever the
+  // charge.
+  L.a.seg_pen = std::is_same<KV, I8>::value ? 3 : IsInt4<KV>::value ? 6 : 2;
   int lg = 0;
   while ((2 << lg) <= NW / L.a.IU) ++lg;
   L.a.lgP = lg;

@@ -93,6 +93,14 @@ __device__ __forceinline__ float row_sum(float d) {
   return d;
 }
 
+// s scale - m with the product rounded as the maximum's was: at most 0, however
+// large the scores.
+__device__ __forceinline__ float score_above(float s, float scale, float m) {
+#pragma clang fp contract(off)
+  const float x = s * scale;
+  return x - m;
+}
+
 template <int D, class QT, class KV, class ST>
 __global__ __launch_bounds__(256) void attn_f32(const F32Args a) {
   constexpr int LPT = D / 4;            // lanes per key row
@@ -210,7 +218,9 @@ __global__ __launch_bounds__(256) void attn_f32(const F32Args a) {
       f32x4 pv = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float p = fast_exp2(__builtin_fmaf(sc[u], a.qk_scale, -mu));   // (one rounding for both)
+        float p;
+        if constexpr (kInt4) p = fast_exp2(score_above(sc[u], a.qk_scale, mu));
+        else p = fast_exp2(__builtin_fmaf(sc[u], a.qk_scale, -mu));   // (one rounding for both)
         psum += p;
         pv += (p * vsc[u]) * vv[u];
       }

@@ -219,8 +219,12 @@ __device__ __forceinline__ void i4_read_v(const char* tile, const I4Lane<D, KV>&
 template <int D, class KV>
 struct I4Query {
   static constexpr int N = KV::half && D <= 128 ? 2 : 1;
+  // |sum| <= 128 x 2^14 in fp16's range, and far above its denormals: the two
+  // parts hold 22 bits of it.  (With the codes' 2^-24, which needs no product
+  // to join the two, the lower part ends at 2^-14 of the largest |q|, times m.)
+  static constexpr float kSums = 0x1p-6f;
   u32x4 op[N][D / 32];
-  u32x2 sums[N];  // NK > 1: operand of the minima's product, 2^-24 times the sums in two fp16 parts
+  u32x2 sums[N];  // NK > 1: operand of the minima's product, kSums times the sums in two fp16 parts
   float sum;      // NK = 1: 2^-24 times the sum
   float mul;
 };
@@ -241,7 +245,9 @@ __device__ __forceinline__ void i4_prep_q(const DecodeArgs& a, QRaw<D>& raw, int
     }
   amax = wave_max_xor16_32(amax);
   const int sh = amax > 0.f ? 14 - __builtin_amdgcn_frexp_expf(amax) : 0;
-  q.mul = ldexpf(a.qk_scale, 24 - sh);
+  // (2^100 for queries beyond 2^93: with more the score of two different keys
+  // differs by far more than the softmax resolves, and the multiplier overflows)
+  q.mul = fminf(ldexpf(a.qk_scale, 24 - sh), 0x1p100f);
   float sum[NK];
 #pragma unroll
   for (int j = 0; j < STEPS; ++j) {
@@ -262,7 +268,7 @@ __device__ __forceinline__ void i4_prep_q(const DecodeArgs& a, QRaw<D>& raw, int
     }
   }
 #pragma unroll
-  for (int g = 0; g < NK; ++g) sum[g] = wave_sum_xor16_32(sum[g]) * 0x1p-24f;
+  for (int g = 0; g < NK; ++g) sum[g] = wave_sum_xor16_32(sum[g]) * (NK == 1 ? 0x1p-24f : I4Query<D, KV>::kSums);
   if constexpr (NK == 1) {
     q.sum = sum[0];
   } else {
@@ -331,21 +337,31 @@ __device__ __forceinline__ void i4_scores(const I4K<D, KV>* c, int t, const I4KP
     }
   };
 #pragma unroll
-  for (int i = 0; i < 4; ++i) s[i] = 0.f;
-  if constexpr (NK > 1) {
-    const f32x4 z = both([&](int ti, int qi, f32x4 acc) { return i4_qm<D, KV>(c[ti], q.sums[qi], acc); });
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = z[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = hi_f32(F16{}, kp.t[i].w[0]) * q.sum;
-  }
-#pragma unroll
   for (int g = 0; g < NK; ++g) {
     const f32x4 acc = both([&](int ti, int qi, f32x4 a0) { return i4_qk<D, KV>(c[ti], q.op[qi], g, a0); });
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(lo_f32(F16{}, kp.t[i].w[g]), acc[i], s[i]);
+    for (int i = 0; i < 4; ++i) {
+      const float step = lo_f32(F16{}, kp.t[i].w[g]);
+      s[i] = g == 0 ? step * acc[i] : __builtin_fmaf(step, acc[i], s[i]);
+    }
   }
+  if constexpr (NK > 1) {
+    const f32x4 z = both([&](int ti, int qi, f32x4 acc) { return i4_qm<D, KV>(c[ti], q.sums[qi], acc); });
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(z[i], 0x1p-24f / I4Query<D, KV>::kSums, s[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(hi_f32(F16{}, kp.t[i].w[0]), q.sum, s[i]);
+  }
+}
+
+// s mul - m with s mul rounded, as the maximum is: never above the threshold,
+// however large the scores.  (In one fma the largest score itself is off by
+// what the maximum's rounding took, from 2^31 on more than an exponent holds.)
+__device__ __forceinline__ float i4_above(float s, float mul, float m) {
+#pragma clang fp contract(off)
+  const float x = s * mul;
+  return x - m;
 }
 
 // Online softmax of NS x 4 scores per lane: weights p (the running maximum
@@ -369,7 +385,7 @@ __device__ __forceinline__ void i4_softmax(const float (&s)[NS][4], float mul, b
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[n][i] = fast_exp2(__builtin_fmaf(s[n][i], mul, -st.m));
+    for (int i = 0; i < 4; ++i) p[n][i] = fast_exp2(i4_above(s[n][i], mul, st.m));
     if (masked) {                  // (uniform)
 #pragma unroll
       for (int i = 0; i < 4; ++i) p[n][i] = s[n][i] == -INFINITY ? 0.f : p[n][i];
@@ -440,6 +456,16 @@ __device__ __forceinline__ void i4_pair(const char* stage, const I4Lane<D, KV>& 
     I4K<D, KV> k[2];
     i4_read_k<D, KV>(stage, o, k[0]);
     i4_read_k<D, KV>(stage + R::kTileBytes, o, k[1]);
+    if constexpr (I4Query<D, KV>::N == 2 && I4Tile<D, KV>::NK > 1) {
+      if (masked) {      // (uniform) one result holds both tiles: 0 x m has to be 0 in a dead token's row
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (lane16 >= (t == 0 ? left0 : left1)) {
+#pragma unroll
+            for (int g = 0; g < I4Tile<D, KV>::NM; ++g) k[t].m.w[g] = 0u;
+          }
+      }
+    }
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
       I4KP<D, KV> kp;

@@ -7,7 +7,7 @@
 //
 // A thread owns 8 consecutive elements of one row of K and of V: one word of
 // codes and one of parameters for 4 bits.  Every value is rounded once, from
-// the fp32 m + n s (int8: the exact product x s) to the output type.
+// the fp32 m + n s (int8: the fp32 product x s) to the output type.
 #include "host_util.hpp"
 #include "int4.hpp"
 #include "kv_rows.hpp"

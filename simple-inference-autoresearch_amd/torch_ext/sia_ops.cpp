@@ -386,6 +386,8 @@ std::tuple<Tensor, OptT> kv_read(const Tensor& k_src, const OptT& v_src, int64_t
   const c10::DeviceGuard guard(dev);
   if (k_src.dim() != 4) throw py::value_error("k_src must have 4 dims");
   if (length < 0) throw py::value_error("length must not be negative");
+  if (start_offset != (int32_t)start_offset || page_size != (int32_t)page_size)
+    throw py::value_error("start_offset and page_size must fit 32 bits");
   const at::ScalarType st = k_src.scalar_type();
   const bool int4 = st == at::kByte, quantised = int4 || st == at::kChar;
   if (block_table.has_value() && block_table->dim() != 2)

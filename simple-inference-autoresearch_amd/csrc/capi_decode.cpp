@@ -262,6 +262,24 @@ int prepare_table(const sia_tensor* bt, const Geometry& g, int page_size, Decode
   return SIA_OK;
 }
 
+// int4 pools of pages that hold no whole tiles: the offsets of the kernels
+// that look up every token, if 32 bits hold them.
+bool any_pages(const sia_tensor* k, const sia_tensor* ks, const sia_tensor* bt, int page_size, DecodeLaunch& L) {
+  auto extent = [&](const sia_tensor* t) {   // bytes of one head's rows, first to last
+    return (double)(t->shape[0] - 1) * bstride(t, 0) + (double)(t->shape[2] - 1) * bstride(t, 2) +
+           (double)t->shape[3] * elem_size(t->dtype);
+  };
+  const double kb = extent(k), sb = extent(ks), tb = ((double)(bt->shape[1] - 1) * bt->stride[1] + 1.0) * 4.0;
+  for (const double x : {kb, sb, tb})
+    if (!(x > 0.0 && x < 4294967280.0)) return false;
+  L.a.page = page_size;
+  L.a.dpage = make_fastdiv((uint32_t)page_size);
+  L.a.k_range = (uint32_t)kb;
+  L.a.ks_range = (uint32_t)sb;
+  L.a.bt_range = (uint32_t)tb;
+  return true;
+}
+
 int prepare_workspace(void* ws, size_t bytes, const Geometry& g, const sia_decode_options* opts, DecodeLaunch& L) {
   if (opts != nullptr) {
     bool dirty = opts->reserved0 != 0;
@@ -333,6 +351,11 @@ int dispatch_f32(const DecodeLaunch& D, const Geometry& g, int kv_dtype, const s
     want = want < 1 ? 1 : want;
     const int64_t most = (cap + 63) / 64;
     if (want > most) want = most;
+    // int4, a length per sequence: eight items per CU while they keep 256 keys,
+    // so that the short sequences' leave room for the long ones' (32 sequences
+    // of 100-4000 tokens, 32/8 heads of 128, fp32: 246 -> 209 us; pieces of 125
+    // keys at head_dim 32 took 31 us for 23)
+    if (kv_dtype == SIA_U8 && d.kv_per_seq && cap >= 512 * want) want *= 2;
     tps = (cap + want - 1) / want;
   }
   tps = (tps + kTile - 1) / kTile * kTile;
@@ -404,7 +427,9 @@ int decode_any(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, co
   L.ws_bytes = ws_bytes;
   // pages that do not hold whole 16-token tiles (page sizes 1-8, or any size
   // other than 16 * 2^k) go to the vector-ALU path with its per-token lookup
-  const bool tiled_pages = bt == nullptr || (kTile << L.a.lg_tiles_per_page) == page_size;
+  bool tiled_pages = bt == nullptr || (kTile << L.a.lg_tiles_per_page) == page_size;
+  // (int4 has matrix kernels for them too, where a layer's pool is below 4 GiB)
+  if (!tiled_pages && k->dtype == SIA_U8 && q->dtype != SIA_F32 && g.D >= 64) tiled_pages = any_pages(k, ks, bt, page_size, L);
   // (int4 at head_dim 16 and 32 too: a row there is a fraction of a k-step)
   if (q->dtype == SIA_F32 || k->dtype == SIA_F32 || !tiled_pages || (k->dtype == SIA_U8 && g.D < 64))
     return dispatch_f32(L, g, k->dtype, out);

@@ -69,7 +69,8 @@ struct I4Ring {
   static constexpr int PI = NK == 8 ? 2 : 1;              // transfers (of 64 words) of its parameters
   static constexpr int kV = 1024 * KI, kKP = 2 * kV, kVP = kKP + 256 * PI;
   static constexpr int kTileBytes = kVP + 256 * PI;
-  static constexpr int kStage = 2 * kTileBytes;
+  static constexpr int kIds = 2 * kTileBytes;             // ANY: page ids of the pair's tokens, then of the pair again
+  static constexpr int kStage = 2 * kTileBytes + (KV::any ? 256 : 0);
   static constexpr int kStages = D == 256 ? 2 : 3;
   static constexpr int kBytes = kStage * kStages;
   static constexpr int kTransfers = 4 * (KI + PI);        // of a stage
@@ -149,6 +150,61 @@ __device__ __forceinline__ void i4_issue(const DecodeArgs& a, const TilePtr& t, 
   for (int i = 0; i < R::KI; ++i) i4_dma16(rv, stage + R::kV + 1024 * i, o.v[i]);
 #pragma unroll
   for (int i = 0; i < R::PI; ++i) i4_dma4(rvp, stage + R::kVP + 256 * i, o.kp[i]);
+}
+
+// ANY: a page holds no whole number of tiles (or one that is no power of two),
+// so every token of a tile is looked up.  The page ids of a pair come by a
+// transfer of their own, one pair ahead of the rows; lane t + 16 i computes the
+// offsets of token t of tile i once, and the lanes that transfer pieces of that
+// token's row fetch them from it.  Offsets are 32-bit, from the pool's start.
+// 32 sequences of 100-4000 tokens in pages of 24, 32/8 heads of 128: 30.6 us, on
+// the vector ALU 251.  (Pages of 16 taken this way cost 1.3% more, over 22
+// shapes, than with one page id per tile.)
+template <int D, class KV>
+struct I4Rows {
+  using C = I4Tile<D, KV>;
+  using R = I4Ring<D, KV>;
+  int k[R::KI], v[R::KI], p[R::PI];            // 4 x the token whose row a lane transfers a piece of
+  uint32_t kc[R::KI], vc[R::KI], pc[R::PI];    // that piece's byte in the row; ~0, past every range, for no piece
+  __device__ __forceinline__ explicit I4Rows(int lane) {
+#pragma unroll
+    for (int i = 0; i < R::KI; ++i) {
+      const int slot = 64 * i + lane, r = slot / R::PC, col = slot % R::PC, t = r & 15;
+      k[i] = 4 * t;
+      v[i] = 4 * (4 * (t & 3) + (t >> 2));
+      kc[i] = r < kTile ? 16u * (uint32_t)(col ^ R::swizzle(r)) : ~0u;
+      vc[i] = r < kTile ? 16u * (uint32_t)col : ~0u;
+    }
+#pragma unroll
+    for (int i = 0; i < R::PI; ++i) {
+      const int w = 64 * i + lane, t = w / C::NK;
+      p[i] = 4 * (t & 15);
+      pc[i] = t < kTile ? 4u * (uint32_t)(w % C::NK) : ~0u;
+    }
+  }
+};
+// Tile i of a pair, from the lanes' offsets of rows of codes and parameters.
+template <int D, class KV>
+__device__ __forceinline__ void i4_issue_rows(__amdgpu_buffer_rsrc_t rk, __amdgpu_buffer_rsrc_t rv,
+                                              __amdgpu_buffer_rsrc_t rkp, __amdgpu_buffer_rsrc_t rvp,
+                                              const I4Rows<D, KV>& o, int i, uint32_t codes, uint32_t params,
+                                              char* stage) {
+  using R = I4Ring<D, KV>;
+  char* dst = stage + i * R::kTileBytes;
+  auto at = [&](uint32_t off, int token, uint32_t byte) {
+    const uint32_t row = (uint32_t)__builtin_amdgcn_ds_bpermute(token + 64 * i, (int)off);
+    return __builtin_elementwise_add_sat(row, byte);
+  };
+#pragma unroll
+  for (int x = 0; x < R::KI; ++x) i4_dma16(rk, dst + 1024 * x, at(codes, o.k[x], o.kc[x]));
+#pragma unroll
+  for (int x = 0; x < R::PI; ++x) {
+    const uint32_t off = at(params, o.p[x], o.pc[x]);
+    i4_dma4(rkp, dst + R::kKP + 256 * x, off);
+    i4_dma4(rvp, dst + R::kVP + 256 * x, off);
+  }
+#pragma unroll
+  for (int x = 0; x < R::KI; ++x) i4_dma16(rv, dst + R::kV + 1024 * x, at(codes, o.v[x], o.vc[x]));
 }
 
 // At most N of the wave's vector memory instructions still outstanding.

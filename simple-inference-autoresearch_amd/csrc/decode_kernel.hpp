@@ -92,6 +92,12 @@ struct DecodeArgs {
   uint32_t k_pg, v_pg, ks_pg, vs_pg;
   uint32_t k_tok, v_tok, ks_tok, vs_tok;
   int32_t cus;                                       // CUs
+  // int4 pools with pages of any size: tokens per page (else 0), and the bytes
+  // from a head's first code, its first parameter and a table row's first entry
+  // to their ends
+  int32_t page;
+  FastDiv dpage;
+  uint32_t k_range, ks_range, bt_range;
 };
 
 // --------------------------------------------------------------------- plan
@@ -660,8 +666,8 @@ struct DecodeWaves {
   static constexpr int value = D <= 64 && (!std::is_same<KV, I8>::value || SV) ? 4 : (D <= 128 ? 2 : 1);
 };
 // int4: 15 KB of ring per wave leave 8 waves to a CU.
-template <int D, int G, bool HALF, bool SV>
-struct DecodeWaves<D, I4G<G, HALF>, SV> {
+template <int D, int G, bool HALF, bool ANY, bool SV>
+struct DecodeWaves<D, I4G<G, HALF, ANY>, SV> {
   static constexpr int value = 2;
 };
 
@@ -899,7 +905,7 @@ void decode_main(const DecodeArgs a) {
       constexpr bool kPartFirst = D > 64 && !(D == 256 && QSplit<KV, QT>::value) && !kInt4;   // (see below)
       // int4: lane l holds the page id of the wave's tile k0 + l, 64 tiles by one load
       auto page_window = [&](int k0) {
-        if (!paged) return 0;      // (nothing to wait for)
+        if (!paged || i4_any<KV>()) return 0;      // (nothing to wait for)
         const int t = t_first + max(0, min(k0 + lane, nt - 1)) * P;
         return btrow[(int64_t)(min(t, cap_tiles - 1) >> a.lg_tiles_per_page) * bt_step];
       };
@@ -978,6 +984,58 @@ void decode_main(const DecodeArgs a) {
           char* ring = smem + wave * i4_wave_lds<D, KV>(a.G16);
           const int np = (nt + 1) >> 1;
           auto left = [&](int k) { return k < nt ? ntok - (t_first + k * P) * kTile : 0; };   // live tokens of tile k
+          if constexpr (i4_any<KV>()) {
+            const I4Rows<D, KV> rows(lane);
+            const __amdgpu_buffer_rsrc_t rk = i4_rsrc(kb, a.k_range), rv = i4_rsrc(vb, a.k_range);
+            const __amdgpu_buffer_rsrc_t rkp = i4_rsrc(ksb, a.ks_range), rvp = i4_rsrc(vsb, a.ks_range);
+            const __amdgpu_buffer_rsrc_t rbt = i4_rsrc((const char*)btrow, a.bt_range);
+            const uint32_t bt_bytes = (uint32_t)bt_step * 4u;
+            int slot = 0;                                // of the lane's token in its page
+            // The page ids of a pair's tokens (tokens and tiles behind the
+            // last ones: those again; what they transfer is never used).
+            auto ask = [&](int pair, int stage) {
+              const int k = min(2 * pair + ((lane >> 4) & 1), nt - 1);
+              const int t = (int)min((uint32_t)((t_first + k * P) * kTile + lane16), (uint32_t)(ntok - 1));
+              const int blk = fdiv(t, a.dpage);
+              slot = t - blk * a.page;
+              i4_dma4(rbt, ring + stage * R::kStage + R::kIds, (uint32_t)blk * bt_bytes);
+            };
+            // A pair, once its ids are there; asks for the next one's ahead of it.
+            auto issue = [&](int pair, int stage) {
+              char* dst = ring + stage * R::kStage;
+              const uint32_t id = *(const uint32_t*)(dst + R::kIds + 4 * lane);
+              const uint32_t pg = id < npages ? id : 0u;               // never read outside the pool
+              const uint32_t codes = pg * a.k_pg + (uint32_t)slot * a.k_tok;
+              const uint32_t params = pg * a.ks_pg + (uint32_t)slot * a.ks_tok;
+              ask(pair + 1, stage + 1 == R::kStages ? 0 : stage + 1);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) i4_issue_rows<D, KV>(rk, rv, rkp, rvp, rows, i, codes, params, dst);
+            };
+            ask(0, 0);
+            i4_wait<0>();
+            issue(0, 0);
+            if constexpr (R::kStages > 2)
+              if (np > 1) {
+                i4_wait<R::kTransfers>();
+                issue(1, 1);
+              }
+            i4_prep_q<D, KV, QT>(a, qraw, lane16, grp, qi);
+            int at = 0;                                  // stage of pair k
+            for (int k = 0; k < np; ++k) {
+              // behind a pair there are the ids of the next but kStages - 1, and that pair
+              if (k + R::kStages - 1 < np) {
+                i4_wait<R::kTransfers>();
+                issue(k + R::kStages - 1, at == 0 ? R::kStages - 1 : at - 1);
+                if constexpr (R::kStages == 2) i4_wait<R::kTransfers + 1>();
+              } else if (R::kStages > 2 && k + 1 < np) {
+                i4_wait<R::kTransfers + 1>();
+              } else {
+                i4_wait<0>();
+              }
+              i4_pair<D, KV>(ring + at * R::kStage, il, ic, qi, left(2 * k), left(2 * k + 1), lane16, grp, st);
+              at = at + 1 == R::kStages ? 0 : at + 1;
+            }
+          } else {
           auto issue = [&](int pair, int stage) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -1011,6 +1069,7 @@ void decode_main(const DecodeArgs a) {
             }
             i4_pair<D, KV>(ring + at * R::kStage, il, ic, qi, left(2 * k), left(2 * k + 1), lane16, grp, st);
             at = at + 1 == R::kStages ? 0 : at + 1;
+          }
           }
           if constexpr (i4_half<KV>()) i4_join<D>(st);
         }

@@ -130,18 +130,22 @@ int launch_decode_q(DecodeLaunch& L) {
 }
 
 // int4 K/V with groups of G elements at head_dim D (64, 128, 256).
-template <int D, int G>
+template <int D, int G, bool ANY = false>
 int launch_decode_i4_typed(DecodeLaunch& L) {
+  using H = I4G<G, true, ANY>;
+  using W = I4G<G, false, ANY>;
   const bool half = L.a.G <= 8;
   if (L.q_dtype == SIA_F16)
-    return half ? launch_decode_typed<D, I4G<G, true>, F16, F16>(L) : launch_decode_typed<D, I4G<G, false>, F16, F16>(L);
+    return half ? launch_decode_typed<D, H, F16, F16>(L) : launch_decode_typed<D, W, F16, F16>(L);
   if (L.q_dtype == SIA_BF16)
-    return half ? launch_decode_typed<D, I4G<G, true>, BF16, F16>(L) : launch_decode_typed<D, I4G<G, false>, BF16, F16>(L);
+    return half ? launch_decode_typed<D, H, BF16, F16>(L) : launch_decode_typed<D, W, BF16, F16>(L);
   return fail(SIA_ERR_UNSUPPORTED, "query dtype must be float16 or bfloat16");
 }
 int launch_decode_i4(DecodeLaunch& L);       // decode_i4.hip
 int launch_decode_i4_128(DecodeLaunch& L);   // decode_i4_d128.hip
 int launch_decode_i4_256(DecodeLaunch& L);   // decode_i4_d256.hip
+int launch_decode_i4_pages(DecodeLaunch& L);       // decode_i4_pages.hip
+int launch_decode_i4_pages_256(DecodeLaunch& L);   // decode_i4_pages_d256.hip
 
 // Entry points implemented by decode_f16.hip / decode_bf16.hip / decode_i8.hip.
 int launch_decode_f16(DecodeLaunch& L);

@@ -33,14 +33,21 @@ namespace sia {
 
 struct I4 { static constexpr int code = SIA_U8; };
 // The same with groups of G elements known to the compiler (the matrix
-// kernels); HALF: at most 8 query heads share a KV head (decode_i4.hpp).
-template <int G, bool HALF>
-struct I4G { static constexpr int group = G; static constexpr bool half = HALF; };
+// kernels); HALF: at most 8 query heads share a KV head, ANY: pages of any
+// size, looked up per token (decode_i4.hpp).
+template <int G, bool HALF, bool ANY = false>
+struct I4G { static constexpr int group = G; static constexpr bool half = HALF, any = ANY; };
 template <class KV> struct IsInt4 { static constexpr bool value = false; };
-template <int G, bool HALF> struct IsInt4<I4G<G, HALF>> { static constexpr bool value = true; };
+template <int G, bool HALF, bool ANY> struct IsInt4<I4G<G, HALF, ANY>> { static constexpr bool value = true; };
 template <class KV>
 constexpr bool i4_half() {
   if constexpr (IsInt4<KV>::value) return KV::half;
+  else return false;
+}
+
+template <class KV>
+constexpr bool i4_any() {
+  if constexpr (IsInt4<KV>::value) return KV::any;
   else return false;
 }
 

@@ -302,7 +302,8 @@ class SimpleCase:
 
 
 def is_matrix(qdt, D, page):
-    return qdt != FP32 and D >= 64 and (page == 0 or (page % 16 == 0 and (page // 16) & (page // 16 - 1) == 0))
+    """Whether the matrix cores take it: any page size, where a layer's pool is below 4 GiB (all pools here)."""
+    return qdt != FP32 and D >= 64
 
 
 DECODES = [

@@ -148,7 +148,11 @@ int sia_paged_gqa_int8_flash_decode(const sia_tensor* q, const sia_tensor* k_poo
  * points but for the cache: k_int4, v_int4 (B', Hkv, S, D / 2) or pools
  * (num_pages, Hkv, page_size, D / 2) uint8, 16-byte aligned rows (8 at
  * head_dim 16); k_scale, v_scale the same shape with a last dim of 2 D / g,
- * f16, 4-byte aligned rows.  q f16|bf16|f32. */
+ * f16, 4-byte aligned rows.  q f16|bf16|f32.  k and v have the same strides, and
+ * so do their parameters (SIA_ERR_UNSUPPORTED otherwise: the kernels compute
+ * every offset once for both).  16-bit q at head_dim 64 and more runs on the
+ * matrix cores whatever the page size, unless a pool is 4 GiB or larger and its
+ * pages are not of 16 * 2^k tokens; everything else on the vector ALUs. */
 int sia_attention_flash_decode_int4(const sia_tensor* q, const sia_tensor* k_int4, const sia_tensor* v_int4,
                                     const sia_tensor* k_scale, const sia_tensor* v_scale,
                                     const sia_tensor* kv_len, float sm_scale, const sia_tensor* out,
@@ -290,8 +294,9 @@ int sia_dequantize_kv_int4(const sia_tensor* codes, const sia_tensor* params, co
  * k_scale_dst / v_scale_dst, shaped like the destination without head_dim,
  * f16 or f32) or uint8 (int4: codes of head_dim / 2 bytes, the parameters of
  * sia_quantize_kv_int4 written to k_scale_dst / v_scale_dst, shaped like the
- * destination with a last dim of 2 D / g).  Positions outside the destination (p >= capacity, page id
- * outside the pool) are skipped on the device, never written. */
+ * destination with a last dim of 2 D / g).  Positions outside the destination
+ * (p >= capacity, page id outside the pool) are skipped on the device, never
+ * written. */
 int sia_kv_write(const sia_tensor* k, const sia_tensor* v, const sia_tensor* k_dst, const sia_tensor* v_dst,
                  const sia_tensor* k_scale_dst, const sia_tensor* v_scale_dst, const sia_tensor* block_table,
                  const sia_tensor* start_pos, int32_t start_pos_host, int32_t page_size, void* stream);

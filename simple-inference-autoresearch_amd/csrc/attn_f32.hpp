@@ -5,16 +5,20 @@
 // (kernels/flash_decode_kernel.py:119-160, kernels/attention_kernel.py:235-305);
 // its decode kernel computes in fp32 on vector lanes, tl.sum(q * k) and
 // tl.sum(p * v) with an online softmax (kernels/flash_decode_kernel.py:85-114).
-// The 16-bit MFMA kernels of this library take 16-bit or int8 operands, so
-// float32 inputs run here instead, in fp32 end to end: products, sums,
-// exponentials and the output (rounded to q's dtype).
+// The 16-bit MFMA kernels of this library take 16-bit, int8 or int4 operands,
+// so float32 inputs run here instead, in fp32 end to end: products, sums,
+// exponentials and the output (rounded to q's dtype).  int4 caches do at
+// head_dim 16 and 32 too, and in pools of 4 GiB and more whose pages hold no
+// 16 x 2^k tokens; their values are formed in fp32, each rounded once.
+// (int4, fp32 queries: 4 x 512 tokens, 32/8 heads of 64, 9.0 us; 8 x 4000, 32/8
+// of 128, 49 us, where the vector ALU bounds: 0.76 TB/s.)
 //
 // attn_f32 (gfx950, wave64):
 //  * A work item is one (sequence, KV head), up to kF32Cols of its query heads
 //    ("columns") and one split of the key range [0, kv_len).  The K/V rows of
 //    the item are read once for all of its columns.
-//  * D/4 lanes share a key row, 4 dimensions each (16-byte fp32 loads; 8 or 4
-//    bytes for 16-bit and int8 K/V), so one load instruction of a wave reads
+//  * D/4 lanes share a key row, 4 dimensions each (16-byte fp32 loads; 8, 4 or
+//    2 bytes for 16-bit, int8 and int4 K/V), so one load instruction of a wave reads
 //    64/(D/4) whole rows.  Each lane group runs an online softmax over its
 //    own keys (kF32Unroll keys per step); the dot products are completed
 //    with cross-lane sums inside the group.  Groups are merged with shuffles,

@@ -20,6 +20,19 @@
 // it took 15 narrow loads (64 rows of 16 bytes for K, 4-byte pieces of V and of
 // the parameters), and the address unit was busy 73% of a call of 64 x 8192
 // tokens, 32/8 heads, that HBM should bound.
+//
+// Bound: HBM for large calls, closely followed by instruction issue (two waves
+// per SIMD, each issuing half of the time); fixed costs for small ones (plan,
+// length, page id, first tile, merge: 9 us of the kernel, 3 of the merge
+// kernel).  Measured, bf16 queries, the call / the same transfers without the
+// arithmetic / the int8 cache:
+//   64 x 8192 tokens, 32/8 heads of 128, groups of 64   104 (5.8 TB/s) / 97 / 188 us
+//   256 log-normal lengths, 64/8 of 128, groups of 32   220 (5.3 TB/s) / 210 / -
+//   32 x 8000, 16/4 of 256, groups of 64                 59 (5.0 TB/s) / 54 / -
+//   16 x 0-4096, 16/16 of 64 (fp16), groups of 32        20 / 17 / 45
+//   1 x 1000, 32/8 of 128, groups of 64                  12.3 / 9.9 / 13.5
+// (The scores of one pair beside V of the pair before, in one wave, took 2.8%
+// more: registers, not overlap, are short.)
 #pragma once
 
 namespace sia {

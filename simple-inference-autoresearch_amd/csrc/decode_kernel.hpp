@@ -1,8 +1,8 @@
 // Paged / contiguous flash-decode for gfx950 (single query per sequence, GQA).
 //
 // One kernel template serves every decode entry point of the library
-// (fp16/bf16 KV, int8 KV with per-token-per-head scales, contiguous or paged,
-// one or many split-K items per sequence).  Semantics follow the reference
+// (fp16/bf16 KV, int8 KV with per-token-per-head scales, int4 KV (its tiles:
+// decode_i4.hpp), contiguous or paged, one or many split-K items per sequence).  Semantics follow the reference
 // kernels: kernels/flash_decode_kernel.py:53-116 (online softmax, l==0 guard),
 // kernels/flash_decode_int8_kernel.py:51-118 (scale folding),
 // kernels/paged_flash_decode_kernel.py:40-104 (block-table indirection) and

@@ -5,6 +5,9 @@
 // position outside the source (past its capacity, page id outside the pool) reads
 // as zeros.
 //
+// Bound: HBM.  16 x 5000 tokens, 4 heads of 256, 4 bits to bf16: 87.9 us, 415 MB
+// at 4.7 TB/s, the rate of a large copy.
+//
 // A thread owns 8 consecutive elements of one row of K and of V: one word of
 // codes and one of parameters for 4 bits.  Every value is rounded once, from
 // the fp32 m + n s (int8: the fp32 product x s) to the output type.

@@ -220,8 +220,9 @@ def attention_flash_decode_int4(q: torch.Tensor, k_int4: torch.Tensor, v_int4: t
 
     k_int4, v_int4: (B, Hkv, S, D/2) uint8 codes; k_scale, v_scale: (B, Hkv, S,
     2D/g) fp16 steps and minima of groups of g elements; kv_len int32, (1,)/()
-    shared or (B,) per sequence.  q (B, Hq, 1, D) fp16, bf16 or fp32; returns
-    (B, 1, Hq, D) in q's dtype.
+    shared or (B,) per sequence.  K and V share their strides, and so do their
+    parameters (NotImplementedError otherwise).  q (B, Hq, 1, D) fp16, bf16 or
+    fp32; returns (B, 1, Hq, D) in q's dtype.
     """
     scale = _common(q, k_int4, sm_scale)
     kl = _kv_len_tensor(kv_len, q.device)
@@ -236,7 +237,8 @@ def paged_gqa_int4_flash_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: t
 
     k_pool, v_pool: (num_blocks, Hkv, page_size, D/2) uint8 codes; k_scale_pool,
     v_scale_pool: (num_blocks, Hkv, page_size, 2D/g) fp16; block_table (B,
-    max_blocks) int32; kv_len (1,)/() or (B,) int32.
+    max_blocks) int32; kv_len (1,)/() or (B,) int32; any page size.  Strides as
+    in :func:`attention_flash_decode_int4`.
     """
     P = k_pool.shape[2]
     if P != page_size:

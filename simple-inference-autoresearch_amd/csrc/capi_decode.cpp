@@ -262,6 +262,10 @@ int prepare_table(const sia_tensor* bt, const Geometry& g, int page_size, Decode
   return SIA_OK;
 }
 
+// The matrix kernels keep 4 bytes per sequence in LDS beside up to 127 KB of
+// rings and merge state, of 160 KB.
+constexpr int kI4MaxBatch = 8192;
+
 // int4 pools of pages that hold no whole tiles: the offsets of the kernels
 // that look up every token, if 32 bits hold them.
 bool any_pages(const sia_tensor* k, const sia_tensor* ks, const sia_tensor* bt, int page_size, DecodeLaunch& L) {
@@ -430,8 +434,10 @@ int decode_any(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, co
   bool tiled_pages = bt == nullptr || (kTile << L.a.lg_tiles_per_page) == page_size;
   // (int4 has matrix kernels for them too, where a layer's pool is below 4 GiB)
   if (!tiled_pages && k->dtype == SIA_U8 && q->dtype != SIA_F32 && g.D >= 64) tiled_pages = any_pages(k, ks, bt, page_size, L);
-  // (int4 at head_dim 16 and 32 too: a row there is a fraction of a k-step)
-  if (q->dtype == SIA_F32 || k->dtype == SIA_F32 || !tiled_pages || (k->dtype == SIA_U8 && g.D < 64))
+  // (int4 at head_dim 16 and 32 too: a row there is a fraction of a k-step; and
+  // batches whose plan does not fit into LDS beside the rings)
+  if (q->dtype == SIA_F32 || k->dtype == SIA_F32 || !tiled_pages ||
+      (k->dtype == SIA_U8 && (g.D < 64 || g.B > kI4MaxBatch)))
     return dispatch_f32(L, g, k->dtype, out);
   return dispatch(L, k->dtype);
 }

@@ -59,7 +59,7 @@ int check_alike(const sia_tensor* k, const sia_tensor* v, const char* kn, const 
   if (v->dtype != k->dtype || v->ndim != k->ndim)
     return fail(SIA_ERR_INVALID_ARGUMENT, "%s and %s must have one dtype and rank", kn, vn);
   for (int d = 0; d < k->ndim; ++d)
-    if (v->shape[d] != k->shape[d] || v->stride[d] != k->stride[d])
+    if (v->shape[d] != k->shape[d] || (k->shape[d] > 1 && v->stride[d] != k->stride[d]))
       return fail(SIA_ERR_INVALID_ARGUMENT, "%s and %s must have the same shape and strides", kn, vn);
   return SIA_OK;
 }

@@ -283,3 +283,57 @@ def test_prompt_of_no_tokens_and_batches_of_none(gpu_pkg):
     assert v is None and not k.any()
     codes, par = gpu_pkg.quantize_kv_int4(e)
     assert gpu_pkg.dequantize_kv_int4(codes, par).shape == e.shape
+
+
+@pytest.mark.parametrize("B", [4200, 8192, 8193])
+@pytest.mark.parametrize("D,page", [(128, 16), (64, 24), (256, 0)])
+def test_large_batches(gpu_pkg, B, D, page):
+    """Thousands of short sequences: plans whose lengths, and then whose prefix, do not fit into LDS."""
+    announce(f"int4 decode batch {B} D {D} page {page}")
+    c = cache_case(gpu_pkg, D, B, 1, D, 32, 20, page)
+    lens = [(7 * b) % 21 for b in range(B)]
+    if page:
+        gpu_pkg.kv_write(c.k, c.v, c.kc, c.vc, c.ks, c.vs, block_table=c.bt, page_size=page)
+    else:
+        gpu_pkg.kv_write(c.k, c.v, c.kc, c.vc, c.ks, c.vs)
+    q = randn(gen(4), B, 2, 1, D)
+    out = c.run(gpu_pkg, q, lens_tensor(lens))
+    torch.cuda.synchronize()
+    some = list(range(0, B, 97)) + [B - 1]
+    k, v = (I4.values(*I4.quantize(t[some].float().cpu().numpy(), 32)) for t in (c.k, c.v))
+    check_decode(out[some], q[some], k, v, [lens[b] for b in some], "large batch", B <= 8192)
+    assert (out[lens.index(0)::21] == 0).all()
+
+
+@pytest.mark.parametrize("D,page,qdt", [(128, 0, BF16), (64, 16, FP16), (128, 24, BF16), (128, 16, FP32)])
+def test_lengths_past_the_cache(gpu_pkg, D, page, qdt):
+    """A kv_len beyond the capacity counts as the capacity, a negative one as none."""
+    announce(f"int4 decode lengths past the cache D {D} page {page} {qdt}")
+    S = 96
+    c = cache_case(gpu_pkg, D, 3, 2, D, 32, S, page)
+    c.fill(gpu_pkg, [S] * 3)
+    q = randn(gen(4), 3, 8, 1, D, dtype=qdt)
+    a = c.run(gpu_pkg, q, lens_tensor([S, 1 << 30, -5]))
+    b = c.run(gpu_pkg, q, lens_tensor([S, S, 0]))
+    torch.cuda.synchronize()
+    assert torch.equal(a, b) and torch.isfinite(a).all() and (a[2] == 0).all()
+    assert torch.equal(c.run(gpu_pkg, q, 2 ** 31 - 1), c.run(gpu_pkg, q, S))
+
+
+def test_strides_of_dims_of_one(gpu_pkg):
+    """Dims of size 1 have no stride to compare."""
+    announce("int4 dims of one")
+    H, S, D = 2, 40, 128
+    c = cache_case(gpu_pkg, 5, 1, H, D, 64, S, 0)
+    c.fill(gpu_pkg, [S])
+    other = [t.new_zeros(3, *t.shape[1:]) for t in (c.vc, c.vs)]
+    for o, t in zip(other, (c.vc, c.vs)):
+        o[1] = t[0]
+    vc, vs = (o.as_strided(t.shape, (80, *o.stride()[1:]), o.stride(0)) for o, t in zip(other, (c.vc, c.vs)))
+    q = randn(gen(4), 1, 4, 1, D)
+    a = gpu_pkg.attention_flash_decode_int4(q, c.kc, vc, c.ks, vs, S)
+    b = gpu_pkg.attention_flash_decode_int4(q, c.kc, c.vc, c.ks, c.vs, S)
+    assert torch.equal(a, b)
+    x = gpu_pkg.kv_read(c.kc, vc, S, c.ks, vs)
+    y = gpu_pkg.kv_read(c.kc, c.vc, S, c.ks, c.vs)
+    assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])

@@ -8,10 +8,11 @@
 // The 16-bit MFMA kernels of this library take 16-bit, int8 or int4 operands,
 // so float32 inputs run here instead, in fp32 end to end: products, sums,
 // exponentials and the output (rounded to q's dtype).  int4 caches do at
-// head_dim 16 and 32 too, and in pools of 4 GiB and more whose pages hold no
-// 16 x 2^k tokens; their values are formed in fp32, each rounded once.
-// (int4, fp32 queries: 4 x 512 tokens, 32/8 heads of 64, 9.0 us; 8 x 4000, 32/8
-// of 128, 49 us, where the vector ALU bounds: 0.76 TB/s.)
+// head_dim 16 and 32 too, in pools of 4 GiB and more whose pages hold no
+// 16 x 2^k tokens, with float32 queries in such pages at all, and with float32
+// queries where a call is small (f32_matrix in capi_decode.cpp); their values
+// are formed in fp32, each rounded once.  (4 x 512 tokens, 32/8 heads of 64,
+// 9.1 us.)
 //
 // attn_f32 (gfx950, wave64):
 //  * A work item is one (sequence, KV head), up to kF32Cols of its query heads

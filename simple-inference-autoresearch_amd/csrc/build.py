@@ -92,6 +92,7 @@ EXTRA_FLAGS = {
     "decode_i8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "decode_i4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "decode_i4_d128.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "decode_i4_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "decode_i4_pages.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attn_f32_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }

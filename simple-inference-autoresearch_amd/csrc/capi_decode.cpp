@@ -262,6 +262,16 @@ int prepare_table(const sia_tensor* bt, const Geometry& g, int page_size, Decode
   return SIA_OK;
 }
 
+// int4 and float32 queries: the matrix cores from 150 thousand rows x tokens of
+// capacity on, if two query heads or more share a KV head.  Below, the
+// vector-ALU kernel's shorter start wins, and it does one column's work where
+// the matrix cores do 16.  us, matrix / vector, head_dim 128: 32/8 heads, 4 x
+// 500 tokens 15.8 / 11.2, 4 x 2000 19.2 / 22.5, 64 x 500 31.4 / 48.4, 4 x 8000
+// 35.4 / 52.8; 64/4 heads, 4 x 500 18.0 / 14.2, 16 x 2000 26.0 / 72.3; 16/8
+// heads, 4 x 2000 19.7 / 18.1, 4 x 8000 35.4 / 40.6; 8/8 heads, 4 x 2000 19.2 /
+// 16.4, 16 x 2000 34.6 / 32.6.
+bool f32_matrix(const Geometry& g, int cap) { return g.G >= 2 && (int64_t)g.B * g.Hq * cap >= 150000; }
+
 // The matrix kernels keep 4 bytes per sequence in LDS beside up to 127 KB of
 // rings and merge state, of 160 KB.
 constexpr int kI4MaxBatch = 8192;
@@ -357,8 +367,8 @@ int dispatch_f32(const DecodeLaunch& D, const Geometry& g, int kv_dtype, const s
     if (want > most) want = most;
     // int4, a length per sequence: eight items per CU while they keep 256 keys,
     // so that the short sequences' leave room for the long ones' (32 sequences
-    // of 100-4000 tokens, 32/8 heads of 128, fp32: 246 -> 209 us; pieces of 125
-    // keys at head_dim 32 took 31 us for 23)
+    // of 100-4000 tokens, 32/8 heads of 128, pages of 24: 251 -> 215 us; pieces
+    // of 125 keys at head_dim 32 took 31 us for 23)
     if (kv_dtype == SIA_U8 && d.kv_per_seq && cap >= 512 * want) want *= 2;
     tps = (cap + want - 1) / want;
   }
@@ -436,9 +446,13 @@ int decode_any(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, co
   if (!tiled_pages && k->dtype == SIA_U8 && q->dtype != SIA_F32 && g.D >= 64) tiled_pages = any_pages(k, ks, bt, page_size, L);
   // (int4 at head_dim 16 and 32 too: a row there is a fraction of a k-step; and
   // batches whose plan does not fit into LDS beside the rings)
-  if (q->dtype == SIA_F32 || k->dtype == SIA_F32 || !tiled_pages ||
-      (k->dtype == SIA_U8 && (g.D < 64 || g.B > kI4MaxBatch)))
+  const bool vector = k->dtype != SIA_U8 ? q->dtype == SIA_F32 || k->dtype == SIA_F32
+                                         : g.D < 64 || g.B > kI4MaxBatch ||
+                                               (q->dtype == SIA_F32 && !f32_matrix(g, L.a.cap_tokens));
+  if (vector || !tiled_pages)
     return dispatch_f32(L, g, k->dtype, out);
+  if (q->dtype == SIA_F32 && (!aligned16(out->data) || bstride(out, 0) % 16 || bstride(out, 2) % 16))
+    return fail(SIA_ERR_INVALID_ARGUMENT, "out rows must be 16-byte aligned");
   return dispatch(L, k->dtype);
 }
 

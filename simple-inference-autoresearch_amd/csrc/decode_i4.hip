@@ -4,6 +4,7 @@
 namespace sia {
 
 int launch_decode_i4(DecodeLaunch& L) {
+  if (L.q_dtype == SIA_F32) return launch_decode_i4_f32(L);
   if (L.a.page > 0) return launch_decode_i4_pages(L);
   switch (L.D) {
     case 64: return L.lg_group == 5 ? launch_decode_i4_typed<64, 32>(L) : launch_decode_i4_typed<64, 64>(L);

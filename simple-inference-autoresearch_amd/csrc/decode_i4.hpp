@@ -578,6 +578,90 @@ __device__ __forceinline__ void i4_pair(const char* stage, const I4Lane<D, KV>& 
   i4_pv<D, KV>(v, ic, pop, st);
 }
 
+// ---- fp32 queries: fp32 MFMAs over the values m + n s, each rounded once to fp32
+// as kv_read rounds them; nothing is rounded to fewer bits.  Tiles, rings and
+// softmax are the same.  Bound: the matrix cores (256 FLOP per cycle per CU, and
+// 16 columns whatever the heads): 32 sequences of 100-4000 tokens, 32/8 heads of
+// 128, 76 us, on the vector ALU 207.  (Which one: f32_matrix in capi_decode.cpp.)
+
+// A lane's query elements, in the order of its codes of K.
+template <int D>
+struct I4Query32 {
+  f32x4 x[D / 16];
+};
+template <int D>
+__device__ __forceinline__ I4Query32<D> i4_load_q32(const DecodeArgs& a, int b, int hq, bool live, int grp) {
+  I4Query32<D> q;
+  const char* qp = a.q + b * a.q_sb + (int64_t)hq * a.q_sh + grp * 32;
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j)
+    q.x[j] = live ? *(const f32x4*)(qp + 128 * (j >> 1) + 16 * (j & 1)) : f32x4{0.f, 0.f, 0.f, 0.f};
+  return q;
+}
+__device__ __forceinline__ f32x4 i4_mfma32(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+// Value i of a word of codes (even: the codes at bits 0-3 of the bytes, odd: at 4-7).
+__device__ __forceinline__ float i4_value_of(uint32_t even, uint32_t odd, int i, uint32_t sm) {
+  const uint32_t w = (i & 1) ? odd : even;
+  const float n = (float)(uint8_t)(w >> (8 * (i >> 1)));
+  return __builtin_fmaf(n, lo_f32(F16{}, sm), hi_f32(F16{}, sm));
+}
+template <int D, class KV>
+__device__ __forceinline__ void i4_pair32(const char* stage, const I4Lane<D, KV>& o, const I4Query32<D>& q, float mul,
+                                          int left0, int left1, int lane16, int grp, WaveState<D>& st) {
+  using R = I4Ring<D, KV>;
+  using C = I4Tile<D, KV>;
+  constexpr int PER = C::G / 32;
+  const bool masked = left0 < kTile || left1 < kTile;
+  float s[2][4], p[2][4];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const char* tile = stage + t * R::kTileBytes;
+    I4K<D, KV> k;
+    i4_read_k<D, KV>(tile, o, k);
+    Raw<4 * C::NK> sm;                                        // of the lane's token
+    i4_read<4 * C::NK>(sm, tile + R::kKP + 4 * C::NK * lane16);
+    f32x4 acc[2] = {};                                        // (two chains: half the roundings of one)
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      const uint32_t even = k.k.w[j] & 0x0f0f0f0fu, odd = (k.k.w[j] >> 4) & 0x0f0f0f0fu;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        acc[i & 1] = i4_mfma32(i4_value_of(even, odd, i, sm.w[j / PER]), q.x[2 * j + (i >> 2)][i & 3], acc[i & 1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[t][i] = acc[0][i] + acc[1][i];
+  }
+  I4V<D, KV> v[2];
+  i4_read_v<D, KV>(stage, o, v[0]);
+  i4_read_v<D, KV>(stage + R::kTileBytes, o, v[1]);
+  if (masked) {      // (uniform) as in i4_pair
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (4 * grp + i >= (t == 0 ? left0 : left1)) {
+          s[t][i] = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < C::NV; ++g) v[t].p[i].w[g] = 0u;
+        }
+  }
+  i4_softmax<D, 2>(s, mul, masked, st, p);
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < D / 128 + (D == 64); ++h) {         // words of the lane's share (D = 64: half of one)
+        const uint32_t w = v[t].v[i].w[h], even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
+        const uint32_t sm = v[t].p[i].w[C::NV == 2 ? h : 0];
+#pragma unroll
+        for (int e = 0; e < (D == 64 ? 4 : 8); ++e)
+          st.acc[8 * h + e] = i4_mfma32(i4_value_of(even, odd, e, sm), p[t][i], st.acc[8 * h + e]);
+      }
+}
+
 // HALF: the two tiles' states of a head, columns c and c + 8, added up.
 template <int D>
 __device__ __forceinline__ void i4_join(WaveState<D>& st) {

@@ -766,10 +766,11 @@ void decode_main(const DecodeArgs a) {
   if (a.direct_only && W == 0) {
     // one shared length of zero, and no merge kernel follows: every output
     // row is zero (the l == 0 guard), written here as 4-byte words
-    const int64_t words = (int64_t)a.B * a.Hq * (D / 2);
+    constexpr int RW = std::is_same<QT, F32>::value ? D : D / 2;      // words of a row
+    const int64_t words = (int64_t)a.B * a.Hq * RW;
     for (int64_t i = (int64_t)blockIdx.x * (NW * 64) + threadIdx.x; i < words; i += (int64_t)gridDim.x * (NW * 64)) {
-      const int64_t row = i / (D / 2);
-      const int wd = (int)(i - row * (D / 2));
+      const int64_t row = i / RW;
+      const int wd = (int)(i - row * RW);
       const int bb = (int)(row / a.Hq), hh = (int)(row - (int64_t)bb * a.Hq);
       *(uint32_t*)(a.out + bb * a.o_sb + (int64_t)hh * a.o_sh + 4 * wd) = 0u;
     }
@@ -853,7 +854,9 @@ void decode_main(const DecodeArgs a) {
   // (Not where its registers do not fit: head_dim 64, two groups per CU in 128
   // registers, and int8 with scattered scales.)
   constexpr bool kNext = D > 64 && (!TileT::kInt8 || SV) && !kInt4;
-  QRaw<D> q_next;
+  constexpr bool kF32Q = std::is_same<QT, F32>::value;                // (int4 only)
+  using QRawT = std::conditional_t<kF32Q, I4Query32<D>, QRaw<D>>;
+  QRawT q_next;
   int pg_next = 0, seg_next = -1;
   bool first_seg = true;
   while (x < x_hi) {
@@ -900,7 +903,7 @@ void decode_main(const DecodeArgs a) {
       // The loads that need only the item go out together: the query row and
       // the page ids of the first tile and of the partial one (the length is
       // already in flight), unless the previous segment loaded them already.
-      QRaw<D> qraw;
+      QRawT qraw;
       int pg0;
       constexpr bool kPartFirst = D > 64 && !(D == 256 && QSplit<KV, QT>::value) && !kInt4;   // (see below)
       // int4: lane l holds the page id of the wave's tile k0 + l, 64 tiles by one load
@@ -916,7 +919,9 @@ void decode_main(const DecodeArgs a) {
         qraw = q_next;
         pg0 = pg_next;
       } else {
-        if constexpr (i4_half<KV>()) {   // column c + 8 holds head c's query too
+        if constexpr (kF32Q) {
+          qraw = i4_load_q32<D>(a, b, hq, live, grp);
+        } else if constexpr (i4_half<KV>()) {   // column c + 8 holds head c's query too
           const int qc = lane16 & 7;
           qraw = load_q_raw<D, KV>(a, b, qc < nh ? hkv * a.G + 16 * hg + qc : 0, qc < nh, grp);
         } else {
@@ -935,7 +940,7 @@ void decode_main(const DecodeArgs a) {
         const int hkv_n = fdiv(unit_n, a.dHG), hg_n = unit_n - hkv_n * a.HG;
         const bool live_n = lane16 < min(16, a.G - 16 * hg_n);
         const int hq_n = live_n ? hkv_n * a.G + 16 * hg_n + lane16 : 0;
-        q_next = load_q_raw<D, KV>(a, nx.b, hq_n, live_n, grp);
+        if constexpr (!kF32Q) q_next = load_q_raw<D, KV>(a, nx.b, hq_n, live_n, grp);
         const int32_t* btrow_n = paged ? a.bt + (int64_t)nx.b * a.bt_sb : a.kv_len;
         const int tn = min(nx.t_lo + phase, cap_tiles - 1);
         pg_next = uniform(btrow_n[(int64_t)(tn >> a.lg_tiles_per_page) * bt_step]);
@@ -1051,7 +1056,7 @@ void decode_main(const DecodeArgs a) {
 #pragma unroll 1
             for (int k = 0; k < min(R::kStages - 1, np); ++k) issue(k, k);
           }
-          i4_prep_q<D, KV, QT>(a, qraw, lane16, grp, qi);
+          if constexpr (!kF32Q) i4_prep_q<D, KV, QT>(a, qraw, lane16, grp, qi);
           int at = 0;                                    // stage of pair k
           for (int k = 0; k < np; ++k) {
             const int kn = k + R::kStages - 1;
@@ -1067,7 +1072,10 @@ void decode_main(const DecodeArgs a) {
             } else {
               i4_wait<0>();
             }
-            i4_pair<D, KV>(ring + at * R::kStage, il, ic, qi, left(2 * k), left(2 * k + 1), lane16, grp, st);
+            if constexpr (kF32Q)
+              i4_pair32<D, KV>(ring + at * R::kStage, il, qraw, a.qk_scale, left(2 * k), left(2 * k + 1), lane16, grp, st);
+            else
+              i4_pair<D, KV>(ring + at * R::kStage, il, ic, qi, left(2 * k), left(2 * k + 1), lane16, grp, st);
             at = at + 1 == R::kStages ? 0 : at + 1;
           }
           }
@@ -1185,6 +1193,14 @@ void decode_main(const DecodeArgs a) {
         if (direct) {
           const float inv = unscale / (lsum == 0.f ? 1.f : lsum);
           char* op = a.out + b * a.o_sb + (int64_t)hq * a.o_sh;
+          if constexpr (kF32Q) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int e = 0; e < E; e += 4)
+                *(f32x4*)(op + out_d<D, KV>(grp, i, e) * 4) =
+                    f32x4{st.acc[e][i] * inv, st.acc[e + 1][i] * inv, st.acc[e + 2][i] * inv, st.acc[e + 3][i] * inv};
+          } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1192,6 +1208,7 @@ void decode_main(const DecodeArgs a) {
               const uint32_t w = pack2(QT{}, st.acc[e][i] * inv, st.acc[e + 1][i] * inv);
               *(uint32_t*)(op + out_d<D, KV>(grp, i, e) * 2) = w;
             }
+          }
         } else {
           float* dst = a.ws_acc + (pslot + lane16) * D;
 #pragma unroll
@@ -1275,8 +1292,10 @@ void decode_main(const DecodeArgs a) {
         const int hqo = hkv * a.G + 16 * hg + cc;
         if (direct) {
           const float ls = L == 0.f ? 1.f : L;            // (A / L, not A times 1 / L: one rounding before the 16-bit one)
-          char* op = a.out + b * a.o_sb + (int64_t)hqo * a.o_sh + DL * lane * (int)sizeof(uint16_t);
-          if constexpr (DL == 1) {
+          char* op = a.out + b * a.o_sb + (int64_t)hqo * a.o_sh + DL * lane * (int)(kF32Q ? sizeof(float) : sizeof(uint16_t));
+          if constexpr (kF32Q) {
+            *(fDL*)op = A / ls;
+          } else if constexpr (DL == 1) {
             store_out(QT{}, op, A[0] / ls);
           } else {
 #pragma unroll
@@ -1440,9 +1459,14 @@ __global__ __launch_bounds__(PW * 64) void decode_reduce(const DecodeArgs a) {
   }
   if (!work) return;
   const float inv = 1.0f / (L == 0.f ? 1.f : L);
+  if constexpr (std::is_same<OT, F32>::value) {
+    *(f32x4*)(a.out + b * a.o_sb + (int64_t)hq * a.o_sh + 4 * li * (int)sizeof(float)) = A * inv;
+    return;
+  } else {
   char* op = a.out + b * a.o_sb + (int64_t)hq * a.o_sh + 4 * li * (int)sizeof(uint16_t);
   *(uint32_t*)op = pack2(OT{}, A[0] * inv, A[1] * inv);
   *(uint32_t*)(op + 4) = pack2(OT{}, A[2] * inv, A[3] * inv);
+  }
 }
 
 }  // namespace sia

@@ -144,6 +144,7 @@ int launch_decode_i4_typed(DecodeLaunch& L) {
 int launch_decode_i4(DecodeLaunch& L);       // decode_i4.hip
 int launch_decode_i4_128(DecodeLaunch& L);   // decode_i4_d128.hip
 int launch_decode_i4_256(DecodeLaunch& L);   // decode_i4_d256.hip
+int launch_decode_i4_f32(DecodeLaunch& L);         // decode_i4_f32.hip (float32 queries)
 int launch_decode_i4_pages(DecodeLaunch& L);       // decode_i4_pages.hip
 int launch_decode_i4_pages_256(DecodeLaunch& L);   // decode_i4_pages_d256.hip
 

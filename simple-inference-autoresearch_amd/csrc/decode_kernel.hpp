@@ -710,7 +710,8 @@ void decode_main(const DecodeArgs a) {
   constexpr int E = D / 16;
   constexpr int KSTEPS = D / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  // LDS: [acc: NW*G16*D f32, int4: the waves' rings][m: NW*G16][l: NW*G16][red: 2*NW+2 ints][pre: B+1 ints][lens: B ints, B <= kLensInLds]
+  // LDS: [acc: NW*G16*D f32, int4: the waves' rings][m: NW*G16][l: NW*G16]
+  // [red: 2*NW+2 ints][pre: B+1 ints][lens: B ints, B <= kLensInLds]
   float* l_acc = (float*)smem;
   // merge state of head column c of wave w (int4: inside the wave's ring)
   auto acc_at = [&](int w, int c) {
@@ -1041,43 +1042,43 @@ void decode_main(const DecodeArgs a) {
               at = at + 1 == R::kStages ? 0 : at + 1;
             }
           } else {
-          auto issue = [&](int pair, int stage) {
+            auto issue = [&](int pair, int stage) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int k = 2 * pair + i, kn = min(k, nt - 1);
-              const TilePtr tp = tile_ptr(t_first + kn * P, __builtin_amdgcn_readlane(pgw, kn & 63));
-              i4_issue<D, KV>(a, tp, il, left(k), ring + stage * R::kStage + i * R::kTileBytes);
-            }
-          };
-          // (one copy of the code for two pairs: 1.5% of a call's time at head_dim 64 and 128)
-          if constexpr (R::kStages == 2) {
-            issue(0, 0);
-          } else {
-#pragma unroll 1
-            for (int k = 0; k < min(R::kStages - 1, np); ++k) issue(k, k);
-          }
-          if constexpr (!kF32Q) i4_prep_q<D, KV, QT>(a, qraw, lane16, grp, qi);
-          int at = 0;                                    // stage of pair k
-          for (int k = 0; k < np; ++k) {
-            const int kn = k + R::kStages - 1;
-            if ((kn & 31) == 0 && kn < np) {
-              pgw = page_window(2 * kn);
-              asm volatile("" ::"v"(pgw));               // (waited for here, not by every round at its readlane)
-            }
-            if (kn < np) {
-              issue(kn, at == 0 ? R::kStages - 1 : at - 1);
-              i4_wait<(R::kStages - 1) * R::kTransfers>();
-            } else if (R::kStages > 2 && k + 1 < np) {   // (one pair behind this one)
-              i4_wait<R::kTransfers>();
+              for (int i = 0; i < 2; ++i) {
+                const int k = 2 * pair + i, kn = min(k, nt - 1);
+                const TilePtr tp = tile_ptr(t_first + kn * P, __builtin_amdgcn_readlane(pgw, kn & 63));
+                i4_issue<D, KV>(a, tp, il, left(k), ring + stage * R::kStage + i * R::kTileBytes);
+              }
+            };
+            // (one copy of the code for two pairs: 1.5% of a call's time at head_dim 64 and 128)
+            if constexpr (R::kStages == 2) {
+              issue(0, 0);
             } else {
-              i4_wait<0>();
+#pragma unroll 1
+              for (int k = 0; k < min(R::kStages - 1, np); ++k) issue(k, k);
             }
-            if constexpr (kF32Q)
-              i4_pair32<D, KV>(ring + at * R::kStage, il, qraw, a.qk_scale, left(2 * k), left(2 * k + 1), lane16, grp, st);
-            else
-              i4_pair<D, KV>(ring + at * R::kStage, il, ic, qi, left(2 * k), left(2 * k + 1), lane16, grp, st);
-            at = at + 1 == R::kStages ? 0 : at + 1;
-          }
+            if constexpr (!kF32Q) i4_prep_q<D, KV, QT>(a, qraw, lane16, grp, qi);
+            int at = 0;                                    // stage of pair k
+            for (int k = 0; k < np; ++k) {
+              const int kn = k + R::kStages - 1;
+              if ((kn & 31) == 0 && kn < np) {
+                pgw = page_window(2 * kn);
+                asm volatile("" ::"v"(pgw));               // (waited for here, not by every round at its readlane)
+              }
+              if (kn < np) {
+                issue(kn, at == 0 ? R::kStages - 1 : at - 1);
+                i4_wait<(R::kStages - 1) * R::kTransfers>();
+              } else if (R::kStages > 2 && k + 1 < np) {   // (one pair behind this one)
+                i4_wait<R::kTransfers>();
+              } else {
+                i4_wait<0>();
+              }
+              if constexpr (kF32Q)
+                i4_pair32<D, KV>(ring + at * R::kStage, il, qraw, a.qk_scale, left(2 * k), left(2 * k + 1), lane16, grp, st);
+              else
+                i4_pair<D, KV>(ring + at * R::kStage, il, ic, qi, left(2 * k), left(2 * k + 1), lane16, grp, st);
+              at = at + 1 == R::kStages ? 0 : at + 1;
+            }
           }
           if constexpr (i4_half<KV>()) i4_join<D>(st);
         }
@@ -1202,12 +1203,12 @@ void decode_main(const DecodeArgs a) {
                     f32x4{st.acc[e][i] * inv, st.acc[e + 1][i] * inv, st.acc[e + 2][i] * inv, st.acc[e + 3][i] * inv};
           } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int e = 0; e < E; e += 2) {
-              const uint32_t w = pack2(QT{}, st.acc[e][i] * inv, st.acc[e + 1][i] * inv);
-              *(uint32_t*)(op + out_d<D, KV>(grp, i, e) * 2) = w;
-            }
+              for (int e = 0; e < E; e += 2) {
+                const uint32_t w = pack2(QT{}, st.acc[e][i] * inv, st.acc[e + 1][i] * inv);
+                *(uint32_t*)(op + out_d<D, KV>(grp, i, e) * 2) = w;
+              }
           }
         } else {
           float* dst = a.ws_acc + (pslot + lane16) * D;
@@ -1459,13 +1460,13 @@ __global__ __launch_bounds__(PW * 64) void decode_reduce(const DecodeArgs a) {
   }
   if (!work) return;
   const float inv = 1.0f / (L == 0.f ? 1.f : L);
+  char* orow = a.out + b * a.o_sb + (int64_t)hq * a.o_sh;
   if constexpr (std::is_same<OT, F32>::value) {
-    *(f32x4*)(a.out + b * a.o_sb + (int64_t)hq * a.o_sh + 4 * li * (int)sizeof(float)) = A * inv;
-    return;
+    *(f32x4*)(orow + 4 * li * (int)sizeof(float)) = A * inv;
   } else {
-  char* op = a.out + b * a.o_sb + (int64_t)hq * a.o_sh + 4 * li * (int)sizeof(uint16_t);
-  *(uint32_t*)op = pack2(OT{}, A[0] * inv, A[1] * inv);
-  *(uint32_t*)(op + 4) = pack2(OT{}, A[2] * inv, A[3] * inv);
+    char* op = orow + 4 * li * (int)sizeof(uint16_t);
+    *(uint32_t*)op = pack2(OT{}, A[0] * inv, A[1] * inv);
+    *(uint32_t*)(op + 4) = pack2(OT{}, A[2] * inv, A[3] * inv);
   }
 }
 

@@ -337,3 +337,31 @@ def test_strides_of_dims_of_one(gpu_pkg):
     x = gpu_pkg.kv_read(c.kc, vc, S, c.ks, vs)
     y = gpu_pkg.kv_read(c.kc, c.vc, S, c.ks, c.vs)
     assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,group,T,table", [(16, 16, 20, FP32), (32, 32, 3, BF16), (64, 32, 33, FP32), (128, 128, 17, FP16),
+                                             (256, 32, 16, FP32)])
+def test_rope_write_positions(gpu_pkg, D, group, T, table, interleaved):
+    """Sequences at their own positions, paged, long and short writes, tables of other types: RoPE, then the plain write.
+    Positions past the table are not written."""
+    announce(f"rope_kv_write int4 D {D} T {T} table {table} interleaved {interleaved}")
+    B, Hq, H, page, rows = 3, 4, 2, 24, 60
+    g = gen(D + T)
+    dt = FP16 if table == FP16 else BF16
+    q, k, v = randn(g, B, T, Hq, D, dtype=dt), randn(g, B, T, H, D, dtype=dt), randn(g, B, T, H, D, dtype=dt)
+    cos, sin = gpu_pkg.RopeFrequencies(D, rows, device=torch.device(DEV)).get(rows, dtype=table)
+    first = [0, 7, rows - 2]
+    bt = torch.randperm(12, generator=torch.Generator().manual_seed(D))[:9].view(3, 3).to(torch.int32).to(DEV)
+    (kc, ks), (vc, vs), (kc2, ks2), (vc2, vs2) = (pools(12, H, page, D, group) for _ in range(4))
+    qr = gpu_pkg.rope_kv_write(q, k, v, cos, sin, kc, vc, ks, vs, block_table=bt, start_pos=lens_tensor(first),
+                               page_size=page, interleaved=interleaved)
+    for b, at in enumerate(first):
+        n = min(T, rows - at)
+        q2, k2 = gpu_pkg.rope_triton(q[b:b + 1, :n], k[b:b + 1, :n], cos[at:at + n], sin[at:at + n], interleaved=interleaved)
+        assert torch.equal(qr[b:b + 1, :n], q2) and not qr[b, n:].any()
+        gpu_pkg.kv_write(k2.transpose(1, 2).contiguous(), v[b:b + 1, :n].transpose(1, 2).contiguous(), kc2,
+                         vc2, ks2, vs2, block_table=bt[b:b + 1], start_offset=at, page_size=page)
+    torch.cuda.synchronize()
+    for x, y in ((kc, kc2), (ks, ks2), (vc, vc2), (vs, vs2)):
+        assert torch.equal(x, y)

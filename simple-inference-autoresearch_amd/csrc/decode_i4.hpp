@@ -435,7 +435,9 @@ __device__ __forceinline__ float i4_above(float s, float mul, float m) {
 
 // Online softmax of NS x 4 scores per lane: weights p (the running maximum
 // moves lazily, as in compute_tile).  A score of -inf weighs 0, also before any
-// other was seen.
+// other was seen.  The threshold is compared with the difference, which is exact
+// where it matters: the sum st.m + 8 rounds up to st.m + 16 from 2^27 on, and a
+// weight of 2^16 is an infinity in fp16.
 template <int D, int NS>
 __device__ __forceinline__ void i4_softmax(const float (&s)[NS][4], float mul, bool masked, WaveState<D>& st,
                                            float (&p)[NS][4]) {
@@ -443,7 +445,7 @@ __device__ __forceinline__ void i4_softmax(const float (&s)[NS][4], float mul, b
 #pragma unroll
   for (int n = 0; n < NS; ++n) lmax = fmaxf(lmax, fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3])));
   lmax *= mul;
-  if (__any(lmax > st.m + kLazyMax)) {
+  if (__any(lmax - st.m > kLazyMax)) {
     const float m_new = fmaxf(st.m, wave_max_xor16_32(lmax));
     const float alpha = fast_exp2(st.m - (m_new == -INFINITY ? 0.f : m_new));
     st.m = m_new;

@@ -433,20 +433,35 @@ __device__ __forceinline__ float i4_above(float s, float mul, float m) {
   return x - m;
 }
 
+// The weights of 16-bit queries enter the matrix cores in fp16.  Their
+// reference st.m stands kI4Lift below the running maximum when that moves, and
+// a score moves it from kI4Lazy above on, so that the largest weight is 2^11 to
+// 2^15.  One of w times the largest is then rounded by at most 2^-11 w + 2^-36.
+// (With the maximum itself for reference the second term is 2^-25: tokens
+// behind a sink, each 2^-20 of its weight, came out up to 3% off.)
+constexpr float kI4Lift = 11.0f, kI4Lazy = 4.0f;
+
 // Online softmax of NS x 4 scores per lane: weights p (the running maximum
 // moves lazily, as in compute_tile).  A score of -inf weighs 0, also before any
 // other was seen.  The threshold is compared with the difference, which is exact
-// where it matters: the sum st.m + 8 rounds up to st.m + 16 from 2^27 on, and a
-// weight of 2^16 is an infinity in fp16.
-template <int D, int NS>
+// where it matters: a sum st.m + 8 rounds up to st.m + 16 from 2^27 on, and a
+// weight of 2^16 is an infinity in fp16.  LIFTED: p goes into fp16 (a reference
+// that the subtraction rounds further down stays at the maximum).
+template <int D, int NS, bool LIFTED>
 __device__ __forceinline__ void i4_softmax(const float (&s)[NS][4], float mul, bool masked, WaveState<D>& st,
                                            float (&p)[NS][4]) {
+  constexpr float kMost = LIFTED ? kI4Lift + kI4Lazy : kLazyMax;
   float lmax = -INFINITY;
 #pragma unroll
   for (int n = 0; n < NS; ++n) lmax = fmaxf(lmax, fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3])));
   lmax *= mul;
-  if (__any(lmax - st.m > kLazyMax)) {
-    const float m_new = fmaxf(st.m, wave_max_xor16_32(lmax));
+  if (__any(lmax - st.m > kMost)) {
+    float ref = wave_max_xor16_32(lmax);
+    if constexpr (LIFTED) {
+      const float low = ref - kI4Lift;
+      ref = ref - low > kMost ? ref : low;
+    }
+    const float m_new = fmaxf(st.m, ref);
     const float alpha = fast_exp2(st.m - (m_new == -INFINITY ? 0.f : m_new));
     st.m = m_new;
     st.l *= alpha;
@@ -567,7 +582,7 @@ __device__ __forceinline__ void i4_pair(const char* stage, const I4Lane<D, KV>& 
           for (int g = 0; g < I4Tile<D, KV>::NV; ++g) v[t].p[i].w[g] = 0u;
         }
   }
-  i4_softmax<D, NS>(s, q.mul, masked, st, p);
+  i4_softmax<D, NS, true>(s, q.mul, masked, st, p);
   u32x4 pop;
   if constexpr (KV::half) {
     const u32x2 w = {pack2(F16{}, p[0][0], p[0][1]), pack2(F16{}, p[0][2], p[0][3])};
@@ -649,7 +664,7 @@ __device__ __forceinline__ void i4_pair32(const char* stage, const I4Lane<D, KV>
           for (int g = 0; g < C::NV; ++g) v[t].p[i].w[g] = 0u;
         }
   }
-  i4_softmax<D, 2>(s, mul, masked, st, p);
+  i4_softmax<D, 2, false>(s, mul, masked, st, p);
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll

@@ -1,7 +1,9 @@
 """Softmax weights of the 4-bit decode at the ends of fp16's range, which the matrix cores take them in.
 
-A weight's rounding to fp16 is off by at most 2^-11 of it, and so is a value's.  (Scores here are exact in fp32, so that
-no other error is left but the fp32 sums'.)
+A weight w, relative to its wave's largest one, enters as p = 2^s w for some s >= 11.  Its rounding to fp16 is off by at
+most 2^-11 p where p is normal and by 2^-25 where it is a denormal, that is by 2^-11 w + 2^-36.  A value's rounding is off
+by 2^-11 of it.  The scores are products of few bits: their factor (twice), the product and its difference to the reference
+round once each, by 2^-24 of the spread of the scores, or are exact.  Sums are in fp32.
 """
 
 from __future__ import annotations
@@ -13,20 +15,21 @@ import pytest
 import torch
 
 from helpers import announce, f64, ulp
-from test_int4_gpu import BF16, DEV, cache_case
+from test_int4_gpu import BF16, DEV, FP16, cache_case
 
 pytestmark = pytest.mark.gpu
 
 
-def check(out, weights, v, what):
-    """out (Hq, D) against ``weights`` (n,), the largest 1, over exact values v (H, n, D)."""
+def check(out, weights, v, what, spread=0.0):
+    """out (Hq, D) against ``weights`` (n,), the largest 1, over exact values v (H, n, D); ``spread`` of the scores in
+    log2 units, 0 where they are exact."""
     n, G = len(weights), out.shape[0] // v.shape[0]
     got = f64(out)
     total = weights.sum()
     for h in range(v.shape[0]):
         ref, wabs = weights @ v[h] / total, weights @ np.abs(v[h]) / total
-        # (sums of n weights and products in fp32, in the numerator and in the normaliser)
-        bound = (2.0 ** -10 + 2 * (n / 4 + 74) * 2.0 ** -24) * wabs
+        # (scores, and sums of n weights and products in fp32: in the numerator and in the normaliser)
+        bound = (2.0 ** -10 + 2 * (4 * spread + n / 4 + 74) * 2.0 ** -24) * wabs + 2.0 ** -36 * np.abs(v[h]).sum(0) / total
         allowed = bound + 0.5 * ulp(np.abs(ref) + bound, out.dtype)
         for x in got[h * G:(h + 1) * G]:
             assert np.isfinite(x).all(), f"{what}: non-finite output"
@@ -63,3 +66,44 @@ def test_maxima_that_grow_at_the_end_of_fp32(gpu_pkg, D, group, page, G, step):
     torch.cuda.synchronize()
     jj = j.cpu().numpy().astype(np.float64)
     check(out[0, 0], 2.0 ** (16 * (jj - jj.max())), v[0], f"step {step}")
+
+
+@pytest.mark.parametrize("D,group,page,qdt", [(64, 32, 0, FP16), (128, 64, 16, BF16), (256, 128, 16, BF16),
+                                              (128, 64, 24, BF16)])
+@pytest.mark.parametrize("G", [4, 12])
+@pytest.mark.parametrize("gap", [13.3, 19.5, 24.4, 25.05, 30.3])
+def test_attention_sink(gpu_pkg, D, group, page, qdt, G, gap):
+    """The first token's weight is 2^gap times every other's, its value zero: the others' weights make the result."""
+    announce(f"int4 decode sink D {D} page {page} G {G} gap {gap}")
+    H, n = 8, 9000
+    c = cache_case(gpu_pkg, D, 2, H, D, group, n, page)
+    c.k[:] = 0
+    c.k[:, :, 0] = 1
+    c.v[:, :, 0] = 0
+    _, v = c.fill(gpu_pkg, [n, 1])
+    q = torch.ones(1, G * H, 1, D, dtype=qdt, device=DEV)
+    out = one_share(gpu_pkg, c, q, n, gap * math.log(2) / D)
+    torch.cuda.synchronize()
+    weights = np.full(n, 2.0 ** -gap)
+    weights[0] = 1
+    check(out[0, 0], weights, v[0], f"gap {gap}", gap)
+
+
+@pytest.mark.parametrize("D,group,page", [(64, 64, 16), (128, 32, 0), (256, 64, 16), (64, 32, 24)])
+@pytest.mark.parametrize("G", [4, 12])
+@pytest.mark.parametrize("growth", [0.5, 3.9375, 4.0625, 7.9375, 15.0])
+def test_scores_that_grow_along_the_sequence(gpu_pkg, D, group, page, G, growth):
+    """Every pair of tiles ``growth`` log2 units above the one before, values up to fp16's largest: weights above the
+    running maximum stay inside fp16."""
+    announce(f"int4 decode growing scores D {D} page {page} G {G} growth {growth}")
+    H, n = 8, 32 * 12
+    c = cache_case(gpu_pkg, D + 1, 2, H, D, group, n, page)
+    # one value a row: the minimum of every group, step 0
+    c.k[:] = (torch.arange(n, device=DEV) // 32).to(BF16)[:, None]
+    c.v[..., ::5] = 65280.0
+    _, v = c.fill(gpu_pkg, [n, 1])
+    q = torch.ones(1, G * H, 1, D, dtype=BF16, device=DEV)
+    out = one_share(gpu_pkg, c, q, n, growth * math.log(2) / D)
+    torch.cuda.synchronize()
+    pair = np.arange(n) // 32
+    check(out[0, 0], 2.0 ** (growth * (pair - pair.max())), v[0], f"growth {growth}", 11 * growth)

@@ -54,13 +54,20 @@ int check_scale(const sia_tensor* s, const sia_tensor* like, const char* name) {
 
 bool head_dim_ok(int64_t D) { return D == 16 || D == 32 || D == 64 || D == 128 || D == 256; }
 
+// Whether two descriptors of one shape have the same strides; a dim of size 1 has none to compare.
+bool strides_alike(const sia_tensor* k, const sia_tensor* v) {
+  for (int d = 0; d < k->ndim; ++d)
+    if (k->shape[d] > 1 && v->stride[d] != k->stride[d]) return false;
+  return true;
+}
+
 // k and v descriptors that are read or written through one set of strides.
 int check_alike(const sia_tensor* k, const sia_tensor* v, const char* kn, const char* vn) {
   if (v->dtype != k->dtype || v->ndim != k->ndim)
     return fail(SIA_ERR_INVALID_ARGUMENT, "%s and %s must have one dtype and rank", kn, vn);
-  for (int d = 0; d < k->ndim; ++d)
-    if (v->shape[d] != k->shape[d] || (k->shape[d] > 1 && v->stride[d] != k->stride[d]))
-      return fail(SIA_ERR_INVALID_ARGUMENT, "%s and %s must have the same shape and strides", kn, vn);
+  bool alike = strides_alike(k, v);
+  for (int d = 0; d < k->ndim; ++d) alike = alike && v->shape[d] == k->shape[d];
+  if (!alike) return fail(SIA_ERR_INVALID_ARGUMENT, "%s and %s must have the same shape and strides", kn, vn);
   return SIA_OK;
 }
 
@@ -113,7 +120,7 @@ int setup_kv_write(const sia_tensor* k, const sia_tensor* v, const sia_tensor* k
     if (v->dtype != k->dtype) return fail(SIA_ERR_INVALID_ARGUMENT, "k and v dtypes differ");
     for (int d = 0; d < 4; ++d)
       if (v->shape[d] != k->shape[d]) return fail(SIA_ERR_INVALID_ARGUMENT, "k and v shapes differ");
-    if (bstride(v, 0) != bstride(k, 0) || bstride(v, 1) != bstride(k, 1) || bstride(v, 2) != bstride(k, 2))
+    if (!strides_alike(k, v))
       return fail(SIA_ERR_INVALID_ARGUMENT, "k and v must have the same strides");
   }
   const int64_t B = k->shape[0], H = k->shape[1], T = k->shape[2], D = k->shape[3];
@@ -129,8 +136,7 @@ int setup_kv_write(const sia_tensor* k, const sia_tensor* v, const sia_tensor* k
     if (v_dst->dtype != dd) return fail(SIA_ERR_INVALID_ARGUMENT, "k_dst and v_dst dtypes differ");
     for (int d = 0; d < 4; ++d)
       if (v_dst->shape[d] != k_dst->shape[d]) return fail(SIA_ERR_INVALID_ARGUMENT, "k_dst and v_dst shapes differ");
-    if (bstride(v_dst, 0) != bstride(k_dst, 0) || bstride(v_dst, 1) != bstride(k_dst, 1) ||
-        bstride(v_dst, 2) != bstride(k_dst, 2))
+    if (!strides_alike(k_dst, v_dst))
       return fail(SIA_ERR_INVALID_ARGUMENT, "k_dst and v_dst must have the same strides");
   }
   const int64_t row = int4 ? i4_code_bytes(D) : D;
@@ -149,8 +155,7 @@ int setup_kv_write(const sia_tensor* k, const sia_tensor* v, const sia_tensor* k
     if ((rc = check_scale(k_scale_dst, k_dst, "k_scale_dst"))) return rc;
     if (two) {
       if ((rc = check_scale(v_scale_dst, k_dst, "v_scale_dst"))) return rc;
-      if (v_scale_dst->dtype != k_scale_dst->dtype || v_scale_dst->stride[0] != k_scale_dst->stride[0] ||
-          v_scale_dst->stride[1] != k_scale_dst->stride[1] || v_scale_dst->stride[2] != k_scale_dst->stride[2])
+      if (v_scale_dst->dtype != k_scale_dst->dtype || !strides_alike(k_scale_dst, v_scale_dst))
         return fail(SIA_ERR_INVALID_ARGUMENT, "k_scale_dst and v_scale_dst must share dtype and strides");
     }
   } else if (dd != SIA_F16 && dd != SIA_BF16 && dd != SIA_F32) {

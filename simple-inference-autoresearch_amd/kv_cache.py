@@ -70,6 +70,8 @@ def kv_read(k_src: torch.Tensor, v_src: torch.Tensor | None, length: int, k_scal
     ``v_src`` is.
     """
     ko, vo = (None, None) if out is None else out
+    if out is not None and ko is None:
+        raise ValueError("out must be a (k, v) pair of tensors, v None exactly where v_src is")
     return _lib.gpu_ops().kv_read(k_src, v_src, length, k_scale, v_scale, block_table, start_pos, start_offset,
                                   page_size, dtype, ko, vo)
 

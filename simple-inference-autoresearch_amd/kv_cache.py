@@ -149,6 +149,11 @@ def int4_pools(rows: tuple, head_dim: int, group: int, device):
             torch.zeros(*rows, 2 * head_dim // group, dtype=torch.float16, device=device))
 
 
+def pools_bytes(k: torch.Tensor, k_params: torch.Tensor | None) -> int:
+    """Bytes of a K pool, its parameters if given, and the same again for V."""
+    return 2 * sum(t.numel() * t.element_size() for t in (k, k_params) if t is not None)
+
+
 def _int32_positions(pos: torch.Tensor) -> torch.Tensor:
     """Device positions as int32 (the reference's ctx.pos_index is int64)."""
     if pos.dtype == torch.int32:
@@ -270,8 +275,12 @@ class KVCache:
         return
 
     def bytes(self) -> int:
-        """Total footprint of the K and V pools in bytes."""
-        return 2 * self.k_cache.numel() * self.k_cache.element_size()
+        """Total footprint of the K and V pools in bytes.
+
+        4-bit pools with their parameters, which are 6 to 25% on top of the
+        codes; int8 ones without their scales.
+        """
+        return pools_bytes(self.k_cache, self.k_scale if self.is_int4 else None)
 
     def __repr__(self) -> str:
         gb = self.bytes() / 1e9

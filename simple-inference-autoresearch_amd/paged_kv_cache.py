@@ -30,7 +30,7 @@ import torch
 
 from . import _lib
 from .decode import PAGED, PAGED_INT4, PAGED_INT8, _common, _run_layer
-from .kv_cache import int4_group, int4_pools, kv_read, kv_write
+from .kv_cache import int4_group, int4_pools, kv_read, kv_write, pools_bytes
 
 
 class PagedKVCache:
@@ -160,7 +160,7 @@ class PagedKVCache:
                        dtype=dtype if dtype is not None or out is not None else self.dtype, out=out)
 
     def __repr__(self):
-        gb = 2 * self.k_pool.numel() * self.k_pool.element_size() / 1e9
+        gb = pools_bytes(self.k_pool, self.k_scale_pool if self.is_int4 else None) / 1e9
         return (f"PagedKVCache(layers={self.n_layers}, blocks={self.num_blocks}, block_size={self.block_size}, "
                 f"max_batch={self.max_batch}, max_seq_len={self.max_seq_len}, kv_dtype={self.kv_dtype}, "
                 f"vram={gb:.2f} GB)")

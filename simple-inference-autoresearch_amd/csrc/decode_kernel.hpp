@@ -290,7 +290,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const char* p) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, -1, kRawBufferFlags);
 }
 
-// BYTES at rsrc + off (BYTES a multiple of 16, or 8, 4 or 2); 16-byte pieces
+// BYTES at rsrc + off (BYTES a multiple of 16, or 8 or 4); 16-byte pieces
 // STRIDE bytes apart.
 template <int BYTES, int STRIDE = 16>
 __device__ __forceinline__ void load_raw_buf(Raw<BYTES>& r, __amdgpu_buffer_rsrc_t rs, uint32_t off) {
@@ -303,8 +303,6 @@ __device__ __forceinline__ void load_raw_buf(Raw<BYTES>& r, __amdgpu_buffer_rsrc
   } else if constexpr (BYTES == 8) {
     const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rs, off, 0, kLoadNT);
     r.w[0] = x[0]; r.w[1] = x[1];
-  } else if constexpr (BYTES == 2) {
-    r.w[0] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, kLoadNT);
   } else {
     static_assert(BYTES == 4, "tile operand size");
     r.w[0] = __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, kLoadNT);

@@ -95,6 +95,13 @@ def rope_kv_write(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor | Non
                                         start_pos, int(start_offset), int(page_size), bool(interleaved), q_out)
 
 
+def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
+    """``x`` if its rows are contiguous and 16-byte aligned, else a copy (a contiguous view may start anywhere)."""
+    if x.stride(-1) == 1 and all((s * x.element_size()) % 16 == 0 for s in x.stride()[:-1]) and x.data_ptr() % 16 == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
 def quantize_kv_int8(x: torch.Tensor, scale_dtype: torch.dtype = torch.float16):
     """Per-(..., head_dim) symmetric int8 quantisation of a K or V tensor.
 
@@ -107,9 +114,7 @@ def quantize_kv_int8(x: torch.Tensor, scale_dtype: torch.dtype = torch.float16):
     ops = _lib.gpu_ops()
     if scale_dtype not in (torch.float16, torch.float32):
         raise ValueError("scale_dtype must be float16 or float32")
-    src = x if x.stride(-1) == 1 and all((s * x.element_size()) % 16 == 0 for s in x.stride()[:-1]) \
-        and x.data_ptr() % 16 == 0 else x.contiguous()
-    return ops.quantize_kv_int8(src, scale_dtype == torch.float32)
+    return ops.quantize_kv_int8(_aligned_rows(x), scale_dtype == torch.float32)
 
 
 def quantize_kv_int4(x: torch.Tensor, group_size: int = 64):
@@ -126,9 +131,7 @@ def quantize_kv_int4(x: torch.Tensor, group_size: int = 64):
     """
     ops = _lib.gpu_ops()
     g = int4_group(x.shape[-1], group_size)
-    src = x if x.stride(-1) == 1 and all((s * x.element_size()) % 16 == 0 for s in x.stride()[:-1]) \
-        and x.data_ptr() % 16 == 0 else x.contiguous()
-    return ops.quantize_kv_int4(src, g)
+    return ops.quantize_kv_int4(_aligned_rows(x), g)
 
 
 def dequantize_kv_int4(codes: torch.Tensor, params: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:

@@ -151,9 +151,12 @@ int sia_paged_gqa_int8_flash_decode(const sia_tensor* q, const sia_tensor* k_poo
  * f16, 4-byte aligned rows.  q f16|bf16|f32.  k and v have the same strides, and
  * so do their parameters (SIA_ERR_UNSUPPORTED otherwise: the kernels compute
  * every offset once for both).  16-bit q at head_dim 64 and more runs on the
- * matrix cores whatever the page size, unless a pool is 4 GiB or larger and its
- * pages are not of 16 * 2^k tokens; large calls with f32 q on the fp32 matrix
- * cores; everything else on the vector ALUs. */
+ * matrix cores whatever the page size, in batches of up to 8192, unless a pool
+ * is 4 GiB or larger and its pages are not of 16 * 2^k tokens; large calls with
+ * f32 q on the fp32 matrix cores, in such batches and pages of 16 * 2^k tokens;
+ * everything else on the vector ALUs.  The matrix cores take 16-bit q's weights
+ * and the values in fp16: each is off by at most 2^-11 of it, a weight by 2^-36
+ * of the largest besides.  The vector ALUs and f32 q keep fp32. */
 int sia_attention_flash_decode_int4(const sia_tensor* q, const sia_tensor* k_int4, const sia_tensor* v_int4,
                                     const sia_tensor* k_scale, const sia_tensor* v_scale,
                                     const sia_tensor* kv_len, float sm_scale, const sia_tensor* out,

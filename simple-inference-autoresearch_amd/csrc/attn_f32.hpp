@@ -8,11 +8,12 @@
 // The 16-bit MFMA kernels of this library take 16-bit, int8 or int4 operands,
 // so float32 inputs run here instead, in fp32 end to end: products, sums,
 // exponentials and the output (rounded to q's dtype).  int4 caches do at
-// head_dim 16 and 32 too, in pools of 4 GiB and more whose pages hold no
-// 16 x 2^k tokens, with float32 queries in such pages at all, and with float32
-// queries where a call is small (f32_matrix in capi_decode.cpp); their values
-// are formed in fp32, each rounded once.  (4 x 512 tokens, 32/8 heads of 64,
-// 9.1 us.)
+// head_dim 16 and 32 too, in batches beyond 8192 sequences, in pools of 4 GiB
+// and more whose pages hold no 16 x 2^k tokens, with float32 queries in such
+// pages at all, and with float32 queries where a call is small (f32_matrix in
+// capi_decode.cpp); their values are formed in fp32, each rounded once.  (4 x
+// 500 tokens, 32/8 heads of 64, fp32 queries: 8.7 us; 32 sequences of 100-4000
+// tokens, 32/8 heads, bf16 queries: 48 us at head_dim 32, 35 at 16.)
 //
 // attn_f32 (gfx950, wave64):
 //  * A work item is one (sequence, KV head), up to kF32Cols of its query heads

@@ -67,12 +67,14 @@ int geometry(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, Geometry& g) {
 // by side and the waves of a wide item read them together; narrower items
 // that still leave a split ran config 2's main kernel 2-2.5 us (7%) slower.
 //
-// int4 goes by the lengths instead, paged or not.  One shared length: the
-// halved IU (8 x 3000 tokens 16.7 us against 17.8, one sequence of 8192 13.9
-// against 18.3; 32/8 heads, D 128).  Lengths of their own: wide items, since
+// int4 goes by how kv_len is given instead, paged or not.  One shared length:
+// the halved IU (8 x 3000 tokens 16.7 us against 17.8, one sequence of 8192 13.9
+// against 18.3; 32/8 heads, D 128).  A length per sequence: wide items, since
 // each of the many segments of a narrow split starts its ring anew (64 requests
 // of 100-8000 tokens 69.8 us at 8 units, 79.8 at 4, 90.1 at 2, 134.4 at 1; 16 of
-// up to 4096, 16/16 heads, D 64, 24.5, 33.9, 49.7, 76.9).
+// up to 4096, 16/16 heads, D 64, 24.5, 33.9, 49.7, 76.9).  Lengths that are
+// equal all the same pay the wide items' split and merge: 64 x 8192 tokens 112.3
+// us against 108.5, 16 x 4000 25.3 against 23.8.
 void item_units(Geometry& g, bool paged, bool int4, bool ragged) {
   const int nw = decode_waves(g.D);
   const int cus = device_info().cus > 0 ? device_info().cus : 256;
@@ -265,11 +267,25 @@ int prepare_table(const sia_tensor* bt, const Geometry& g, int page_size, Decode
 // int4 and float32 queries: the matrix cores from 150 thousand rows x tokens of
 // capacity on, if two query heads or more share a KV head.  Below, the
 // vector-ALU kernel's shorter start wins, and it does one column's work where
-// the matrix cores do 16.  us, matrix / vector, head_dim 128: 32/8 heads, 4 x
-// 500 tokens 15.8 / 11.2, 4 x 2000 19.2 / 22.5, 64 x 500 31.4 / 48.4, 4 x 8000
-// 35.4 / 52.8; 64/4 heads, 4 x 500 18.0 / 14.2, 16 x 2000 26.0 / 72.3; 16/8
-// heads, 4 x 2000 19.7 / 18.1, 4 x 8000 35.4 / 40.6; 8/8 heads, 4 x 2000 19.2 /
-// 16.4, 16 x 2000 34.6 / 32.6.
+// the matrix cores do 16.  us, matrix / vector, lengths equal to the capacity.
+// One length for all, head_dim 128: 32/8 heads, 4 x 500 tokens 15.8 / 11.2, 4 x
+// 2000 19.2 / 22.5, 64 x 500 31.4 / 48.4, 4 x 8000 35.4 / 52.8; 64/4 heads, 4 x
+// 500 18.0 / 14.2, 16 x 2000 26.0 / 72.3; 16/8 heads, 4 x 2000 19.7 / 18.1, 4 x
+// 8000 35.4 / 40.6; 8/8 heads, 4 x 2000 19.2 / 16.4, 16 x 2000 34.6 / 32.6.  A
+// length per sequence, where the wide items (item_units) cost the matrix cores
+// more at 1000 to 2000 tokens:
+//                       head_dim 64, 32/8   128, 32/8     256, 16/4
+//   4 x 500                 12.0 /  8.7    15.1 / 10.5   16.6 / 13.7
+//   1 x 2000                13.3 / 11.5    17.9 / 13.2   23.0 / 16.7
+//   4 x 2000                18.2 / 16.8    24.8 / 22.1   28.5 / 21.4
+//   16 x 500                13.3 / 14.2    17.9 / 19.6   19.5 / 18.5
+//   1 x 8000                14.1 / 25.5    19.0 / 30.6   24.6 / 30.3
+//   4 x 8000                23.5 / 30.5    35.6 / 49.4   39.7 / 57.4
+// (The rule's worst picks: 64/4 heads of 128, 4 x 1000, 33.5 / 17.9 and 16/8 of
+// 64, 1 x 8000, 13.7 / 23.0.)  It goes by the capacity because the vector kernel
+// does: that cuts the capacity into its pieces, the lengths being on the device,
+// and a short sequence in a long cache costs it most.  One sequence of 100 tokens
+// in 32768, 32/8 heads of 128: 13.3 / 30.2; 16 of 500 in 4096: 17.8 / 78.9.
 bool f32_matrix(const Geometry& g, int cap) { return g.G >= 2 && (int64_t)g.B * g.Hq * cap >= 150000; }
 
 // The matrix kernels keep 4 bytes per sequence in LDS beside up to 127 KB of

@@ -45,7 +45,8 @@ typedef enum sia_dtype {
   SIA_I8 = 3,
   SIA_I32 = 4,
   SIA_I64 = 5,
-  SIA_U8 = 6
+  SIA_U8 = 6,
+  SIA_F64 = 7
 } sia_dtype;
 
 typedef enum sia_status {
@@ -245,6 +246,51 @@ int sia_prefill_workspace_size(int64_t batch, int64_t kv_heads, int64_t kv_len, 
  * workspace such a call runs unsplit. */
 int sia_attention_flash_fwd_workspace_size(const sia_tensor* q, const sia_tensor* k, size_t* bytes);
 
+/* ------------------------------------------------- scored attention */
+
+/* Attention whose scores are shaped and whose keys are masked (no counterpart
+ * in the reference, which has the scale and the causal mask alone).  A query
+ * at position p of its sequence b sees key j, in query head h, with the score
+ *   x = sm_scale q . k;   x = softcap tanh(x / softcap);   x -= alibi_slopes[h] |p - j|
+ * where  kv_start[b] <= j < kv_len[b],  |p - j| < window,  p and j lie in the
+ * same document (no entry c of cu_seqlens with min(p, j) < c <= max(p, j)) and,
+ * in a causal call, j <= p or j < prefix_len[b].  A query that sees no key
+ * gives zeros; what stands in keys that it does not see (a NaN too) does not
+ * reach it.
+ * Fields left 0 or NULL shape and hide nothing.  Tensors are read on the device:
+ * kv_start, kv_len, prefix_len int32, (1)/() shared or (B); alibi_slopes f32
+ * (Hq); cu_seqlens int32 (n) shared or (B, n), in any order, last stride 1. */
+typedef struct sia_score_options {
+  float softcap;                    /* 0: none */
+  int32_t window;                   /* 0: none */
+  const sia_tensor* alibi_slopes;
+  const sia_tensor* kv_start;
+  const sia_tensor* kv_len;         /* prompts only, as the next two: a decode call has its own kv_len */
+  const sia_tensor* prefix_len;
+  const sia_tensor* cu_seqlens;
+  int64_t reserved[4];              /* must be zero */
+} sia_score_options;
+
+/* Prompts and chunks: q (B,Hq,Tq,D), k, v (B,Hkv,Tk,D), out, layouts, types and
+ * workspace as for sia_attention_flash_fwd (workspace: the size that
+ * sia_scored_attention_flash_fwd_workspace_size reports); query i sits at
+ * position Tk - Tq + i. */
+int sia_scored_attention_flash_fwd(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, int32_t causal,
+                                   float sm_scale, const sia_score_options* score, const sia_tensor* out,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+int sia_scored_attention_flash_fwd_workspace_size(const sia_tensor* q, const sia_tensor* k, size_t* bytes);
+
+/* One decode step, the query at position kv_len[b] - 1: the arguments of
+ * sia_attention_flash_decode (block_table NULL, page_size 0) or
+ * sia_paged_attention_flash_decode over f16|bf16|f32 caches, of their int8
+ * and int4 forms with k_scale and v_scale (NULL otherwise). */
+int sia_scored_attention_flash_decode(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v,
+                                      const sia_tensor* k_scale, const sia_tensor* v_scale,
+                                      const sia_tensor* block_table, const sia_tensor* kv_len, int32_t page_size,
+                                      float sm_scale, const sia_score_options* score, const sia_tensor* out,
+                                      void* workspace, size_t workspace_bytes, const sia_decode_options* opts,
+                                      void* stream);
+
 /* ------------------------------------------------------------ KV write path */
 
 /* Replaces quantize_kv_int8 (model/kv_cache.py:58-67): per-vector symmetric
@@ -362,6 +408,21 @@ int sia_rope_kv_write(const sia_tensor* q, const sia_tensor* k, const sia_tensor
  * multiply-add), then rounded to the output dtype (nearest even). */
 int sia_rope_qk(const sia_tensor* q, const sia_tensor* k, const sia_tensor* cos, const sia_tensor* sin,
                 int32_t interleaved, const sia_tensor* q_out, const sia_tensor* k_out, void* stream);
+
+/* Rotary positions from frequencies, of the first rotary_dim elements of each
+ * head (no counterpart in the reference, whose tables cover whole heads).
+ * q (B, T, Hq, D), k (B, T, Hkv, D) or NULL, f16|bf16|f32, any strides with
+ * head_dim contiguous; positions int32 or int64 (T) or (B, T); inv_freq
+ * (rotary_dim / 2) f32 or f64, contiguous.  Pair i, elements (i, i +
+ * rotary_dim / 2) or, interleaved, (2 i, 2 i + 1), is turned by the angle
+ * position x inv_freq[i] and multiplied by scale; elements from rotary_dim on
+ * are copied.  Angles are reduced to one turn in 64-bit integers, exact for any
+ * position, and their sines and cosines are off by at most 2^-23; products and
+ * sums in fp32, one rounding to the output type.  q_out, k_out: the inputs'
+ * shapes and types, head_dim contiguous. */
+int sia_rope_scaled(const sia_tensor* q, const sia_tensor* k, const sia_tensor* positions, const sia_tensor* inv_freq,
+                    int32_t rotary_dim, int32_t interleaved, float scale, const sia_tensor* q_out,
+                    const sia_tensor* k_out, void* stream);
 
 #ifdef __cplusplus
 }

@@ -25,6 +25,7 @@ from .decode import (
     paged_gqa_int4_flash_decode,
     paged_gqa_int8_flash_decode,
 )
+from .scored import paged_scored_attention_flash_decode, scored_attention_flash, scored_attention_flash_decode
 from .prefill import attention_flash_triton, prefill_workspace_size, rope_attention_flash_triton
 from .kv_cache import (
     KVCache,
@@ -36,7 +37,7 @@ from .kv_cache import (
     rope_kv_write,
 )
 from .paged_kv_cache import PagedKVCache
-from .rope import RopeFrequencies, apply_rope, rope_triton
+from .rope import RopeFrequencies, ScaledRope, apply_rope, rope_scaled, rope_triton
 from .attention import (
     DecodeCtx,
     decode_step_attention,
@@ -55,7 +56,12 @@ __all__ = [
     "apply_rope",
     "rope_decode_step_attention",
     "rope_kv_write",
+    "rope_scaled",
     "rope_triton",
+    "ScaledRope",
+    "paged_scored_attention_flash_decode",
+    "scored_attention_flash",
+    "scored_attention_flash_decode",
     "decode_step_attention",
     "gqa_attention",
     "kv_read",

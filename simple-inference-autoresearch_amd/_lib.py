@@ -32,7 +32,7 @@ EXT_NAME = "_sia_ops"
 EXT_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), EXT_NAME + ".so")
 
 SIA_MAX_DIMS = 5
-SIA_F16, SIA_BF16, SIA_F32, SIA_I8, SIA_I32, SIA_I64, SIA_U8 = range(7)
+SIA_F16, SIA_BF16, SIA_F32, SIA_I8, SIA_I32, SIA_I64, SIA_U8, SIA_F64 = range(8)
 
 SIA_OK = 0
 SIA_ERR_INVALID_ARGUMENT = -1
@@ -49,6 +49,7 @@ _DTYPE_CODES = {
     torch.int32: SIA_I32,
     torch.int64: SIA_I64,
     torch.uint8: SIA_U8,
+    torch.float64: SIA_F64,
 }
 
 
@@ -81,6 +82,21 @@ class DecodeOptions(ctypes.Structure):
 
 
 _P = ctypes.POINTER(SiaTensor)
+
+
+class ScoreOptions(ctypes.Structure):
+    _fields_ = [
+        ("softcap", ctypes.c_float),
+        ("window", ctypes.c_int32),
+        ("alibi_slopes", _P),
+        ("kv_start", _P),
+        ("kv_len", _P),
+        ("prefix_len", _P),
+        ("cu_seqlens", _P),
+        ("reserved", ctypes.c_int64 * 4),
+    ]
+
+
 _VP = ctypes.c_void_p
 _SZ = ctypes.c_size_t
 _F = ctypes.c_float
@@ -107,6 +123,11 @@ _SIGNATURES = {
     "sia_attention_flash_fwd": [_P, _P, _P, _I32, _F, _P, _VP, _SZ, _VP],
     "sia_attention_flash_fwd_rope": [_P, _P, _P, _P, _P, _I32, _P, _I32, _I32, _F, _P, _VP, _SZ, _VP],
     "sia_attention_flash_fwd_workspace_size": [_P, _P, ctypes.POINTER(_SZ)],
+    "sia_scored_attention_flash_fwd": [_P, _P, _P, _I32, _F, ctypes.POINTER(ScoreOptions), _P, _VP, _SZ, _VP],
+    "sia_scored_attention_flash_fwd_workspace_size": [_P, _P, ctypes.POINTER(_SZ)],
+    "sia_scored_attention_flash_decode": [_P, _P, _P, _P, _P, _P, _P, _I32, _F, ctypes.POINTER(ScoreOptions), _P, _VP,
+                                          _SZ, ctypes.POINTER(DecodeOptions), _VP],
+    "sia_rope_scaled": [_P, _P, _P, _P, _I32, _I32, _F, _P, _P, _VP],
     "sia_prefill_workspace_size": [_I64, _I64, _I64, _I64, ctypes.POINTER(_SZ)],
     "sia_attention_flash_decode_int4": [_P, _P, _P, _P, _P, _P, _F, _P, _VP, _SZ,
                                         ctypes.POINTER(DecodeOptions), _VP],

@@ -31,6 +31,7 @@
 //    stay on the device), so one captured graph serves every length.
 #pragma once
 
+#include "score.hpp"
 #include "sia_common.hpp"
 
 namespace sia {
@@ -61,8 +62,15 @@ struct F32Args {
   float* part;                                       // nsplit > 1: [row][split][D + 4] (acc, m, l)
 };
 
+struct F32ScoredArgs : F32Args {
+  ScoreArgs s;
+};
+template <bool SC>
+using F32ArgsOf = std::conditional_t<SC, F32ScoredArgs, F32Args>;
+
 struct F32Launch {
   F32Args a;
+  const ScoreArgs* score;   // launch_attn_f32_scored only
   int D;
   int q_dtype;       // also the output dtype
   int kv_dtype;
@@ -74,6 +82,8 @@ struct F32Launch {
 
 // Launches attn_f32 (and attn_f32_merge when nsplit > 1); implemented in attn_f32.hip.
 int launch_attn_f32(F32Launch& L);
+// The same with L.score's score function (attn_f32_scored.hip).
+int launch_attn_f32_scored(F32Launch& L);
 
 // Prefill of float32 q, k, v on the matrix cores: nchunk = ceil(ncol /
 // kF32TileCols), no split, no paging (attn_f32_prefill.hip).

@@ -8,6 +8,7 @@
 #include "decode_launch.hpp"
 #include "host_util.hpp"
 #include "int4.hpp"
+#include "scored.hpp"
 
 namespace sia {
 const char* last_message();
@@ -371,7 +372,9 @@ int dispatch_f32(const DecodeLaunch& D, const Geometry& g, int kv_dtype, const s
   // workspace
   const int64_t rows = (int64_t)g.B * g.Hq;
   const int64_t base = (int64_t)g.B * g.Hkv * a.nchunk;
-  const int64_t cap = a.cap > 0 ? a.cap : 1;
+  // (keys that a sequence can see)
+  const int64_t most_keys = D.score != nullptr && D.score->window < a.cap ? D.score->window : a.cap;
+  const int64_t cap = most_keys > 0 ? most_keys : 1;
   int64_t tps;
   if (d.tps_force > 0) {
     tps = (int64_t)d.tps_force * kTile;
@@ -412,7 +415,8 @@ int dispatch_f32(const DecodeLaunch& D, const Geometry& g, int kv_dtype, const s
   L.stream = D.stream;
   L.begin_event = D.begin_event;
   L.end_event = D.end_event;
-  return launch_attn_f32(L);
+  L.score = D.score;
+  return L.score != nullptr ? launch_attn_f32_scored(L) : launch_attn_f32(L);
 }
 
 int dispatch(DecodeLaunch& L, int kv_dtype) {
@@ -428,7 +432,8 @@ int dispatch(DecodeLaunch& L, int kv_dtype) {
 int decode_any(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, const sia_tensor* ks,
                const sia_tensor* vs, const sia_tensor* bt, const sia_tensor* kv_len, int page_size,
                float sm_scale, const sia_tensor* out, void* ws, size_t ws_bytes,
-               const sia_decode_options* opts, void* stream, int want) {   // want: SIA_I8, SIA_U8 (int4) or 0
+               const sia_decode_options* opts, void* stream, int want,   // want: SIA_I8, SIA_U8 (int4) or 0
+               const ScoreArgs* score = nullptr) {
   DecodeLaunch L;
   memset(&L, 0, sizeof(L));
   Geometry g;
@@ -455,6 +460,8 @@ int decode_any(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, co
   L.stream = (hipStream_t)stream;
   L.ws = ws;
   L.ws_bytes = ws_bytes;
+  L.score = score;
+  if (score != nullptr) return dispatch_f32(L, g, k->dtype, out);
   // pages that do not hold whole 16-token tiles (page sizes 1-8, or any size
   // other than 16 * 2^k) go to the vector-ALU path with its per-token lookup
   bool tiled_pages = bt == nullptr || (kTile << L.a.lg_tiles_per_page) == page_size;
@@ -619,6 +626,24 @@ int sia_paged_gqa_int4_flash_decode(const sia_tensor* q, const sia_tensor* k_poo
   if (block_table == nullptr) return fail(SIA_ERR_INVALID_ARGUMENT, "block_table is NULL");
   return decode_any(q, k_pool, v_pool, k_scale_pool, v_scale_pool, block_table, kv_len, page_size, sm_scale,
                     out, workspace, workspace_bytes, opts, stream, SIA_U8);
+}
+
+int sia_scored_attention_flash_decode(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v,
+                                      const sia_tensor* k_scale, const sia_tensor* v_scale,
+                                      const sia_tensor* block_table, const sia_tensor* kv_len, int32_t page_size,
+                                      float sm_scale, const sia_score_options* score, const sia_tensor* out,
+                                      void* workspace, size_t workspace_bytes, const sia_decode_options* opts,
+                                      void* stream) {
+  if (q == nullptr || k == nullptr) return fail(SIA_ERR_INVALID_ARGUMENT, "q or k is NULL");
+  if (q->ndim != 4) return fail(SIA_ERR_INVALID_ARGUMENT, "q must have 4 dims");
+  const int want = k->dtype == SIA_I8 || k->dtype == SIA_U8 ? k->dtype : 0;
+  if (want == 0 && (k_scale != nullptr || v_scale != nullptr))
+    return fail(SIA_ERR_INVALID_ARGUMENT, "k_scale and v_scale belong to int8 and int4 caches");
+  ScoreArgs s;
+  const int rc = fill_score(score, false, q->shape[0], q->shape[1], sm_scale, 1, s);
+  if (rc) return rc;
+  return decode_any(q, k, v, k_scale, v_scale, block_table, kv_len, page_size, sm_scale, out, workspace,
+                    workspace_bytes, opts, stream, want, &s);
 }
 
 }  // extern "C"

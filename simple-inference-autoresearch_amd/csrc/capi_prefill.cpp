@@ -5,6 +5,7 @@
 #include "attn_f32.hpp"
 #include "host_util.hpp"
 #include "prefill_launch.hpp"
+#include "scored.hpp"
 
 using namespace sia;
 
@@ -190,8 +191,31 @@ int setup_rope(const RopeIn& r, int64_t B, int64_t Tq, int64_t D, int q_dtype, P
   return SIA_OK;
 }
 
+// Options of the scored entry point (NULL pointer to this: the plain ones).
+struct ScoreIn {
+  const sia_score_options* options;
+};
+
+// Scored attention one row per wave: any type.
+int scored_rows(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, float sm_scale, const ScoreArgs& s,
+                const sia_tensor* out, void* stream) {
+  ScoredRowsArgs a;
+  memset(&a, 0, sizeof(a));
+  a.q = (const char*)q->data; a.q_sb = bstride(q, 0); a.q_sh = bstride(q, 1); a.q_sm = bstride(q, 2);
+  a.k = (const char*)k->data; a.k_sb = bstride(k, 0); a.k_sh = bstride(k, 1); a.k_sn = bstride(k, 2);
+  a.v = (const char*)v->data; a.v_sb = bstride(v, 0); a.v_sh = bstride(v, 1); a.v_sn = bstride(v, 2);
+  a.out = (char*)out->data; a.o_sb = bstride(out, 0); a.o_sh = bstride(out, 1); a.o_sm = bstride(out, 2);
+  a.B = (int)q->shape[0]; a.Hq = (int)q->shape[1]; a.G = (int)(q->shape[1] / k->shape[1]);
+  a.Tq = (int)q->shape[2]; a.Tk = (int)k->shape[2];
+  a.rows = q->shape[0] * q->shape[1] * q->shape[2];
+  a.qk_scale = sm_scale * kLog2e;
+  a.s = s;
+  return launch_scored_rows(a, (int)q->shape[3], q->dtype, (hipStream_t)stream);
+}
+
 int flash_fwd(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, int32_t causal, float sm_scale,
-              const sia_tensor* out, void* workspace, size_t workspace_bytes, void* stream, const RopeIn* rope) {
+              const sia_tensor* out, void* workspace, size_t workspace_bytes, void* stream, const RopeIn* rope,
+              const ScoreIn* score = nullptr) {
   int rc;
   if ((rc = check4(q, "q")) || (rc = check4(k, "k")) || (rc = check4(v, "v")) || (rc = check4(out, "out"))) return rc;
   if (q->dtype != SIA_F16 && q->dtype != SIA_BF16 && q->dtype != SIA_F32)
@@ -223,6 +247,13 @@ int flash_fwd(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, int
     return fail(SIA_ERR_UNSUPPORTED, "v token stride %lld bytes: expected [%lld, 2^31/64)", (long long)v_sn,
                 (long long)(2 * D));
   if (!(sm_scale > 0.f) || !isfinite(sm_scale)) return fail(SIA_ERR_INVALID_ARGUMENT, "sm_scale must be positive");
+  ScoreArgs sc;
+  if (score != nullptr) {
+    if ((rc = fill_score(score->options, true, B, Hq, sm_scale, causal, sc))) return rc;
+    if ((rc = device_ok())) return rc;
+    if (Tq == 0) return SIA_OK;
+    return scored_rows(q, k, v, sm_scale, sc, out, stream);
+  }
   if (q->dtype == SIA_F32) {
     if (rope != nullptr)
       return fail(SIA_ERR_UNSUPPORTED, "the rotary prologue runs on the float16/bfloat16 MFMA path only");
@@ -374,4 +405,16 @@ extern "C" int sia_attention_flash_fwd_rope(const sia_tensor* q, const sia_tenso
                                             size_t workspace_bytes, void* stream) {
   const RopeIn r{cos, sin, start_pos, start_pos_host, interleaved};
   return flash_fwd(q, k, v, causal, sm_scale, out, workspace, workspace_bytes, stream, &r);
+}
+
+extern "C" int sia_scored_attention_flash_fwd(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v,
+                                              int32_t causal, float sm_scale, const sia_score_options* score,
+                                              const sia_tensor* out, void* workspace, size_t workspace_bytes,
+                                              void* stream) {
+  const ScoreIn in{score};
+  return flash_fwd(q, k, v, causal, sm_scale, out, workspace, workspace_bytes, stream, nullptr, &in);
+}
+
+extern "C" int sia_scored_attention_flash_fwd_workspace_size(const sia_tensor* q, const sia_tensor* k, size_t* bytes) {
+  return sia_attention_flash_fwd_workspace_size(q, k, bytes);
 }

@@ -5,6 +5,7 @@
 
 #include "decode_kernel.hpp"
 #include "host_util.hpp"
+#include "score.hpp"
 
 namespace sia {
 
@@ -29,6 +30,7 @@ struct DecodeLaunch {
   size_t ws_bytes;
   int page_size;            // paged pools: tokens per page (0: contiguous cache)
   int lg_group;             // int4 only: log2 of the elements per parameter pair
+  const ScoreArgs* score;   // scored calls only
 };
 
 // wave_bytes: what a wave has of it by itself (its merge state; int4: its ring, which the merge reuses)

@@ -56,7 +56,7 @@ inline int elem_size(int dtype) {
     case SIA_F16: case SIA_BF16: return 2;
     case SIA_F32: case SIA_I32: return 4;
     case SIA_I8: case SIA_U8: return 1;
-    case SIA_I64: return 8;
+    case SIA_I64: case SIA_F64: return 8;
     default: return 0;
   }
 }
@@ -70,6 +70,7 @@ inline const char* dtype_name(int dtype) {
     case SIA_I32: return "int32";
     case SIA_I64: return "int64";
     case SIA_U8: return "uint8";
+    case SIA_F64: return "float64";
     default: return "unknown";
   }
 }

@@ -12,6 +12,13 @@ engine:
 * :class:`RopeFrequencies` -- ``ops/rope.py:72-185``: the cos/sin tables
   (Llama 3 frequency scaling) and their per-dtype cast cache.
 
+Without a counterpart in the reference:
+
+* :func:`rope_scaled` -- a part of each head rotated, at any positions, with
+  angles computed from frequencies in the kernel.
+* :class:`ScaledRope` -- the frequencies of scaled contexts (linear, NTK, YaRN,
+  Llama 3), applied by it or as tables for the functions that take tables.
+
 The rotation is ``out_a = x_a cos - x_b sin``, ``out_b = x_b cos + x_a sin``
 in fp32 with every product and sum rounded on its own (no fused
 multiply-add), stored in the input dtype with round-to-nearest-even.  Row
@@ -122,3 +129,93 @@ class RopeFrequencies:
                 self._cast_cache[dtype] = cached
             cos_tbl, sin_tbl = cached
         return cos_tbl[start_pos:start_pos + seq_len], sin_tbl[start_pos:start_pos + seq_len]
+
+
+def rope_scaled(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
+                rotary_dim: int | None = None, interleaved: bool = False, scale: float = 1.0):
+    """Rotate the first ``rotary_dim`` elements of every head of ``q (B, T, Hq, D)`` and ``k (B, T, Hkv, D)``.
+
+    ``positions``: int32 or int64 ``(T,)`` or ``(B, T)``; ``inv_freq``: float32
+    or float64 ``(rotary_dim / 2,)``, the angle per position of each pair, which
+    is ``(i, i + rotary_dim / 2)`` or, ``interleaved``, ``(2i, 2i + 1)``.  The
+    rotated part is multiplied by ``scale``, the rest copied.  Angles are exact
+    modulo a turn whatever the position (no table, no limit).  Strided views
+    are read in place; returns contiguous ``(q_rot, k_rot)``, ``k_rot`` None
+    where ``k`` is.
+    """
+    if rotary_dim is None:
+        rotary_dim = q.shape[-1]
+    return _lib.gpu_ops().rope_scaled(q, k, positions, inv_freq, rotary_dim, bool(interleaved), float(scale))
+
+
+class ScaledRope:
+    """Rotary frequencies of a context scaled beyond the one a model was trained on, and their application.
+
+    ``rotary_dim`` elements of each head of ``head_dim`` are rotated (default:
+    all).  ``rope_type``:
+
+    * ``"default"``: ``f_i = theta^(-2i/R)``;
+    * ``"linear"``: ``f_i / factor``;
+    * ``"ntk"``: ``theta`` times ``factor^(R / (R - 2))``;
+    * ``"yarn"``: ``f_i`` for pairs that turn more than ``beta_fast`` times in
+      ``original_max_seq_len`` positions, ``f_i / factor`` below ``beta_slow``
+      turns, a linear blend over the pairs between; rotated elements are
+      multiplied by ``attention_factor`` (default ``0.1 ln(factor) + 1``);
+    * ``"llama3"``: :class:`RopeFrequencies`' rule.
+
+    ``inv_freq`` is kept in float64 on ``device``.  Call the object with ``q``,
+    ``k`` and positions to rotate them (:func:`rope_scaled`), or take
+    :meth:`tables` for the fused calls that read tables of whole heads.
+    """
+
+    def __init__(self, head_dim: int, rotary_dim: int | None = None, rope_theta: float = 10_000.0,
+                 rope_type: str = "default", factor: float = 1.0, original_max_seq_len: int = 8192,
+                 beta_fast: float = 32.0, beta_slow: float = 1.0, low_freq_factor: float = 1.0,
+                 high_freq_factor: float = 4.0, attention_factor: float | None = None, interleaved: bool = False,
+                 device: torch.device | str | None = None):
+        R = head_dim if rotary_dim is None else rotary_dim
+        if R < 2 or R % 2 or R > head_dim:
+            raise ValueError(f"rotary_dim {R} must be even, at least 2 and at most head_dim {head_dim}")
+        if not factor > 0:
+            raise ValueError("factor must be positive")
+        self.head_dim, self.rotary_dim, self.interleaved = head_dim, R, interleaved
+        i = torch.arange(R // 2, dtype=torch.float64)
+        theta = float(rope_theta)
+        if rope_type == "ntk":
+            if R == 2:
+                raise ValueError('rope_type "ntk" needs a rotary_dim above 2')
+            theta *= factor ** (R / (R - 2))
+        freq = theta ** (-2.0 * i / R)
+        self.scale = 1.0
+        if rope_type == "linear":
+            freq = freq / factor
+        elif rope_type == "yarn":
+            low, high = (R * math.log(original_max_seq_len / (turns * 2 * math.pi)) / (2 * math.log(theta))
+                         for turns in (beta_fast, beta_slow))
+            low, high = max(math.floor(low), 0), min(math.ceil(high), R // 2 - 1)
+            ramp = ((i - low) / max(high - low, 0.001)).clamp(0, 1)
+            freq = freq / factor * ramp + freq * (1 - ramp)
+            self.scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+        elif rope_type == "llama3":
+            freq = RopeFrequencies._llama3_scaled(freq, factor, low_freq_factor, high_freq_factor, original_max_seq_len)
+        elif rope_type not in ("default", "ntk"):
+            raise ValueError(f"unknown rope_type {rope_type!r}")
+        if attention_factor is not None:
+            self.scale = float(attention_factor)
+        device = torch.device(device) if device is not None else torch.device("cuda" if torch.cuda.is_available() else "cpu")
+        self.inv_freq = freq.to(device)
+
+    def __call__(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor):
+        """``q (B, T, Hq, D)``, ``k (B, T, Hkv, D)`` rotated at ``positions (T,)`` or ``(B, T)``."""
+        return rope_scaled(q, k, positions, self.inv_freq, self.rotary_dim, self.interleaved, self.scale)
+
+    def tables(self, max_seq_len: int, dtype: torch.dtype = torch.float32):
+        """``(cos, sin)``, each ``(max_seq_len, head_dim)``, for the functions that rotate whole heads from tables.
+
+        Angles in float64, each entry rounded once; the factor of the rotated elements is in the entries.
+        """
+        if self.rotary_dim != self.head_dim:
+            raise ValueError("tables cover whole heads; a part of the head is rotated by calling the object")
+        angle = torch.arange(max_seq_len, dtype=torch.float64, device=self.inv_freq.device)[:, None] * self.inv_freq
+        angle = torch.cat([angle, angle], dim=-1)
+        return (self.scale * angle.cos()).to(dtype), (self.scale * angle.sin()).to(dtype)

@@ -14,6 +14,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <mutex>
 #include <tuple>
 #include <unordered_map>
@@ -52,6 +53,7 @@ int32_t dtype_code(at::ScalarType t) {
     case at::kInt: return SIA_I32;
     case at::kLong: return SIA_I64;
     case at::kByte: return SIA_U8;
+    case at::kDouble: return SIA_F64;
     default: throw py::value_error(std::string("dtype ") + c10::toString(t) + " is not supported by the attention kernels");
   }
 }
@@ -178,7 +180,26 @@ enum DecodeKind { kContig = 0, kContigInt8 = 1, kGqaInt8 = 2, kPaged = 3, kPaged
 Tensor decode_call(int64_t kind, const Tensor& q, const sia_tensor& dk, const sia_tensor& dv, const sia_tensor* dks,
                    const sia_tensor* dvs, const sia_tensor* dbt, const sia_tensor& dl, int64_t page_size,
                    double sm_scale, int64_t tiles_per_split, int64_t begin_event, int64_t end_event,
-                   const at::Device& dev);
+                   const at::Device& dev, const sia_score_options* score = nullptr);
+
+// Score options of a scored call (its tensors on `dev`).
+struct Score {
+  OptDesc slopes, start, len, prefix, cuts;
+  sia_score_options o;
+  Score(double softcap, int64_t window, const OptT& slopes_t, const OptT& start_t, const at::Device& dev,
+        const OptT& len_t = {}, const OptT& prefix_t = {}, const OptT& cuts_t = {})
+      : slopes(slopes_t, dev, "alibi_slopes"), start(start_t, dev, "kv_start"), len(len_t, dev, "kv_len"),
+        prefix(prefix_t, dev, "prefix_len"), cuts(cuts_t, dev, "cu_seqlens") {
+    memset(&o, 0, sizeof(o));
+    o.softcap = (float)softcap;
+    o.window = (int32_t)std::min<int64_t>(window, 0x7fffffff);
+    o.alibi_slopes = slopes.ptr();
+    o.kv_start = start.ptr();
+    o.kv_len = len.ptr();
+    o.prefix_len = prefix.ptr();
+    o.cu_seqlens = cuts.ptr();
+  }
+};
 
 // One decode call (q (B, Hq, 1, D)) -> out (B, 1, Hq, D) in q's dtype.
 Tensor decode(int64_t kind, const Tensor& q, const Tensor& k, const Tensor& v, const OptT& k_scale,
@@ -221,7 +242,7 @@ Tensor decode_layer(int64_t kind, const Tensor& q, const Tensor& k_pool, const T
 Tensor decode_call(int64_t kind, const Tensor& q, const sia_tensor& dk, const sia_tensor& dv, const sia_tensor* dks,
                    const sia_tensor* dvs, const sia_tensor* dbt, const sia_tensor& dl, int64_t page_size,
                    double sm_scale, int64_t tiles_per_split, int64_t begin_event, int64_t end_event,
-                   const at::Device& dev) {
+                   const at::Device& dev, const sia_score_options* score) {
   const int64_t B = q.size(0), Hq = q.size(1), D = q.size(3), Hkv = dk.shape[1];
   const sia_tensor dq = desc(q, dev, "q");
   Tensor out = at::empty({B, 1, Hq, D}, q.options());
@@ -237,6 +258,11 @@ Tensor decode_call(int64_t kind, const Tensor& q, const sia_tensor& dk, const si
   void* s = stream_of(dev);
   const float sc = (float)sm_scale;
   int rc;
+  if (score != nullptr) {
+    check(sia_scored_attention_flash_decode(&dq, &dk, &dv, dks, dvs, dbt, &dl, (int32_t)page_size, sc, score, &dout,
+                                            ws.data_ptr(), ws_bytes, po, s));
+    return out;
+  }
   switch (kind) {
     case kContig:
       rc = sia_attention_flash_decode(&dq, &dk, &dv, &dl, sc, &dout, ws.data_ptr(), ws_bytes, po, s);
@@ -267,6 +293,42 @@ Tensor decode_call(int64_t kind, const Tensor& q, const sia_tensor& dk, const si
   }
   check(rc);
   return out;
+}
+
+// A decode call with a score function, whatever the cache: k_scale, v_scale for int8 and int4, block_table for pools.
+Tensor decode_scored(const Tensor& q, const Tensor& k, const Tensor& v, const OptT& k_scale, const OptT& v_scale,
+                     const OptT& block_table, const Tensor& kv_len, int64_t page_size, double sm_scale, double softcap,
+                     const OptT& slopes, int64_t window, const OptT& kv_start, int64_t tiles_per_split,
+                     int64_t begin_event, int64_t end_event) {
+  const at::Device dev = gpu_of(q, "q");
+  const c10::DeviceGuard guard(dev);
+  if (q.dim() != 4) throw py::value_error("q must be (B, Hq, 1, D)");
+  if (k.dim() != 4) throw py::value_error("k must have 4 dims");
+  if (q.size(0) == 0) return at::empty({0, 1, q.size(1), q.size(3)}, q.options());
+  const sia_tensor dk = desc(k, dev, "k"), dv = desc(v, dev, "v"), dl = desc(kv_len, dev, "kv_len");
+  const OptDesc dks(k_scale, dev, "k_scale"), dvs(v_scale, dev, "v_scale"), dbt(block_table, dev, "block_table");
+  const Score sc(softcap, window, slopes, kv_start, dev);
+  return decode_call(0, q, dk, dv, dks.ptr(), dvs.ptr(), dbt.ptr(), dl, page_size, sm_scale, tiles_per_split,
+                     begin_event, end_event, dev, &sc.o);
+}
+
+// The same over layer `layer` of a cache's whole pools (as decode_layer).
+Tensor decode_layer_scored(const Tensor& q, const Tensor& k_pool, const Tensor& v_pool, const OptT& k_scales,
+                           const OptT& v_scales, int64_t layer, const OptT& block_table, const Tensor& kv_len,
+                           int64_t page_size, double sm_scale, double softcap, const OptT& slopes, int64_t window,
+                           const OptT& kv_start, int64_t tiles_per_split, int64_t begin_event, int64_t end_event) {
+  const at::Device dev = gpu_of(q, "q");
+  const c10::DeviceGuard guard(dev);
+  if (q.dim() != 4) throw py::value_error("q must be (B, Hq, 1, D)");
+  if (k_pool.dim() != 5) throw py::value_error("the cache's k must have 5 dims");
+  const int64_t B = q.size(0);
+  if (B == 0) return at::empty({0, 1, q.size(1), q.size(3)}, q.options());
+  const LayerDescs c(k_pool, v_pool, k_scales, v_scales, block_table, layer, B, dev);
+  sia_tensor dl = desc(kv_len, dev, "kv_len");
+  if (c.has_bt) dl = first_rows(dl, B);
+  const Score sc(softcap, window, slopes, kv_start, dev);
+  return decode_call(0, q, c.k, c.v, c.ksp(), c.vsp(), c.btp(), dl, page_size, sm_scale, tiles_per_split, begin_event,
+                     end_event, dev, &sc.o);
 }
 
 // A prefill operand as the kernels read it: in place when head_dim is
@@ -302,6 +364,29 @@ Tensor prefill(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, bool 
   Tensor ws = ws_bytes > 0 ? at::empty({(int64_t)ws_bytes}, q.options().dtype(at::kByte)) : Tensor();
   check(sia_attention_flash_fwd(&dq, &dk, &dv, causal ? 1 : 0, (float)sm_scale, &dout,
                                 ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, stream_of(dev)));
+  return out;
+}
+
+// prefill with a score function (scored attention).
+Tensor prefill_scored(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, bool causal, double sm_scale,
+                      double softcap, const OptT& slopes, int64_t window, const OptT& cu_seqlens, const OptT& prefix_len,
+                      const OptT& kv_start, const OptT& kv_len, bool out_token_major) {
+  const at::Device dev = gpu_of(q_in, "q");
+  const c10::DeviceGuard guard(dev);
+  if (q_in.dim() != 4 || k_in.dim() != 4 || v_in.dim() != 4) throw py::value_error("q, k and v must have 4 dims");
+  const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in);
+  const int64_t B = q.size(0), Hq = q.size(1), Tq = q.size(2), D = q.size(3);
+  const sia_tensor dq = desc(q, dev, "q"), dk = desc(k, dev, "k"), dv = desc(v, dev, "v");
+  Tensor out = out_token_major ? at::empty({B, Tq, Hq, D}, q.options()) : at::empty({B, Hq, Tq, D}, q.options());
+  if (B == 0) return out;
+  const Tensor view = out_token_major ? out.transpose(1, 2) : out;
+  const sia_tensor dout = desc(view, dev, "out");
+  const Score sc(softcap, window, slopes, kv_start, dev, kv_len, prefix_len, cu_seqlens);
+  size_t ws_bytes = 0;
+  check(sia_scored_attention_flash_fwd_workspace_size(&dq, &dk, &ws_bytes));
+  Tensor ws = ws_bytes > 0 ? at::empty({(int64_t)ws_bytes}, q.options().dtype(at::kByte)) : Tensor();
+  check(sia_scored_attention_flash_fwd(&dq, &dk, &dv, causal ? 1 : 0, (float)sm_scale, &sc.o, &dout,
+                                       ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, stream_of(dev)));
   return out;
 }
 
@@ -499,6 +584,28 @@ std::tuple<Tensor, Tensor> rope_qk(const Tensor& q_in, const Tensor& k_in, const
   return {qo, ko};
 }
 
+// Rotary positions from frequencies -> contiguous outputs.
+std::tuple<Tensor, OptT> rope_scaled(const Tensor& q_in, const OptT& k_in, const Tensor& positions, const Tensor& inv_freq,
+                                     int64_t rotary_dim, bool interleaved, double scale) {
+  const at::Device dev = gpu_of(q_in, "q");
+  const c10::DeviceGuard guard(dev);
+  if (q_in.dim() != 4 || (k_in.has_value() && k_in->dim() != 4)) throw py::value_error("q and k must be (B, T, H, D)");
+  if (rotary_dim != (int32_t)rotary_dim) throw py::value_error("rotary_dim must fit 32 bits");
+  const Tensor q = q_in.stride(3) == 1 ? q_in : q_in.contiguous();
+  OptT k = k_in;
+  if (k.has_value() && k->stride(3) != 1) k = k->contiguous();
+  const sia_tensor dq = desc(q, dev, "q"), dp = desc(positions, dev, "positions"), df = desc(inv_freq, dev, "inv_freq");
+  const OptDesc dk(k, dev, "k");
+  Tensor qo = at::empty(q.sizes(), q.options());
+  OptT ko;
+  if (k.has_value()) ko = at::empty(k->sizes(), k->options());
+  const sia_tensor dqo = desc(qo, dev, "q_out");
+  const OptDesc dko(ko, dev, "k_out");
+  check(sia_rope_scaled(&dq, dk.ptr(), &dp, &df, (int32_t)rotary_dim, interleaved ? 1 : 0, (float)scale, &dqo, dko.ptr(),
+                        stream_of(dev)));
+  return {qo, ko};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_sia_ops, m) {
@@ -531,4 +638,8 @@ PYBIND11_MODULE(_sia_ops, m) {
   m.def("rope_kv_write", &rope_kv_write);
   m.def("rope_kv_write_layer", &rope_kv_write_layer);
   m.def("rope_qk", &rope_qk);
+  m.def("prefill_scored", &prefill_scored);
+  m.def("decode_scored", &decode_scored);
+  m.def("decode_layer_scored", &decode_layer_scored);
+  m.def("rope_scaled", &rope_scaled);
 }

@@ -252,7 +252,7 @@ int flash_fwd(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, int
     if ((rc = fill_score(score->options, true, B, Hq, sm_scale, causal, sc))) return rc;
     if ((rc = device_ok())) return rc;
     if (Tq == 0) return SIA_OK;
-    return scored_rows(q, k, v, sm_scale, sc, out, stream);
+    if (q->dtype == SIA_F32 || sc.cap_out > kMaxFastCap * kLog2e) return scored_rows(q, k, v, sm_scale, sc, out, stream);
   }
   if (q->dtype == SIA_F32) {
     if (rope != nullptr)
@@ -269,6 +269,10 @@ int flash_fwd(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, int
 
   PrefillLaunch L;
   memset(&L, 0, sizeof(L));
+  if (score != nullptr) {
+    L.mod = score_mod(sc);
+    L.s = sc;
+  }
   PrefillArgs& a = L.a;
   a.q = (const char*)q->data; a.q_sb = bstride(q, 0); a.q_sh = bstride(q, 1); a.q_sm = bstride(q, 2);
   a.k = (const char*)k->data; a.k_sb = bstride(k, 0); a.k_sh = bstride(k, 1); a.k_sn = k_sn;
@@ -284,7 +288,7 @@ int flash_fwd(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, int
   L.var = D == 128 && groups(B, Hkv, a.G, Tq, (int)D, 0) <= dev.cus ? 1 : 0;
   // Few query rows over many keys: variant 3 or 4, when the caller's workspace
   // also holds the partials (the size of sia_attention_flash_fwd_workspace_size)
-  const KeySplit ks = v_rows_ok ? key_splits(B, Hq, Hkv, Tq, Tk, D, q->dtype == SIA_BF16, dev.cus) : KeySplit();
+  const KeySplit ks = v_rows_ok && score == nullptr ? key_splits(B, Hq, Hkv, Tq, Tk, D, q->dtype == SIA_BF16, dev.cus) : KeySplit();
   const int64_t images = ks.var == 4 ? need : 0;         // (variant 3 needs none)
   if (ks.ns > 1 && workspace != nullptr && (uintptr_t)workspace % 256 == 0 &&
       workspace_bytes >= (size_t)(images + ks.bytes))
@@ -324,6 +328,9 @@ int flash_fwd(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, int
   const int64_t nall = (int64_t)a.nqblk * nunit;
   a.fold = L.var == 1 && dev.cus % 8 == 0 && nall > dev.cus && nall <= 2 * (int64_t)dev.cus ? dev.cus : 0;
 
+  if (score != nullptr) {   // (for the rows that are computed again)
+    a.v = (const char*)v->data; a.v_sb = bstride(v, 0); a.v_sh = bstride(v, 1); a.v_sn = v_sn;
+  }
   PackArgs& p = L.pack;
   p.v = (const char*)v->data; p.v_sb = bstride(v, 0); p.v_sh = bstride(v, 1); p.v_sn = bstride(v, 2);
   p.vimg = (char*)workspace;

@@ -45,6 +45,7 @@ static int launch_fwd(PrefillLaunch& L, int rope) {
 }
 
 int launch_prefill(PrefillLaunch& L) {
+  if (L.mod != kModNone) return launch_prefill_scored(L);
   const bool bf = L.dtype == SIA_BF16;
   switch (L.D) {
     case 16: return bf ? launch_prefill_typed<16, BF16>(L) : launch_prefill_typed<16, F16>(L);

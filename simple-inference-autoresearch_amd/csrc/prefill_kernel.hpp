@@ -41,6 +41,7 @@
 //    on the same XCD so their K/V tiles are served by one L2.
 #pragma once
 
+#include "score.hpp"
 #include "sia_common.hpp"
 
 namespace sia {
@@ -86,6 +87,15 @@ struct PrefillArgs {
   int64_t nrows;                                // B * Hq * Tq
   FastDiv dS, dTq, dHq;                         // divisions by nsplit (kernel), Tq and Hq (merge)
 };
+
+// scored attention (MOD): the score function and the masks on top
+struct ScoredPrefillArgs : PrefillArgs {
+  ScoreArgs s;
+};
+// (compared with a plain 0: a kernel's name holds this expression, and one with an enumeration that has no name differs
+// between host and device, so that the launch finds no kernel)
+template <int MOD>
+using PfArgs = std::conditional_t<MOD != 0, ScoredPrefillArgs, PrefillArgs>;
 
 struct PackArgs {
   const char* v; int64_t v_sb, v_sh, v_sn;      // byte strides; head_dim contiguous
@@ -162,8 +172,13 @@ __device__ __forceinline__ int image_key(int c, int i) { return 16 * (c >> 1) + 
 // One 16-bit V element (raw bits) as f16 bits: bf16 is widened to f32,
 // clamped to the f16 range and rounded (the PV product runs in f16 so that P
 // keeps 11 significant bits).
+// (WIDE, scored attention: not clamped; a value past the range becomes an Inf,
+// and the rows that it leaves not finite are computed again, see prefill_fwd)
+template <bool WIDE>
 __device__ __forceinline__ uint32_t elem_f16(F16, uint32_t bits) { return bits; }
+template <bool WIDE>
 __device__ __forceinline__ uint32_t elem_f16(BF16, uint32_t bits) {
+  if constexpr (WIDE) return __builtin_bit_cast(uint16_t, (_Float16)__builtin_bit_cast(float, bits << 16));
   const float f = __builtin_amdgcn_fmed3f(__builtin_bit_cast(float, bits << 16), -65504.0f, 65504.0f);
   return __builtin_bit_cast(uint16_t, (_Float16)f);
 }
@@ -175,7 +190,7 @@ __device__ __forceinline__ uint32_t elem_f16(BF16, uint32_t bits) {
 // by 8 bytes so the 8 rows one output chunk gathers sit in different banks),
 // then every thread assembles whole output chunks, so each store instruction
 // of a wave writes one contiguous 1 KB run.
-template <int D, class T>
+template <int D, class T, bool WIDE = false>
 __global__ __launch_bounds__(256) void prefill_pack_v(const PackArgs a) {
   constexpr int DV = PfCfg<D>::DV;
   constexpr int RS = D + 4;                       // LDS row stride in 16-bit elements
@@ -210,8 +225,8 @@ __global__ __launch_bounds__(256) void prefill_pack_v(const PackArgs a) {
     if (d < D) {
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
-        const uint32_t lo = elem_f16(T{}, tile[image_key(c, 2 * m) * RS + d]);
-        const uint32_t hi = elem_f16(T{}, tile[image_key(c, 2 * m + 1) * RS + d]);
+        const uint32_t lo = elem_f16<WIDE>(T{}, tile[image_key(c, 2 * m) * RS + d]);
+        const uint32_t hi = elem_f16<WIDE>(T{}, tile[image_key(c, 2 * m + 1) * RS + d]);
         w[m] = lo | (hi << 16);
       }
     }
@@ -398,9 +413,18 @@ __device__ __forceinline__ void wait_vmcnt() {
 template <int C> constexpr int kPfThreads = PfCfg<C / 8, C % 8>::waves * 64;
 template <int C> constexpr int kPfWpe = PfCfg<C / 8, C % 8>::wpe;
 
-template <int D, class T, int ROPE, int VAR>
+// MOD (scored attention, score.hpp): kModNone, or which score function.  Every
+// query row then has a run of keys of its own, [mlo, mhi); the work-group walks
+// the union of its rows' runs, and only the blocks that do not lie whole in all
+// of a wave's runs are masked there.  Masks alone cost nothing inside the block
+// loop; a cap or a bias reshapes each score between the QK product and the row
+// max (see `shape`), and the weights are then taken from the shaped scores.
+// A row whose result is not finite is computed again on the vector ALUs
+// (scored_row): a hidden key's NaN or Inf in V turns up in it as weight 0 times
+// that, and so does a bfloat16 V past float16's range.
+template <int D, class T, int ROPE, int VAR, int MOD = kModNone>
 __global__ __launch_bounds__(kPfThreads<8 * D + VAR>) __attribute__((amdgpu_waves_per_eu(kPfWpe<8 * D + VAR>)))
-void prefill_fwd(const PrefillArgs a) {
+void prefill_fwd(const PfArgs<MOD> a) {
   using C = PfCfg<D, VAR>;
   constexpr int NW = C::waves, S = C::stages, DV = C::DV;
   constexpr int KST = D / 16;                   // QK k-steps
@@ -468,8 +492,8 @@ void prefill_fwd(const PrefillArgs a) {
   }
   // variants 3 and 4 work on their run of key blocks as on a call of those keys alone
   // (key 0 and the causal offset moved to the run's first key)
-  const int key_lo = C::split ? split * a.bps * kPfBN : 0;
-  const int Tk = C::split ? max(0, min(a.Tk - key_lo, a.bps * kPfBN)) : a.Tk;
+  int key_lo = C::split ? split * a.bps * kPfBN : 0;
+  int Tk = C::split ? max(0, min(a.Tk - key_lo, a.bps * kPfBN)) : a.Tk;
   const int bhn = a.B * a.Hkv;
   const int hgrp = fdiv(u, a.dBH);
   const int bh = u - hgrp * bhn;
@@ -479,6 +503,7 @@ void prefill_fwd(const PrefillArgs a) {
   const int lane = threadIdx.x & 63;
   const int wave = uniform(threadIdx.x >> 6);
   const int l32 = lane & 31, h = lane >> 5;
+  constexpr bool kMod = MOD != kModNone, kShape = mod_cap(MOD) || mod_bias(MOD);
   const int off = a.Tk - a.Tq - key_lo;                  // bottom-right causal offset
   // This wave's head (wave % hpw) and 32-row group (wave / hpw) of the
   // work-group's rpg = NW / hpw row groups per head.  With 8 waves, waves w
@@ -492,6 +517,27 @@ void prefill_fwd(const PrefillArgs a) {
   const int hq = hkv * a.G + (hgrp << a.hpw_lg) + hw;
   const int q0 = qblk * 32 * rpg;                        // the work-group's first row (every head)
   const int qi = q0 + rg * 32 + l32;                     // this lane's query row
+
+  // MOD: this lane's keys [mlo, mhi), the wave's first blocks that some row sees
+  // not whole at the front, [0, mfront), and the keys of its first and last rows
+  // (all from key_lo on, the work-group's first block)
+  int mlo = 0, mhi = 0, mfront = 0, mhi0 = 0, mhi1 = 0;
+  if constexpr (kMod) {
+    const int p0 = a.Tk - a.Tq;                          // position of row 0
+    const int w0 = min(q0 + rg * 32, a.Tq - 1), nw = min(32, a.Tq - w0);   // the wave's first row, its rows
+    const int g1 = min(q0 + 32 * rpg, a.Tq) - 1;
+    const SeqBounds sb = seq_bounds(a.s, b, a.Tk);
+    const Documents dc = documents(a.s, b, p0 + w0, p0 + q0, p0 + g1, lane);
+    key_lo = min(row_lo(a.s, sb, p0 + q0, dc.g_below), a.Tk) & ~(kPfBN - 1);
+    key_lo = max(key_lo, 0);
+    Tk = max(0, row_hi(a.s, sb, p0 + g1, dc.g_above) - key_lo);
+    const int i = min(l32, nw - 1);                      // (a row past Tq is masked as the last one)
+    mlo = row_lo(a.s, sb, p0 + w0 + i, dc.lo(p0 + w0, i)) - key_lo;
+    mhi = row_hi(a.s, sb, p0 + w0 + i, dc.hi(p0 + w0, i)) - key_lo;
+    mfront = (row_lo(a.s, sb, p0 + w0 + nw - 1, dc.lo(p0 + w0, nw - 1)) - key_lo + kPfBN - 1) / kPfBN;
+    mhi0 = max(0, row_hi(a.s, sb, p0 + w0, dc.hi(p0 + w0, 0)) - key_lo);
+    mhi1 = q0 + rg * 32 < a.Tq ? min(Tk, row_hi(a.s, sb, p0 + w0 + nw - 1, dc.hi(p0 + w0, nw - 1)) - key_lo) : 0;
+  }
 
   // ---- Q^T operand (B of S^T = K Q^T): query qi, d = 16 j + 8 h + [0, 8)
   // (through LDS, see dma_q, or straight into registers)
@@ -510,18 +556,18 @@ void prefill_fwd(const PrefillArgs a) {
     }
   };
 
-  const int kend = a.causal ? min(Tk, off + q0 + 32 * rpg) : Tk;
+  const int kend = a.causal && !kMod ? min(Tk, off + q0 + 32 * rpg) : Tk;
   const int nblk = kend > 0 ? (kend + kPfBN - 1) / kPfBN : 0;   // key blocks of the work-group
   const int wrow0 = q0 + rg * 32;                        // this wave's first row
-  const int wend = a.causal ? min(Tk, off + wrow0 + 32) : Tk;   // keys this wave can see
+  const int wend = kMod ? mhi1 : a.causal ? min(Tk, off + wrow0 + 32) : Tk;   // keys this wave can see
   const int wblk = wend > 0 ? min(nblk, (wend + kPfBN - 1) / kPfBN) : 0;   // blocks this wave computes
   // blocks [0, wfull) are visible to every row of the wave: no mask
   const int lim_all = a.causal ? min(Tk - 1, off + wrow0) : Tk - 1;
-  const int wfull = lim_all >= 0 ? (lim_all + 1) / kPfBN : 0;
+  const int wfull = kMod ? mhi0 / kPfBN : lim_all >= 0 ? (lim_all + 1) / kPfBN : 0;
   const int lim = a.causal ? min(Tk - 1, off + qi) : Tk - 1;   // this lane's last visible key
 
   const char* kb = a.k + b * a.k_sb + (int64_t)hkv * a.k_sh + (int64_t)key_lo * a.k_sn;
-  const char* vimg = a.vimg + (((int64_t)b * a.Hkv + hkv) * a.nkb + (C::split ? split * a.bps : 0)) * VB;
+  const char* vimg = a.vimg + (((int64_t)b * a.Hkv + hkv) * a.nkb + (kMod ? key_lo / kPfBN : C::split ? split * a.bps : 0)) * VB;
   // K stages are row-major with an XOR swizzle: 16-byte chunk c of key row r
   // sits in slot c ^ (r % NC) of the row's RB bytes.  A DMA instruction then
   // reads whole rows (16 lanes per 256-byte row at D = 128: coalesced), and
@@ -705,8 +751,9 @@ void prefill_fwd(const PrefillArgs a) {
         for (int m = 0; m < 4; ++m) {
           const uint32_t x = w[i][m];
           const float f0 = __builtin_bit_cast(float, x << 16), f1 = __builtin_bit_cast(float, x & 0xffff0000u);
-          w[i][m] = pack2(F16{}, __builtin_amdgcn_fmed3f(f0, -65504.0f, 65504.0f),
-                          __builtin_amdgcn_fmed3f(f1, -65504.0f, 65504.0f));
+          w[i][m] = kMod ? pack2(F16{}, f0, f1)
+                         : pack2(F16{}, __builtin_amdgcn_fmed3f(f0, -65504.0f, 65504.0f),
+                                 __builtin_amdgcn_fmed3f(f1, -65504.0f, 65504.0f));
         }
 #pragma unroll
       for (int i = 0; i < CH; ++i) *(u32x4*)(LV + (t + i * NW * 64) * 16) = w[i];
@@ -755,7 +802,19 @@ void prefill_fwd(const PrefillArgs a) {
   // keys past this lane's last visible key -> -inf (diagonal / ragged blocks)
   // (each compare feeds its select at once: compares hoisted ahead of the
   // selects would hold 32 lane masks in scalar registers)
+  // (MOD: outside [mlo, mhi), one unsigned compare)
+  const uint32_t mlen = (uint32_t)max(0, mhi - mlo);
   auto mask = [&](f32x16& s0, f32x16& s1, int key0) {
+    if constexpr (kMod) {
+      const int from = key0 + 4 * h - mlo;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int c = (j >> 2) * 8 + (j & 3);
+        if ((uint32_t)(from + c) >= mlen) s0[j] = -INFINITY;
+        if ((uint32_t)(from + c + 32) >= mlen) s1[j] = -INFINITY;
+      }
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       const int key = key0 + ((j & 15) >> 2) * 8 + 4 * h + (j & 3);
@@ -763,6 +822,32 @@ void prefill_fwd(const PrefillArgs a) {
       if (key + 32 > lim) s1[j] = -INFINITY;
     }
   };
+  auto masked = [&](int j) { return j >= wfull || (kMod && j < mfront); };   // some row of the wave sees block j not whole
+  // MOD with a cap or a bias: the scores of one block in log2 units
+  float slope2 = 0.f;
+  int kp = 0;                                              // position of key 4 h of block 0 less this lane's query's
+  if constexpr (mod_bias(MOD)) {
+    slope2 = a.s.slopes[hq] * kLog2e;
+    kp = key_lo + 4 * h - (a.Tk - a.Tq + qi);
+  }
+  auto shape = [&](f32x16& s0, f32x16& s1, int key0) {
+    if constexpr (kShape) {
+      const float d = (float)(kp + key0);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          float x = t ? s1[j] : s0[j];
+          if constexpr (mod_cap(MOD)) x = capped(a.s, x);
+          else x *= a.qk_scale;
+          if constexpr (mod_bias(MOD)) x = __builtin_fmaf(-slope2, fabsf(d + (float)(32 * t + (j >> 2) * 8 + (j & 3))), x);
+          if (t) s1[j] = x;
+          else s0[j] = x;
+        }
+    }
+  };
+  // the weight's exponent from a score as the block loop holds it
+  auto above = [&](float x, float mu) { return kShape ? x - mu : __builtin_fmaf(x, a.qk_scale, -mu); };
   // row max over the 64 keys: a lane-local tree plus the partner half of the wave
   // (a three-input tree, 32 values in 16 v_maximum3; pairs of two-input
   // maxima had compiled to 21, several of them with a repeated operand)
@@ -789,7 +874,7 @@ void prefill_fwd(const PrefillArgs a) {
   // lazy running max: (l, o) are rescaled only when the block max exceeds m by
   // 2^8 (p <= 2^8 otherwise, well inside f16)
   auto raise_max = [&](float rmax) {
-    const float smax = rmax * a.qk_scale;
+    const float smax = kShape ? rmax : rmax * a.qk_scale;
     if (__any(smax > m + 8.0f)) {
       const float m_new = __builtin_elementwise_maximum(m, smax);
       const float alpha = m_new == -INFINITY ? 1.0f : fast_exp2(m - m_new);   // row still sees nothing
@@ -844,8 +929,8 @@ void prefill_fwd(const PrefillArgs a) {
           const int j0 = (ks & 1) * 8 + 2 * i;
           const float x0 = ks < 2 ? sa0[j0] : sa1[j0];
           const float x1 = ks < 2 ? sa0[j0 + 1] : sa1[j0 + 1];
-          const float p0 = fast_exp2(__builtin_fmaf(x0, a.qk_scale, -mu));
-          const float p1 = fast_exp2(__builtin_fmaf(x1, a.qk_scale, -mu));
+          const float p0 = fast_exp2(above(x0, mu));
+          const float p1 = fast_exp2(above(x1, mu));
           const uint32_t w = pack2(F16{}, p0, p1);
           lb[ks] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), ones, lb[ks], false);
           pop[ks][i] = w;
@@ -878,6 +963,7 @@ void prefill_fwd(const PrefillArgs a) {
         if (i == NQK - 1) ex(3);
       }
       l += (lb[0] + lb[1]) + (lb[2] + lb[3]);
+      shape(sb0, sb1, (j + 1) * kPfBN);
       // the next block's row max (unmasked; redone below on masked blocks)
       rmax = rowmax(sb0, sb1);
       // slot pattern: two reads ahead, then per slot one MFMA, the read two
@@ -917,7 +1003,7 @@ void prefill_fwd(const PrefillArgs a) {
       // below the branch that follows, where nothing overlaps it)
       asm volatile("" : "+v"(l));
       // (the scores of block wblk are discarded: no mask for them)
-      if (j + 1 >= wfull && j + 1 < wblk) {
+      if (masked(j + 1) && j + 1 < wblk) {
         mask(sb0, sb1, (j + 1) * kPfBN);
         rmax = rowmax(sb0, sb1);
       }
@@ -929,7 +1015,8 @@ void prefill_fwd(const PrefillArgs a) {
   auto first_scores = [&]() {
     if (wblk > 0) {
       qk(lk0, s0, s1, no_piece);
-      if (wfull == 0) mask(s0, s1, 0);
+      shape(s0, s1, 0);
+      if (masked(0)) mask(s0, s1, 0);
       rmax = rowmax(s0, s1);
     }
   };
@@ -939,7 +1026,7 @@ void prefill_fwd(const PrefillArgs a) {
   // whose second half lies past the wave's rows, or a ragged last block), the
   // second key tile's weights are all zero and its exponentials and PV MFMAs
   // are skipped.  Its V stage is picked at run time (one block per group).
-  const int wlim = a.causal ? min(Tk - 1, off + wrow0 + 31) : Tk - 1;   // the wave's last visible key
+  const int wlim = kMod ? mhi1 - 1 : a.causal ? min(Tk - 1, off + wrow0 + 31) : Tk - 1;   // the wave's last visible key
   auto work_last = [&](const char* Vstage, int j, const f32x16& sa0, const f32x16& sa1) {
     if (j >= wblk) return;
     raise_max(rmax);
@@ -954,8 +1041,8 @@ void prefill_fwd(const PrefillArgs a) {
         const int j0 = (ks & 1) * 8 + 2 * i;
         const float x0 = ks < 2 ? sa0[j0] : sa1[j0];
         const float x1 = ks < 2 ? sa0[j0 + 1] : sa1[j0 + 1];
-        const float p0 = fast_exp2(__builtin_fmaf(x0, a.qk_scale, -mu));
-        const float p1 = fast_exp2(__builtin_fmaf(x1, a.qk_scale, -mu));
+        const float p0 = fast_exp2(above(x0, mu));
+        const float p1 = fast_exp2(above(x1, mu));
         const uint32_t w = pack2(F16{}, p0, p1);
         lb[ks] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), ones, lb[ks], false);
         pop[ks][i] = w;
@@ -1154,6 +1241,27 @@ void prefill_fwd(const PrefillArgs a) {
     tile += (wave & 1) * 32 * RB;
     const float lt = half_swap_sum(l);
     const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+    if constexpr (kMod) {
+      // not finite: from what the row sees, or from a hidden key's value times 0
+      float t = 0.f;
+#pragma unroll
+      for (int e = 0; e < ET; ++e)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) t = __builtin_fmaf(o[e][j], 0.f, t);
+      if (__any(t != t && qi < a.Tq)) {
+        const char* kr = a.k + b * a.k_sb + (int64_t)hkv * a.k_sh;
+        const char* vr = a.v + b * a.v_sb + (int64_t)hkv * a.v_sh;
+        const float sl = a.s.slopes != nullptr ? a.s.slopes[hq] * kLog2e : 0.f;
+#pragma unroll 1
+        for (int r = 0; r < min(32, a.Tq - wrow0); ++r) {
+          const int lo = __builtin_amdgcn_readlane(mlo, r) + key_lo, hi = __builtin_amdgcn_readlane(mhi, r) + key_lo;
+          scored_row<D, T>(a.s, a.qk_scale, sl, a.q + b * a.q_sb + (int64_t)hq * a.q_sh + (int64_t)(wrow0 + r) * a.q_sm,
+                           kr, a.k_sn, vr, a.v_sn, a.Tk - a.Tq + wrow0 + r, lo, hi,
+                           a.out + b * a.o_sb + (int64_t)hq * a.o_sh + (int64_t)(wrow0 + r) * a.o_sm, lane);
+        }
+        return;
+      }
+    }
 #pragma unroll
     for (int e = 0; e < ET; ++e)
 #pragma unroll

@@ -14,6 +14,8 @@ struct PrefillLaunch {
                    // 2 = variant 1 with the V^T images built in LDS (short key ranges; no prefill_pack_v),
                    // 3 and 4 = key blocks split over work-groups (head_dim 64, 128 and 256; prefill_split.hip)
   hipStream_t stream;
+  int mod;         // kModNone, or the score function of a scored call (kModMask ...) and its arguments
+  ScoreArgs s;
 };
 
 // Longest key range that runs variant 2 (bfloat16: float16 at D = 128 reads
@@ -33,6 +35,11 @@ constexpr int kPackvMaxKeysD64 = 768;
 int launch_prefill(PrefillLaunch& L);
 // Variants 3 and 4: prefill_fwd over runs of key blocks, then prefill_merge (called by launch_prefill).
 int launch_prefill_split(PrefillLaunch& L);
+
+// Scored calls (variants 0-2; called by launch_prefill), compiled by head_dim: prefill_scored.hip and its _d128 and _d256.
+int launch_prefill_scored(PrefillLaunch& L);
+int launch_prefill_scored_128(PrefillLaunch& L);
+int launch_prefill_scored_256(PrefillLaunch& L);
 
 // Rotary variant: none, or split-half / interleaved pairs from 16-bit / fp32 tables.
 inline int rope_variant(const PrefillArgs& a) {

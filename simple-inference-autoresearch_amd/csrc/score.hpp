@@ -33,12 +33,16 @@ struct ScoreArgs {
 };
 
 // Score kernels are compiled for: masks alone, capped scores, a bias by distance, or both (kModNone: none of this).
-enum : int { kModNone = 0, kModMask = 4, kModCap = 5, kModBias = 6, kModCapBias = 7 };
+constexpr int kModNone = 0, kModMask = 4, kModCap = 5, kModBias = 6, kModCapBias = 7;
 constexpr bool mod_cap(int m) { return (m & 1) != 0; }
 constexpr bool mod_bias(int m) { return (m & 2) != 0; }
 inline int score_mod(const ScoreArgs& s) { return kModMask | (s.cap_out > 0.f ? 1 : 0) | (s.slopes != nullptr ? 2 : 0); }
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+// The largest cap of the matrix kernels: their `capped` is off by 2^-22 of it, at 512 as much as the weights' rounding to
+// fp16 (2^-11 half a step; 512 2^-22 log2(e) = 2^-12.5).  Larger ones go to the vector kernels.
+constexpr float kMaxFastCap = 512.0f;
 
 // c tanh(x / c) in log2 units from the raw product, as c (1 - 2 / (1 + e^(2 x / c))): two transcendentals and three
 // instructions.  Off by at most about 3 ulp of c, 2^-22 c: below every rounding of 16-bit inputs and weights (c = 50: 2e-5

@@ -94,6 +94,9 @@ EXTRA_FLAGS = {
     "decode_i4_d128.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "decode_i4_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "decode_i4_pages.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "decode_scored_f16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "decode_scored_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "decode_scored_i8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attn_f32_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

@@ -429,6 +429,16 @@ int dispatch(DecodeLaunch& L, int kv_dtype) {
   }
 }
 
+int dispatch_scored(DecodeLaunch& L, int kv_dtype) {
+  if (L.D == 256) return launch_decode_scored_256(L, kv_dtype);
+  switch (kv_dtype) {
+    case SIA_F16: return launch_decode_scored_f16(L);
+    case SIA_BF16: return launch_decode_scored_bf16(L);
+    case SIA_I8: return launch_decode_scored_i8(L);
+    default: return fail(SIA_ERR_UNSUPPORTED, "k/v dtype %s not supported", dtype_name(kv_dtype));
+  }
+}
+
 int decode_any(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, const sia_tensor* ks,
                const sia_tensor* vs, const sia_tensor* bt, const sia_tensor* kv_len, int page_size,
                float sm_scale, const sia_tensor* out, void* ws, size_t ws_bytes,
@@ -461,7 +471,6 @@ int decode_any(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, co
   L.ws = ws;
   L.ws_bytes = ws_bytes;
   L.score = score;
-  if (score != nullptr) return dispatch_f32(L, g, k->dtype, out);
   // pages that do not hold whole 16-token tiles (page sizes 1-8, or any size
   // other than 16 * 2^k) go to the vector-ALU path with its per-token lookup
   bool tiled_pages = bt == nullptr || (kTile << L.a.lg_tiles_per_page) == page_size;
@@ -472,6 +481,14 @@ int decode_any(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, co
   const bool vector = k->dtype != SIA_U8 ? q->dtype == SIA_F32 || k->dtype == SIA_F32
                                          : g.D < 64 || g.B > kI4MaxBatch ||
                                                (q->dtype == SIA_F32 && !f32_matrix(g, L.a.cap_tokens));
+  if (score != nullptr) {
+    // the matrix kernels with a score function take 16-bit q over 16-bit and int8 caches; their cap has a limit
+    if (vector || !tiled_pages || g.D < 64 || k->dtype == SIA_U8 || score->cap_out > kMaxFastCap * kLog2e)
+      return dispatch_f32(L, g, k->dtype, out);
+    L.len_per_seq = L.a.kv_per_seq;
+    L.a.kv_per_seq |= score->start_per_seq;
+    return dispatch_scored(L, k->dtype);
+  }
   if (vector || !tiled_pages)
     return dispatch_f32(L, g, k->dtype, out);
   if (q->dtype == SIA_F32 && (!aligned16(out->data) || bstride(out, 0) % 16 || bstride(out, 2) % 16))

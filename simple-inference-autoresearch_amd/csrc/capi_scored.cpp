@@ -35,7 +35,8 @@ int fill_score(const sia_score_options* o, bool prompt, int64_t B, int64_t Hq, f
     s.cap_in = 2.0f * kLog2e * sm_scale / o->softcap;
     s.cap_out = o->softcap * kLog2e;
     s.cap_inv = sm_scale / o->softcap;
-    if (!(o->softcap > 0.f) || !isfinite(s.cap_in) || !isfinite(s.cap_out))
+    s.cap_log2 = 2.0f / o->softcap;
+    if (!(o->softcap > 0.f) || !isfinite(s.cap_in) || !isfinite(s.cap_out) || !isfinite(s.cap_log2))
       return fail(SIA_ERR_INVALID_ARGUMENT, "softcap must be a positive finite number");
   }
   if (o->window < 0) return fail(SIA_ERR_INVALID_ARGUMENT, "window must be positive");

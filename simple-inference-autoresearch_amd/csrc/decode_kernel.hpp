@@ -38,6 +38,7 @@
 #pragma once
 
 #include "int4.hpp"
+#include "score.hpp"
 #include "sia_common.hpp"
 #include "sk_split.hpp"
 
@@ -100,20 +101,39 @@ struct DecodeArgs {
   uint32_t k_range, ks_range, bt_range;
 };
 
+// Calls with a score function (MOD, score.hpp): each sequence's tiles are those
+// of its visible keys, from the tile of the first one on.
+struct ScoredDecodeArgs : DecodeArgs {
+  ScoreArgs s;
+  int32_t len_per_seq;                               // (kv_per_seq: lengths or first keys differ)
+};
+template <int MOD>
+using DecArgs = std::conditional_t<MOD != 0, ScoredDecodeArgs, DecodeArgs>;
+
 // --------------------------------------------------------------------- plan
 
 // Batches up to this size keep their per-sequence token counts in LDS after
 // the plan (4 bytes each), so a segment's length needs no second global read.
 constexpr int kLensInLds = 4096;
 
-__device__ __forceinline__ int seq_tiles(const DecodeArgs& a, int b) {
-  int n = a.kv_len[a.kv_per_seq ? b : 0];
-  n = n < 0 ? 0 : (n > a.cap_tokens ? a.cap_tokens : n);
-  return (n + kTile - 1) / kTile;
-}
 __device__ __forceinline__ int seq_tokens(const DecodeArgs& a, int b) {
   int n = a.kv_len[a.kv_per_seq ? b : 0];
   return n < 0 ? 0 : (n > a.cap_tokens ? a.cap_tokens : n);
+}
+__device__ __forceinline__ int seq_tokens(const ScoredDecodeArgs& a, int b) {
+  int n = a.kv_len[a.len_per_seq ? b : 0];
+  return n < 0 ? 0 : (n > a.cap_tokens ? a.cap_tokens : n);
+}
+// First visible key of sequence b of n keys, at most n (the query sits at n - 1).
+__device__ __forceinline__ int seq_first(const DecodeArgs&, int, int) { return 0; }
+__device__ __forceinline__ int seq_first(const ScoredDecodeArgs& a, int b, int n) {
+  const int start = a.s.start != nullptr ? a.s.start[a.s.start_per_seq ? b : 0] : 0;
+  return min(n, max(max(start, 0), n - a.s.window));
+}
+// Tiles that hold keys [first, n).
+__device__ __forceinline__ int tiles_of(const DecodeArgs&, int n, int) { return (n + kTile - 1) / kTile; }
+__device__ __forceinline__ int tiles_of(const ScoredDecodeArgs&, int n, int first) {
+  return n > first ? (n + kTile - 1) / kTile - first / kTile : 0;
 }
 
 // Exclusive scan over the sequences of their work (tiles + pen per nonempty
@@ -163,12 +183,12 @@ __device__ __forceinline__ void block_scan(const DecodeArgs& a, int* pre, int* r
 // and a charge would only move work between the groups of a sequence: there
 // pen is 0.  One length for the whole batch has a closed form; per-sequence
 // lengths take a block-wide min/max and scan.
-template <int NW>
-__device__ int plan_work(const DecodeArgs& a, int* pre, int* red, int tok0, int& pen) {
+template <int NW, class Args>
+__device__ int plan_work(const Args& a, int* pre, int* red, int nt0, int& pen) {
   const int T = NW * 64;
   if (!a.kv_per_seq) {
     pen = 0;   // (no prefix in LDS: seg_at has the closed form)
-    return a.B * (((tok0 + kTile - 1) / kTile) * a.UB);
+    return a.B * (nt0 * a.UB);
   }
   int* lens = pre + a.B + 1;                 // token counts, kept for the segments (small batches)
   if (a.B <= 64) {
@@ -177,7 +197,7 @@ __device__ int plan_work(const DecodeArgs& a, int* pre, int* red, int tok0, int&
     // with it 2.2 us of a group's start at 8 sequences)
     const int lane = threadIdx.x & 63;
     const int n = lane < a.B ? seq_tokens(a, lane) : 0;
-    const int nt = (n + kTile - 1) / kTile;
+    const int nt = tiles_of(a, n, lane < a.B ? seq_first(a, lane, n) : 0);
     pen = __all(lane >= a.B || nt == uniform(nt)) ? 0 : a.seg_pen;
     const int w = (nt + (nt > 0 ? pen : 0)) * a.UB;
     int incl = w;
@@ -199,7 +219,7 @@ __device__ int plan_work(const DecodeArgs& a, int* pre, int* red, int tok0, int&
   int nmin = 0x7fffffff, nmax = -1;
   for (int b = threadIdx.x; b < a.B; b += T) {
     const int n = seq_tokens(a, b);
-    const int nt = (n + kTile - 1) / kTile;
+    const int nt = tiles_of(a, n, seq_first(a, b, n));
     pre[b] = nt;
     nmin = min(nmin, nt);
     nmax = max(nmax, nt);
@@ -242,6 +262,13 @@ template <class ST, bool SV>
 __device__ __forceinline__ float scale_of(const Scales<ST, SV>& s, int i) {
   if constexpr (std::is_same<ST, F32>::value) return s.f[i];
   else return SV ? ((i & 1) ? hi_f32(F16{}, s.w[i >> 1]) : lo_f32(F16{}, s.w[i >> 1])) : lo_f32(F16{}, s.w[i]);
+}
+
+template <class ST, bool SV>
+__device__ __forceinline__ void zero_scale(Scales<ST, SV>& s, int i) {
+  if constexpr (std::is_same<ST, F32>::value) s.f[i] = 0.f;
+  else if constexpr (SV) s.w[i >> 1] &= (i & 1) ? 0xffffu : 0xffff0000u;
+  else s.w[i] = 0u;
 }
 
 // One 16-token tile's operands as held by one lane.
@@ -430,9 +457,17 @@ struct WaveState {
   f32x4 acc[D / 16];
 };
 
-template <int D, class KV, class QT, class ST, bool FULL, bool SV>
-__device__ __forceinline__ void compute_tile(const Tile<D, KV, ST, SV>& c, const u32x4* qop, const u32x4* qop_lo,
-                                             float qmul, int tile, int ntok, int grp, WaveState<D>& st) {
+// What a lane's scores of one segment are shaped with (MOD): its sequence's first
+// visible key, its head's slope in log2 units.
+struct LaneScore {
+  int first;
+  float slope2;
+};
+
+template <int D, class KV, class QT, class ST, bool FULL, bool SV, int MOD = kModNone>
+__device__ __forceinline__ void compute_tile(std::conditional_t<MOD != 0, Tile<D, KV, ST, SV>, const Tile<D, KV, ST, SV>>& c, const u32x4* qop, const u32x4* qop_lo,
+                                             float qmul, int tile, int ntok, int grp, WaveState<D>& st,
+                                             const ScoreArgs* sc = nullptr, LaneScore ls = LaneScore{}) {
   using MT = typename MmaOf<KV>::T;
   constexpr int KSTEPS = D / 32;
   constexpr int E = D / 16;
@@ -472,6 +507,24 @@ __device__ __forceinline__ void compute_tile(const Tile<D, KV, ST, SV>& c, const
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[i] = sacc[i] * qmul;
   }
+  if constexpr (MOD != kModNone) {
+    const int tok = tile * kTile + 4 * grp;
+    const float dist = (float)(ntok - 1 - tok);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (mod_cap(MOD)) s[i] = capped_log2(*sc, s[i]);
+      s[i] = __builtin_fmaf(-ls.slope2, dist - (float)i, s[i]);
+    }
+    if (tile * kTile < ls.first) {      // (uniform) the tile of the first visible key: what stands before it is no part of P V
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (tok + i < ls.first) {
+          s[i] = -INFINITY;
+          zero_raw(c.v[i]);
+          if constexpr (kInt8) zero_scale(c.vs, i);
+        }
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (!FULL && tile * kTile + 4 * grp + i >= ntok) s[i] = -INFINITY;
@@ -483,13 +536,14 @@ __device__ __forceinline__ void compute_tile(const Tile<D, KV, ST, SV>& c, const
   bool rescale = false;
   if (__any(lmax > st.m + kLazyMax)) {
     const float m_new = fmaxf(st.m, wave_max_xor16_32(lmax));
-    alpha = fast_exp2(st.m - m_new);
+    alpha = MOD != kModNone && m_new == -INFINITY ? 1.0f : fast_exp2(st.m - m_new);
     st.m = m_new;
     rescale = true;
   }
+  const float mref = MOD != kModNone && st.m == -INFINITY ? 0.f : st.m;   // (MOD: a head may have seen only scores of -Inf)
   float p[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) p[i] = fast_exp2(s[i] - st.m);
+  for (int i = 0; i < 4; ++i) p[i] = fast_exp2(s[i] - mref);
 
   u32x2 pop, pop_lo;
   if constexpr (kInt8) {
@@ -702,9 +756,9 @@ __device__ __forceinline__ int aligned_groups(const DecodeArgs& a, int nt, int G
   return uniform(more * (float)row_bytes * (1.3f / 128.0f) < 6.0f) ? G1 : G;
 }
 
-template <int D, class KV, class QT, class ST, int NW, bool SV>
+template <int D, class KV, class QT, class ST, int NW, bool SV, int MOD = kModNone>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DecodeWaves<D, KV, SV>::value)))
-void decode_main(const DecodeArgs a) {
+void decode_main(const DecArgs<MOD> a) {
   constexpr int E = D / 16;
   constexpr int KSTEPS = D / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -735,7 +789,9 @@ void decode_main(const DecodeArgs a) {
   // the split for decode_reduce.
   const int tok0 = a.kv_per_seq ? 0 : uniform(seq_tokens(a, 0));
   int pen = 0;
-  const int W = plan_work<NW>(a, pre, red, tok0, pen);
+  const int first0 = MOD != kModNone && !a.kv_per_seq ? uniform(seq_first(a, 0, tok0)) : 0;
+  const int nt0 = tiles_of(a, tok0, first0);                // (one shared length)
+  const int W = plan_work<NW>(a, pre, red, nt0, pen);
   int G = (int)gridDim.x;
   if (a.tps_force > 0) G = min(G, max(1, (W + a.tps_force - 1) / a.tps_force));   // forced share (tests)
   // least work per group, but never fewer groups than (sequence, unit block)
@@ -750,7 +806,6 @@ void decode_main(const DecodeArgs a) {
     if (a.tps_force <= 0 && G > a.cus &&
         (W < kTwoGroupTiles * shape.P * G || (pen == 0 && a.B * a.UB == a.cus)))
       G = min(G, max(a.cus, a.B * a.UB));
-  const int nt0 = (tok0 + kTile - 1) / kTile;               // (one shared length)
   if (!a.kv_per_seq && a.tps_force <= 0) G = aligned_groups(a, nt0, G, shape.P, kv_bytes<KV>(D));
   if (blockIdx.x == 0) {
     for (int i = threadIdx.x; i <= a.B; i += NW * 64)
@@ -810,13 +865,14 @@ void decode_main(const DecodeArgs a) {
   // it: a few dependent memory round trips) followed by its ntile tiles; a
   // piece of the virtual span maps to real tiles [t_lo, t_hi).
   struct SegAt {
-    int b, ntok, ntile, ublk, t_lo, t_hi, seg_end;
+    int b, ntok, ntile, ublk, t_lo, t_hi, seg_end, first;   // (tiles from the one of `first` on)
   };
   auto seg_at = [&](int xs) {
     SegAt s;
     int pb;
     if (!a.kv_per_seq) {
       s.ntok = tok0;
+      s.first = first0;
       s.ntile = nt0;
       const int sidx = (int)((uint32_t)xs / (uint32_t)nt0);  // (xs < W: nt0 > 0)
       s.b = uniform(fdiv(sidx, a.dUB));
@@ -834,7 +890,8 @@ void decode_main(const DecodeArgs a) {
       const int i = base + lane;
       s.b = base + __popcll(__ballot(i < a.B && pre[i] <= xs)) - 1;
       s.ntok = uniform(a.B <= kLensInLds ? pre[a.B + 1 + s.b] : seq_tokens(a, s.b));
-      s.ntile = (s.ntok + kTile - 1) / kTile;
+      s.first = uniform(seq_first(a, s.b, s.ntok));
+      s.ntile = tiles_of(a, s.ntok, s.first);
       pb = uniform(pre[s.b]);
     }
     const int nvt = s.ntile + pen;
@@ -860,13 +917,14 @@ void decode_main(const DecodeArgs a) {
   bool first_seg = true;
   while (x < x_hi) {
     const SegAt sg = seg_at(x);
-    const int b = sg.b, ntok = sg.ntok, ntile = sg.ntile, ublk = sg.ublk, t_lo = sg.t_lo, t_hi = sg.t_hi;
+    const int b = sg.b, ntok = sg.ntok, ntile = sg.ntile, ublk = sg.ublk;
     const int seg_end = sg.seg_end;
-    if (t_hi == t_lo) {        // only the start cost of a segment, at the end of the share
+    if (sg.t_hi == sg.t_lo) {  // only the start cost of a segment, at the end of the share
       x = seg_end;
       continue;
     }
-    const bool direct = t_lo == 0 && t_hi == ntile;
+    const bool direct = sg.t_lo == 0 && sg.t_hi == ntile;
+    const int t0 = sg.first / kTile, t_lo = sg.t_lo + t0, t_hi = sg.t_hi + t0;
     const int pslot_id = first_seg ? 2 * g : 2 * g + 1;
     const int unit = ublk * shape.units + uin;
     const bool wave_live = uin < shape.units && unit < a.U;
@@ -874,6 +932,15 @@ void decode_main(const DecodeArgs a) {
     const int nh = wave_live ? min(16, a.G - 16 * hg) : 0;    // live head columns of this wave's unit
     const bool live = lane16 < nh;
     const int hq = live ? hkv * a.G + 16 * hg + lane16 : 0;
+
+    LaneScore ls;
+    ls.first = sg.first;
+    ls.slope2 = 0.f;
+    const ScoreArgs* sc = nullptr;
+    if constexpr (MOD != kModNone) {
+      sc = &a.s;
+      if (a.s.slopes != nullptr) ls.slope2 = a.s.slopes[hq] * kLog2e;
+    }
 
     WaveState<D> st;
     st.m = -INFINITY; st.l = 0.f; st.sexp = -100;
@@ -904,7 +971,8 @@ void decode_main(const DecodeArgs a) {
       // already in flight), unless the previous segment loaded them already.
       QRawT qraw;
       int pg0;
-      constexpr bool kPartFirst = D > 64 && !(D == 256 && QSplit<KV, QT>::value) && !kInt4;   // (see below)
+      constexpr bool kPartFirst =
+          D > 64 && !(D == 256 && (QSplit<KV, QT>::value || (MOD != kModNone && !TileT::kInt8))) && !kInt4;   // (see below)
       // int4: lane l holds the page id of the wave's tile k0 + l, 64 tiles by one load
       auto page_window = [&](int k0) {
         if (!paged || i4_any<KV>()) return 0;      // (nothing to wait for)
@@ -941,7 +1009,7 @@ void decode_main(const DecodeArgs a) {
         const int hq_n = live_n ? hkv_n * a.G + 16 * hg_n + lane16 : 0;
         if constexpr (!kF32Q) q_next = load_q_raw<D, KV>(a, nx.b, hq_n, live_n, grp);
         const int32_t* btrow_n = paged ? a.bt + (int64_t)nx.b * a.bt_sb : a.kv_len;
-        const int tn = min(nx.t_lo + phase, cap_tiles - 1);
+        const int tn = min(nx.t_lo + nx.first / kTile + phase, cap_tiles - 1);
         pg_next = uniform(btrow_n[(int64_t)(tn >> a.lg_tiles_per_page) * bt_step]);
         seg_next = seg_end;
       };
@@ -1093,13 +1161,18 @@ void decode_main(const DecodeArgs a) {
       // 2000, 32/8 heads, 50.0 us against 43.8, 64 sequences of 500-2000
       // tokens, 16/16 heads, 51.1 against 43.5.  At one sequence of 1000 tokens
       // it costs 0.6 us.)  So does the split query at head_dim 256, which with it
-      // spilled 25 registers: 64 x 4096 tokens, 16/4 heads, 171.8 us against 164.9.
+      // spilled 25 registers: 64 x 4096 tokens, 16/4 heads, 171.8 us against 164.9,
+      // and 16-bit K/V with a score function there, which spilled 4.
       auto load_part = [&](TileT& last) {
         load_tile<D, KV, ST, false, SV>(a, tile_ptr(t_first + nfull * P, pgl), lo,
                                            ntok - (t_first + nfull * P) * kTile, last, lane16, grp);
       };
-      auto compute_part = [&](const TileT& last) {
-        compute_tile<D, KV, QT, ST, false>(last, qop, qop_lo, qmul, t_first + nfull * P, ntok, grp, st);
+      auto compute_part = [&](std::conditional_t<MOD != 0, TileT, const TileT>& last) {
+        compute_tile<D, KV, QT, ST, false, SV, MOD>(last, qop, qop_lo, qmul, t_first + nfull * P, ntok, grp, st, sc, ls);
+      };
+      auto compute_full = [&](std::conditional_t<MOD != 0, TileT, const TileT>& c, int k) {
+        const int t = MOD != kModNone ? t_first + k * P : 0;
+        compute_tile<D, KV, QT, ST, true, SV, MOD>(c, qop, qop_lo, qmul, t, ntok, grp, st, sc, ls);
       };
       const bool part = nt > nfull;
       std::conditional_t<kPartFirst, TileT, int> first;     // (the partial tile, where it is taken first)
@@ -1146,9 +1219,9 @@ void decode_main(const DecodeArgs a) {
           const int pg1 = __builtin_amdgcn_readlane(pgv, 0), pg2 = __builtin_amdgcn_readlane(pgv, 1);
           load_tile<D, KV, ST, true, SV>(a, tile_ptr(t_first + (k + 1) * P, pg1), lo, 16, bufB, lane16, grp);
           pgv = page_pair(k + 3);
-          compute_tile<D, KV, QT, ST, true>(bufA, qop, qop_lo, qmul, 0, ntok, grp, st);
+          compute_full(bufA, k);
           load_tile<D, KV, ST, true, SV>(a, tile_ptr(t_first + (k + 2) * P, pg2), lo, 16, bufA, lane16, grp);
-          compute_tile<D, KV, QT, ST, true>(bufB, qop, qop_lo, qmul, 0, ntok, grp, st);
+          compute_full(bufB, k + 1);
         }
         if constexpr (NW == 8) {
           __builtin_amdgcn_s_setprio(0);
@@ -1160,10 +1233,10 @@ void decode_main(const DecodeArgs a) {
         if (k + 1 < nfull) {
           load_tile<D, KV, ST, true, SV>(a, tile_ptr(t_first + (k + 1) * P, __builtin_amdgcn_readlane(pgv, 0)), lo,
                                          16, bufB, lane16, grp);
-          compute_tile<D, KV, QT, ST, true>(bufA, qop, qop_lo, qmul, 0, ntok, grp, st);
-          compute_tile<D, KV, QT, ST, true>(bufB, qop, qop_lo, qmul, 0, ntok, grp, st);
+          compute_full(bufA, k);
+          compute_full(bufB, k + 1);
         } else {
-          compute_tile<D, KV, QT, ST, true>(bufA, qop, qop_lo, qmul, 0, ntok, grp, st);
+          compute_full(bufA, k);
         }
       } else {
         prefetch_next();

@@ -31,6 +31,7 @@ struct DecodeLaunch {
   int page_size;            // paged pools: tokens per page (0: contiguous cache)
   int lg_group;             // int4 only: log2 of the elements per parameter pair
   const ScoreArgs* score;   // scored calls only
+  int len_per_seq;          // scored calls only: kv_len has an entry per sequence (a.kv_per_seq: it or kv_start has)
 };
 
 // wave_bytes: what a wave has of it by itself (its merge state; int4: its ring, which the merge reuses)
@@ -39,15 +40,15 @@ inline size_t decode_lds_bytes(size_t wave_bytes, int G16, int B, int NW) {
          (size_t)(B + 1) * 4 + (B <= kLensInLds ? (size_t)B * 4 : 0);
 }
 
-template <int D, class KV, class QT, class ST>
+template <int D, class KV, class QT, class ST, int MOD = kModNone>
 int launch_decode_typed(DecodeLaunch& L) {
   constexpr int NW = decode_waves(D);
   // int8 K/V: one vector scale load per lane (16 bytes of fp32 or 8 of fp16
   // scales) when the scale rows allow it (decided on the host, compiled as
   // two kernels)
-  auto kmain = decode_main<D, KV, QT, ST, NW, false>;
+  auto kmain = decode_main<D, KV, QT, ST, NW, false, MOD>;
   if constexpr (std::is_same<KV, I8>::value)
-    if (L.a.scale_vec) kmain = decode_main<D, KV, QT, ST, NW, true>;
+    if (L.a.scale_vec) kmain = decode_main<D, KV, QT, ST, NW, true, MOD>;
   // The split charges every segment start this many virtual tiles: starting
   // a segment costs about four dependent memory round trips (its length and
   // query, its first page id, its first tile), about two tiles of streaming
@@ -88,8 +89,14 @@ int launch_decode_typed(DecodeLaunch& L) {
                     L.a.max_items / 2 >= L.a.slots;
   // 1. main (persistent, stream-K share per group), 2. merge of the split
   // pieces (unless direct_only)
+  DecArgs<MOD> args;
+  (DecodeArgs&)args = L.a;
+  if constexpr (MOD != kModNone) {
+    args.s = *L.score;
+    args.len_per_seq = L.len_per_seq;
+  }
   const int rc = launch_kernel(kmain, dim3(L.a.slots), dim3(NW * 64), lds, L.stream, L.begin_event, L.end_event,
-                               "decode", L.a);
+                               "decode", args);
   if (rc != SIA_OK || L.a.direct_only) return rc;
   const int rows = L.a.B * L.a.Hq;
   constexpr int kRowsPerGroup = 64 / (D / 4);
@@ -149,6 +156,20 @@ int launch_decode_i4_256(DecodeLaunch& L);   // decode_i4_d256.hip
 int launch_decode_i4_f32(DecodeLaunch& L);         // decode_i4_f32.hip (float32 queries)
 int launch_decode_i4_pages(DecodeLaunch& L);       // decode_i4_pages.hip
 int launch_decode_i4_pages_256(DecodeLaunch& L);   // decode_i4_pages_d256.hip
+
+// Calls with a score function (16-bit q over f16, bf16 and int8 caches at head_dim 64, 128 and 256): capped scores, or
+// not; a head's slope is 0 where there is no bias.  decode_scored_f16.hip, _bf16.hip, _i8.hip and _d256.hip.
+template <int D, class KV, class ST>
+int launch_decode_scored_q(DecodeLaunch& L) {
+  const bool cap = L.score->cap_out > 0.f;
+  if (L.q_dtype == SIA_F16)
+    return cap ? launch_decode_typed<D, KV, F16, ST, kModCapBias>(L) : launch_decode_typed<D, KV, F16, ST, kModBias>(L);
+  return cap ? launch_decode_typed<D, KV, BF16, ST, kModCapBias>(L) : launch_decode_typed<D, KV, BF16, ST, kModBias>(L);
+}
+int launch_decode_scored_f16(DecodeLaunch& L);
+int launch_decode_scored_bf16(DecodeLaunch& L);
+int launch_decode_scored_i8(DecodeLaunch& L);
+int launch_decode_scored_256(DecodeLaunch& L, int kv_dtype);
 
 // Entry points implemented by decode_f16.hip / decode_bf16.hip / decode_i8.hip.
 int launch_decode_f16(DecodeLaunch& L);

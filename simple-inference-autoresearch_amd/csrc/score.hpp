@@ -20,6 +20,7 @@ struct ScoreArgs {
   float cap_in;                  // softcap: 2 log2(e) sm_scale / c, so that 2^(cap_in q.k) = e^(2 x / c)
   float cap_out;                 // c log2(e)
   float cap_inv;                 // sm_scale / c
+  float cap_log2;                // 2 / c
   const float* slopes;           // (Hq) fp32, or nullptr
   const int32_t* start;          // first key of a row of the batch, (1) or (B), or nullptr (0)
   const int32_t* len;            // its keys, likewise, or nullptr (all)
@@ -49,6 +50,11 @@ constexpr float kMaxFastCap = 512.0f;
 // of a weight).  float32 calls use capped_f32.
 __device__ __forceinline__ float capped(const ScoreArgs& s, float raw) {
   const float e = fast_exp2(raw * s.cap_in);
+  return __builtin_fmaf(__builtin_amdgcn_rcpf(1.0f + e), -2.0f * s.cap_out, s.cap_out);
+}
+// The same from a score in log2 units.
+__device__ __forceinline__ float capped_log2(const ScoreArgs& s, float x) {
+  const float e = fast_exp2(x * s.cap_log2);
   return __builtin_fmaf(__builtin_amdgcn_rcpf(1.0f + e), -2.0f * s.cap_out, s.cap_out);
 }
 // The same off by a few ulp of itself: near 0 the series of tanh up to its 9th power (off by 1e-8 of it at 1/4), from

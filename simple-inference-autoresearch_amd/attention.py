@@ -20,6 +20,10 @@ those lines, so a caller keeps its own projections and RoPE:
   of a prompt behind a cached prefix, whatever the cache holds (the reference's
   int8 cache returns the chunk alone, ``model/kv_cache.py:133-184``, so that it
   never sees its prefix).
+The steps take the options of a score function too (``softcap``,
+``alibi_slopes``, ``window``, ``kv_start``; :mod:`~.scored`), which the
+reference's attention does not have; without one they run as they always did.
+
 * :class:`DecodeCtx` -- the device buffers of ``model/cuda_graph_decode.py:53-56``
   (``cos``, ``sin``, ``pos_index``, ``kv_len``), with int32 positions and
   :meth:`DecodeCtx.set_position` for the per-step update
@@ -34,23 +38,28 @@ from .decode import (CONTIG, CONTIG_INT4, CONTIG_INT8, _common, _kv_len_tensor, 
                      attention_flash_decode_int4, attention_flash_decode_int8)
 from .kv_cache import KVCache
 from .prefill import attention_flash_triton
+from .scored import _scored_layer, is_scored, scored_attention_flash
 
 
-def gqa_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool | None = None) -> torch.Tensor:
+def gqa_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool | None = None, **score) -> torch.Tensor:
     """Attention of ``q (B, Hq, T, D)`` over ``k, v (B, Hkv, S, D)`` -> ``(B, T, Hq * D)``.
 
     ``causal`` defaults to the reference's rule ``T > 1`` (bottom-right
     aligned, so a query block at the end of a longer cache sees its prefix).
+    ``score``: options of :func:`~.scored.scored_attention_flash`.
     """
     B, Hq, T, D = q.shape
     if causal is None:
         causal = T > 1
+    if any(x is not None for x in score.values()):
+        return scored_attention_flash(q, k, v, causal=causal, out_token_major=True, **score).view(B, T, Hq * D)
     out = attention_flash_triton(q, k, v, causal=causal, assume_contiguous=True, out_token_major=True)
     return out.view(B, T, Hq * D)
 
 
 def prefill_step_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache: KVCache, layer_idx: int,
-                           start_pos: int) -> torch.Tensor:
+                           start_pos: int, *, softcap: float | None = None, alibi_slopes: torch.Tensor | None = None,
+                           window: int | None = None, kv_start: torch.Tensor | None = None) -> torch.Tensor:
     """Write a chunk of a prompt and attend to it and to its cached prefix, causally.
 
     ``q (B, Hq, T, D)``, ``k, v (B, Hkv, T, D)`` after RoPE, for positions
@@ -66,7 +75,8 @@ def prefill_step_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv
         kv_cache.read(layer_idx, B, start_pos, out=(kc[:, :, :start_pos], vc[:, :, :start_pos]))
         kc[:, :, start_pos:].copy_(k)
         vc[:, :, start_pos:].copy_(v)
-    return gqa_attention(q, kc, vc, causal=True)
+    return gqa_attention(q, kc, vc, causal=True, softcap=softcap, alibi_slopes=alibi_slopes, window=window,
+                         kv_start=kv_start)
 
 
 class DecodeCtx:
@@ -93,7 +103,9 @@ class DecodeCtx:
 
 def rope_decode_step_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
                                sin: torch.Tensor, kv_cache: KVCache, layer_idx: int, ctx: DecodeCtx,
-                               sm_scale: float | None = None, interleaved: bool = False) -> torch.Tensor:
+                               sm_scale: float | None = None, interleaved: bool = False, *,
+                               softcap: float | None = None, alibi_slopes: torch.Tensor | None = None,
+                               window: int | None = None, kv_start: torch.Tensor | None = None) -> torch.Tensor:
     """RoPE, cache write and attention of one decode step: ``q (B, 1, Hq, D)``, ``k, v (B, 1, Hkv, D)``.
 
     Replaces ``ops/attention.py:202-231`` (``apply_rope`` through the
@@ -108,13 +120,18 @@ def rope_decode_step_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
     qh = q_rot.transpose(1, 2)
     scale = _common(qh, kv_cache.k_cache, sm_scale)
     kl = _kv_len_tensor(ctx.kv_len, qh.device)
+    if is_scored(softcap, alibi_slopes, window, kv_start):
+        return _scored_layer(qh, kv_cache.k_cache, kv_cache.v_cache, kv_cache.k_scale, kv_cache.v_scale, layer_idx, None,
+                             kl, 0, scale, softcap, alibi_slopes, window, kv_start)
     kind = CONTIG_INT4 if kv_cache.is_int4 else CONTIG_INT8 if kv_cache.is_int8 else CONTIG
     return _run_layer(kind, qh, kv_cache.k_cache, kv_cache.v_cache, kv_cache.k_scale, kv_cache.v_scale,
                       layer_idx, None, kl, 0, scale)
 
 
 def decode_step_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache: KVCache, layer_idx: int,
-                          ctx: DecodeCtx, sm_scale: float | None = None) -> torch.Tensor:
+                          ctx: DecodeCtx, sm_scale: float | None = None, *, softcap: float | None = None,
+                          alibi_slopes: torch.Tensor | None = None, window: int | None = None,
+                          kv_start: torch.Tensor | None = None) -> torch.Tensor:
     """Write this step's K/V and attend: ``q (B, Hq, 1, D)``, ``k, v (B, Hkv, 1, D)`` -> ``(B, 1, Hq, D)``.
 
     Replaces ``ops/attention.py:210-231``: the token is written at
@@ -124,6 +141,10 @@ def decode_step_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_
     """
     B = q.shape[0]
     kv_cache.write_decode(layer_idx, ctx.pos_index, k, v)
+    if is_scored(softcap, alibi_slopes, window, kv_start):
+        return _scored_layer(q, kv_cache.k_cache, kv_cache.v_cache, kv_cache.k_scale, kv_cache.v_scale, layer_idx, None,
+                             _kv_len_tensor(ctx.kv_len, q.device), 0, _common(q, kv_cache.k_cache, sm_scale), softcap,
+                             alibi_slopes, window, kv_start)
     kc, vc, ks, vs = kv_cache._layer(layer_idx, B)
     if kv_cache.is_int4:
         return attention_flash_decode_int4(q, kc, vc, ks, vs, ctx.kv_len, sm_scale)

@@ -31,6 +31,7 @@ import torch
 from . import _lib
 from .decode import PAGED, PAGED_INT4, PAGED_INT8, _common, _run_layer
 from .kv_cache import int4_group, int4_pools, kv_read, kv_write, pools_bytes
+from .scored import _scored_layer, is_scored
 
 
 class PagedKVCache:
@@ -139,9 +140,18 @@ class PagedKVCache:
                                                   self.block_tables, self.seq_lens, -1, self.block_size,
                                                   bool(interleaved))
 
-    def decode_attention(self, layer_idx: int, q: torch.Tensor, sm_scale: float | None = None) -> torch.Tensor:
-        """Decode attention of ``q (B, Hq, 1, D)`` over each request's ``seq_lens[b]`` cached tokens."""
+    def decode_attention(self, layer_idx: int, q: torch.Tensor, sm_scale: float | None = None, *,
+                         softcap: float | None = None, alibi_slopes: torch.Tensor | None = None,
+                         window: int | None = None, kv_start: torch.Tensor | None = None) -> torch.Tensor:
+        """Decode attention of ``q (B, Hq, 1, D)`` over each request's ``seq_lens[b]`` cached tokens.
+
+        With a score function where an option of :func:`~.scored.paged_scored_attention_flash_decode` is given.
+        """
         scale = _common(q, self.k_pool, sm_scale)
+        if is_scored(softcap, alibi_slopes, window, kv_start):
+            return _scored_layer(q, self.k_pool, self.v_pool, self.k_scale_pool, self.v_scale_pool, layer_idx,
+                                 self.block_tables, self.seq_lens, self.block_size, scale, softcap, alibi_slopes, window,
+                                 kv_start)
         kind = PAGED_INT4 if self.is_int4 else PAGED_INT8 if self.is_int8 else PAGED
         return _run_layer(kind, q, self.k_pool, self.v_pool, self.k_scale_pool, self.v_scale_pool, layer_idx,
                           self.block_tables, self.seq_lens, self.block_size, scale)

@@ -28,6 +28,7 @@ import torch
 from .kv_cache import KVCache
 from .paged_kv_cache import PagedKVCache
 from .prefill import attention_flash_triton
+from .scored import scored_attention_flash
 
 ATTENTION_NAME = "sia"
 
@@ -75,6 +76,17 @@ def _padding_free(attention_mask) -> bool:
     return attention_mask is None
 
 
+def _documents(query: torch.Tensor, key: torch.Tensor, kwargs: dict) -> torch.Tensor | None:
+    """First positions of the documents packed into one row, from the lengths that the caller's collator passes."""
+    cuts, of_keys = kwargs.get("cu_seq_lens_q"), kwargs.get("cu_seq_lens_k")
+    if cuts is None and of_keys is None:
+        return None
+    if query.shape[0] != 1 or query.shape[2] != key.shape[2] or cuts is None or of_keys is None:
+        raise NotImplementedError("packed documents are supported in one row without a cached prefix, with cu_seq_lens_q "
+                                  "and cu_seq_lens_k alike")
+    return cuts if cuts.dtype == torch.int32 else cuts.to(torch.int32)
+
+
 def sia_attention_forward(module, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, attention_mask,
                           dropout: float = 0.0, scaling: float | None = None, is_causal: bool | None = None,
                           **kwargs):
@@ -82,19 +94,25 @@ def sia_attention_forward(module, query: torch.Tensor, key: torch.Tensor, value:
 
     Causal (bottom-right aligned, so a query block at the end of a cached
     prefix sees the whole prefix) when the module is causal, full otherwise.
-    GQA is resolved by head index, with no ``repeat_kv`` copy.  Padding masks,
-    dropout, sliding windows and soft-capping have no kernel here and raise
-    ``NotImplementedError`` rather than being ignored.
+    GQA is resolved by head index, with no ``repeat_kv`` copy.  ``softcap`` and
+    ``sliding_window`` (a key is seen from fewer than that many positions away)
+    run the scored kernels, as do the documents of a packed row, passed as
+    ``cu_seq_lens_q`` and ``cu_seq_lens_k`` for a batch of one.  Padding masks
+    and dropout have no kernel here and raise ``NotImplementedError`` rather
+    than being ignored.
     """
     if dropout:
         raise NotImplementedError("attention dropout is not supported by the gfx950 kernels")
-    if kwargs.get("sliding_window") is not None or kwargs.get("softcap") is not None:
-        raise NotImplementedError("sliding-window / soft-capped attention is not supported")
     if not _padding_free(attention_mask):
         raise NotImplementedError("an attention mask (padded batch or static-cache slots) is not supported; "
                                   "un-padded batches reach this function with attention_mask=None")
     causal = getattr(module, "is_causal", True) if is_causal is None else bool(is_causal)
-    out = attention_flash_triton(query, key, value, causal=causal, sm_scale=scaling, out_token_major=True)
+    softcap, window, cuts = kwargs.get("softcap"), kwargs.get("sliding_window"), _documents(query, key, kwargs)
+    if softcap is None and window is None and cuts is None:
+        out = attention_flash_triton(query, key, value, causal=causal, sm_scale=scaling, out_token_major=True)
+    else:
+        out = scored_attention_flash(query, key, value, causal=causal, sm_scale=scaling, softcap=softcap, window=window,
+                                     cu_seqlens=cuts, out_token_major=True)
     return out, None
 
 

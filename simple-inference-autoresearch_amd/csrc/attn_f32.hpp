@@ -70,7 +70,7 @@ using F32ArgsOf = std::conditional_t<SC, F32ScoredArgs, F32Args>;
 
 struct F32Launch {
   F32Args a;
-  const ScoreArgs* score;   // launch_attn_f32_scored only
+  const ScoreArgs* score;   // launch_attn_f32_scored; launch_attn_f32_prefill: nullptr, or with a score function
   int D;
   int q_dtype;       // also the output dtype
   int kv_dtype;

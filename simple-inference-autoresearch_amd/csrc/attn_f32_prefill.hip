@@ -44,9 +44,11 @@ __device__ __forceinline__ int f32_dim(int r, int e) {
   return ET <= 4 ? ET * r + e : 128 * (e >> 2) + 4 * r + (e & 3);
 }
 
-template <int D>
+// SC (1, or 2: with a cap): scores shaped by a.s, and a run of keys [clo, lim) per column (score.hpp);
+// the group walks the tiles of the union of its columns' runs.
+template <int D, int SC = 0>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1)))
-void attn_f32_prefill(const F32Args a) {
+void attn_f32_prefill(const F32ArgsOf<(SC != 0)> a) {
   constexpr int ET = D < 32 ? 1 : D / 32;       // 32-dimension tiles of O^T
   constexpr int KQ = D / 8;                      // 16-byte pieces of a row per half wave
   constexpr bool kAhead = D <= 32;               // whole tiles of K and V in flight (else parts of them)
@@ -69,10 +71,24 @@ void attn_f32_prefill(const F32Args a) {
   const bool live = col < a.ncol;
   const int i = live ? col / a.G : 0, g = live ? col - i * a.G : 0;
   const int off = a.Tk - a.Tq + 1;               // keys visible to row 0 under the causal mask
-  const int lim = !live ? 0 : a.causal ? max(0, min(a.Tk, off + i)) : a.Tk;
+  int lim = !live ? 0 : a.causal ? max(0, min(a.Tk, off + i)) : a.Tk;
   const int i_last = uniform(min(chunk * kF32TileCols + kF32TileCols - 1, a.ncol - 1) / a.G);
-  const int hi = a.causal ? max(0, min(a.Tk, off + i_last)) : a.Tk;   // keys of the group's last column
+  int hi = a.causal ? max(0, min(a.Tk, off + i_last)) : a.Tk;   // keys of the group's last column
   const int lim0 = a.causal ? min(a.Tk, off + uniform(chunk * kF32TileCols / a.G)) : a.Tk;   // of its first one
+  int clo = 0, t_first = 0;                      // SC: this column's first key, the group's first tile
+  float slope2 = 0.f;
+  const int p = a.Tk - a.Tq + i;                 // this column's position
+  if constexpr (SC != 0) {
+    const int i0 = uniform(chunk * kF32TileCols / a.G), p0 = a.Tk - a.Tq + i0, n = i_last - i0;
+    const SeqBounds sb = seq_bounds(a.s, b, a.Tk);
+    const Documents dc = documents(a.s, b, p0, p0, p0 + n, lane);
+    const int r = live ? i - i0 : 0;             // (dead columns: anything, they see no key)
+    clo = max(0, row_lo(a.s, sb, p, dc.lo(p0, r)));
+    lim = live ? row_hi(a.s, sb, p, dc.hi(p0, r)) : 0;
+    t_first = uniform(max(0, row_lo(a.s, sb, p0, dc.g_below)) / 32);
+    hi = uniform(row_hi(a.s, sb, p0 + n, dc.g_above));
+    if (a.s.slopes != nullptr) slope2 = a.s.slopes[hkv * a.G + g] * kLog2e;
+  }
 
   const char* qp = a.q + b * a.q_sb + (int64_t)(hkv * a.G + g) * a.q_sh + (int64_t)i * a.q_sm + 16 * h;
   // q operand: column l32, dims 8 j + 4 h + [0, 4) of piece j (dead columns
@@ -120,6 +136,7 @@ void attn_f32_prefill(const F32Args a) {
       load_v1(min(t * 32 + 8 * ((j0 + j) >> 2) + 4 * h + ((j0 + j) & 3), hi - 1), v[j], e0);
   };
 
+  const uint32_t clen = (uint32_t)max(0, lim - clo);
   f32x16 o[ET];
 #pragma unroll
   for (int e = 0; e < ET; ++e) o[e] = f32x16{};
@@ -130,18 +147,25 @@ void attn_f32_prefill(const F32Args a) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       const int key = t * 32 + 8 * (j >> 2) + 4 * h + (j & 3);
-      s[j] = key < lim ? s[j] : -INFINITY;
+      if constexpr (SC != 0) {                          // (log2 units from here on)
+        s[j] = SC == 2 ? capped_f32(a.s, s[j]) : s[j] * a.qk_scale;
+        s[j] -= slope2 * fabsf((float)(p - key));
+        s[j] = (uint32_t)(key - clo) < clen ? s[j] : -INFINITY;
+        if (D >= 128 || (j & 3) == 3) __builtin_amdgcn_sched_barrier(0);   // (few at a time: sixteen together spilled)
+      } else {
+        s[j] = key < lim ? s[j] : -INFINITY;
+      }
       mx = fmaxf(mx, s[j]);
     }
     float lo, up;
     halves(mx, lo, up);
-    const float M = fmaxf(m, fmaxf(lo, up) * a.qk_scale);
+    const float M = fmaxf(m, SC != 0 ? fmaxf(lo, up) : fmaxf(lo, up) * a.qk_scale);
     const float mu = M == -INFINITY ? 0.f : M;     // nothing visible yet
     const float alpha = fast_exp2(m - mu);
     float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      s[j] = fast_exp2(__builtin_fmaf(s[j], a.qk_scale, -mu));
+      s[j] = fast_exp2(SC != 0 ? s[j] - mu : __builtin_fmaf(s[j], a.qk_scale, -mu));
       ps[j & 3] += s[j];
     }
     l = l * alpha + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
@@ -194,7 +218,8 @@ void attn_f32_prefill(const F32Args a) {
   // was 2.0-2.1e-7 of the result up to head_dim 64, now 1.9e-7.)  In a tile
   // with keys that not every column sees (they weigh 0), values that are not
   // finite go one key at a time, as 0 times those is NaN: so a hidden key's
-  // never reach a column, whichever columns share the group.
+  // never reach a column, whichever columns share the group.  (SC:
+  // columns that come out not finite are computed again at the end instead.)
   auto pv = [&](const float (*v)[EP], int t, int j0, int n, int e0, const f32x16& s, auto check) {
     if (decltype(check)::value && t * 32 + 31 >= lim0) {
       float z[4] = {0.f, 0.f, 0.f, 0.f};               // (0 x Inf and 0 x NaN are NaN, and stay)
@@ -226,10 +251,10 @@ void attn_f32_prefill(const F32Args a) {
       if ((t + 4) * 32 < hi) load_k(t + 4, knext, 0, KQ);
       f32x16 s = qk(k, 0, std::integral_constant<int, KQ>{});
       softmax(t, s);
-      pv(v, t, 0, 16, 0, s, std::true_type{});
+      pv(v, t, 0, 16, 0, s, std::bool_constant<SC == 0>{});
     };
     f32x4 ka[KQ], kn[KQ];
-    int t = wave;
+    int t = t_first + wave;
     if (t * 32 < hi) load_k(t, ka, 0, KQ);
     for (; t * 32 < hi; t += 8) {
       tile(t, ka, kn);
@@ -241,7 +266,7 @@ void attn_f32_prefill(const F32Args a) {
     constexpr int NH = ET / EP, NV = NC * NH;      // V parts: VC registers, EP tiles of dimensions
     f32x4 k[2][KC];
     float v[2][VC][EP];
-    if (wave * 32 < hi) load_k(wave, k[0], 0, KC);
+    if ((t_first + wave) * 32 < hi) load_k(t_first + wave, k[0], 0, KC);
     auto tile = [&](int t, auto check) {
       f32x16 s;
 #pragma unroll
@@ -266,9 +291,10 @@ void attn_f32_prefill(const F32Args a) {
         __builtin_amdgcn_sched_barrier(0);
       }
     };
-    int t = wave;
-    for (; t * 32 + 31 < lim0; t += 4) tile(t, std::false_type{});   // (with the check 2-4% slower from 512 tokens on)
-    for (; t * 32 < hi; t += 4) tile(t, std::true_type{});
+    int t = t_first + wave;
+    if constexpr (SC == 0)
+      for (; t * 32 + 31 < lim0; t += 4) tile(t, std::false_type{});   // (with the check 2-4% slower from 512 tokens on)
+    for (; t * 32 < hi; t += 4) tile(t, std::bool_constant<SC == 0>{});
   }
 
   // merge the 4 waves: every state scaled to the common max, then added
@@ -307,9 +333,32 @@ void attn_f32_prefill(const F32Args a) {
   if (wave < 2) add(sm_o[wave]);
   if (wave == 1) put(sm_o[1]);
   __syncthreads();
-  if (wave != 0 || chunk * kF32TileCols + l32 >= a.ncol) return;
+  if (wave != 0 || (SC == 0 && chunk * kF32TileCols + l32 >= a.ncol)) return;
   add(sm_o[1]);
   const float inv = L == 0.f ? 0.f : 1.0f / L;     // no visible key: zeros (the reference's l_safe guard)
+  if constexpr (SC != 0) {
+    float z = 0.f;
+#pragma unroll
+    for (int e = 0; e < ET; ++e)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) z = __builtin_fmaf(o[e][j], 0.f, z);
+    if (__any(z != z)) {
+#pragma unroll 1
+      for (int r = 0; r < min(kF32TileCols, a.ncol - chunk * kF32TileCols); ++r) {
+        const int cr = chunk * kF32TileCols + r, ir = cr / a.G, hr = hkv * a.G + cr - ir * a.G;
+        const int pr = a.Tk - a.Tq + ir;
+        const SeqBounds sb = seq_bounds(a.s, b, a.Tk);
+        const Documents dc = documents(a.s, b, pr, pr, pr, lane);
+        scored_row<D, F32>(a.s, a.qk_scale, a.s.slopes != nullptr ? a.s.slopes[hr] * kLog2e : 0.f,
+                           a.q + b * a.q_sb + (int64_t)hr * a.q_sh + (int64_t)ir * a.q_sm, a.k + b * a.k_s0 + (int64_t)hkv * a.k_sh,
+                           a.k_sn, a.v + b * a.v_s0 + (int64_t)hkv * a.v_sh, a.v_sn, pr,
+                           row_lo(a.s, sb, pr, dc.g_below), row_hi(a.s, sb, pr, dc.g_above),
+                           a.out + b * a.o_sb + (int64_t)hr * a.o_sh + (int64_t)ir * a.o_sm, lane);
+      }
+      return;
+    }
+  }
+  if (SC != 0 && chunk * kF32TileCols + l32 >= a.ncol) return;   // (every lane takes part in a row computed again)
   int c2 = (int)threadIdx.x & 31;
   asm volatile("" : "+v"(c2));                     // (computed again: held through the loop, they were spilled)
   c2 += chunk * kF32TileCols;
@@ -339,7 +388,15 @@ static int launch_d(F32Launch& L) {
   if (items == 0) return SIA_OK;
   const int cus = device_info().cus;
   L.a.fold = L.a.causal && items > cus && items <= 2 * (int64_t)cus && D <= 128 ? cus : 0;
-  hipLaunchKernelGGL((attn_f32_prefill<D>), dim3((unsigned)items), dim3(256), 0, L.stream, L.a);
+  if (L.score != nullptr) {
+    F32ScoredArgs a;
+    (F32Args&)a = L.a;
+    a.s = *L.score;
+    if (a.s.cap_out > 0.f) hipLaunchKernelGGL((attn_f32_prefill<D, 2>), dim3((unsigned)items), dim3(256), 0, L.stream, a);
+    else hipLaunchKernelGGL((attn_f32_prefill<D, 1>), dim3((unsigned)items), dim3(256), 0, L.stream, a);
+  } else {
+    hipLaunchKernelGGL((attn_f32_prefill<D>), dim3((unsigned)items), dim3(256), 0, L.stream, L.a);
+  }
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? SIA_OK : fail(SIA_ERR_LAUNCH, "fp32 prefill launch: %s", hipGetErrorString(e));
 }

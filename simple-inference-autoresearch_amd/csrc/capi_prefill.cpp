@@ -105,7 +105,7 @@ KeySplit key_splits(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk, 
 // Float32 q/k/v: fp32 MFMAs (attn_f32_prefill.hip), one work-group per
 // (sequence, KV head, 32 query rows x heads), no workspace.
 int prefill_f32(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, int32_t causal, float sm_scale,
-                const sia_tensor* out, void* stream) {
+                const sia_tensor* out, void* stream, const ScoreArgs* score = nullptr) {
   const int64_t B = q->shape[0], Hq = q->shape[1], Tq = q->shape[2], D = q->shape[3];
   const int64_t Hkv = k->shape[1], Tk = k->shape[2];
   const int64_t G = Hq / Hkv;
@@ -131,6 +131,7 @@ int prefill_f32(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, i
   L.q_dtype = SIA_F32;
   L.kv_dtype = SIA_F32;
   L.stream = (hipStream_t)stream;
+  L.score = score;
   return launch_attn_f32_prefill(L);
 }
 
@@ -252,7 +253,8 @@ int flash_fwd(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, int
     if ((rc = fill_score(score->options, true, B, Hq, sm_scale, causal, sc))) return rc;
     if ((rc = device_ok())) return rc;
     if (Tq == 0) return SIA_OK;
-    if (q->dtype == SIA_F32 || sc.cap_out > kMaxFastCap * kLog2e) return scored_rows(q, k, v, sm_scale, sc, out, stream);
+    if (q->dtype == SIA_F32) return prefill_f32(q, k, v, causal, sm_scale, out, stream, &sc);
+    if (sc.cap_out > kMaxFastCap * kLog2e) return scored_rows(q, k, v, sm_scale, sc, out, stream);
   }
   if (q->dtype == SIA_F32) {
     if (rope != nullptr)

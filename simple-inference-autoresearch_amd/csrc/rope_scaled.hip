@@ -9,7 +9,8 @@
 //
 // Memory-bound: q and k once in, once out.  A work-group takes a few tokens: it computes each token's R / 2 pairs of sine
 // and cosine once, into LDS, while its first elements are in flight, and every head's items read them there.  An item is
-// PP pairs of a head (8: two 16-byte accesses of 16-bit elements), or 2 PP of the elements behind the rotated part.
+// PP pairs of a head, in two runs of PP elements (half layout) or one of 2 PP (interleaved), 16 bytes each where the
+// layout allows, or as many of the elements behind the rotated part: consecutive items take consecutive runs.
 #include <string.h>
 
 #include <algorithm>
@@ -25,7 +26,7 @@ struct RopeScaledArgs {
   const char* pos; int64_t p_sb, p_st;                 // element strides
   const char* freq;
   int32_t rows, T, Hq, H, D, R;                        // rows = B T, H = Hq + Hkv
-  int32_t tokens;                                      // per work-group
+  int32_t tokens, block;                               // per work-group; its threads
   int32_t pos64, freq64;
   float scale;
   FastDiv dT, dHead, dItems;                           // by T, items of a head, items of a token
@@ -110,17 +111,43 @@ __device__ __forceinline__ Words<N * T::bytes> words(const float* x) {
   return r;
 }
 
-constexpr int kRopeThreads = 256;
+// Two runs of BYTES as one item, and its run i.  (Runs of a single 16-bit element share a word.)
+template <int BYTES>
+__device__ __forceinline__ Words<2 * BYTES> join(const Words<BYTES>& a, const Words<BYTES>& b) {
+  Words<2 * BYTES> r;
+  if constexpr (BYTES == 2) {
+    r.w[0] = a.w[0] | b.w[0] << 16;
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 4; ++i) { r.w[i] = a.w[i]; r.w[BYTES / 4 + i] = b.w[i]; }
+  }
+  return r;
+}
+template <int BYTES>
+__device__ __forceinline__ Words<BYTES> part(const Words<2 * BYTES>& x, int i) {
+  Words<BYTES> r;
+  if constexpr (BYTES == 2) {
+    r.w[0] = i ? x.w[0] >> 16 : x.w[0] & 0xffffu;
+  } else {
+#pragma unroll
+    for (int k = 0; k < BYTES / 4; ++k) r.w[k] = x.w[i * (BYTES / 4) + k];
+  }
+  return r;
+}
+
+constexpr int kRopeThreads = 256;     // most threads of a work-group
 constexpr int kRopeMaxSc = 2048;      // (sine, cosine) pairs that a work-group's LDS holds: 16 KB
 
 template <class T, bool IL, int PP>
 __global__ __launch_bounds__(kRopeThreads) void rope_scaled_kernel(const RopeScaledArgs a) {
   __shared__ float2 sc[kRopeMaxSc];
   constexpr int ES = T::bytes, N = PP * ES;
+  constexpr bool kOneRun = IL && PP > 1;               // an item's 2 N bytes are one run (else two of N)
   const int row0 = blockIdx.x * a.tokens, nrow = min(a.tokens, a.rows - row0), half = a.R / 2;
   const int token_items = a.H * a.head_items;
   const int items = nrow * token_items;
-  // item it -> its two runs of PP elements in and out, and its first pair (-1: copied)
+  const int copy_items = a.head_items - a.rot_items;
+  // item it -> its runs in and out, the distance of the second, and its first pair (-1: copied)
   struct Item { const char* src; char* dst; int gap, pair; };
   auto item = [&](int it) {
     Item r;
@@ -128,26 +155,27 @@ __global__ __launch_bounds__(kRopeThreads) void rope_scaled_kernel(const RopeSca
     const int h = fdiv(i, a.dHead), c = i - h * a.head_items;
     const int row = row0 + t, b = fdiv(row, a.dT), tt = row - b * a.T;
     const int w = h < a.Hq ? 0 : 1, hh = h - (w ? a.Hq : 0);
-    r.src = a.x[w] + b * a.sb[w] + tt * a.st[w] + hh * a.sh[w];
-    r.dst = a.o[w] + b * a.ob[w] + tt * a.ot[w] + hh * a.oh[w];
     const bool rot = c < a.rot_items;
-    const int at = rot ? (IL ? 2 * PP * c : PP * c) : a.R + 2 * PP * (c - a.rot_items);
-    r.gap = (rot && !IL ? half : PP) * ES;
+    const int at = rot ? c * (IL ? 2 * N : N) : a.R * ES + (c - a.rot_items) * (kOneRun ? 2 * N : N);
+    r.src = a.x[w] + b * a.sb[w] + tt * a.st[w] + hh * a.sh[w] + at;
+    r.dst = a.o[w] + b * a.ob[w] + tt * a.ot[w] + hh * a.oh[w] + at;
+    r.gap = !rot ? copy_items * N : IL ? N : half * ES;
     r.pair = rot ? t * half + PP * c : -1;
-    r.src += at * ES;
-    r.dst += at * ES;
     return r;
+  };
+  auto load = [&](const Item& r) {
+    if constexpr (kOneRun) return get<2 * N>(r.src);
+    else return join(get<N>(r.src), get<N>(r.src + r.gap));
   };
   // the first item's elements fly while the sines are computed
   int it = threadIdx.x;
   Item cur{};
-  Words<N> wa{}, wb{};
+  Words<2 * N> x{};
   if (it < items) {
     cur = item(it);
-    wa = get<N>(cur.src);
-    wb = get<N>(cur.src + cur.gap);
+    x = load(cur);
   }
-  for (int i = threadIdx.x; i < nrow * half; i += kRopeThreads) {
+  for (int i = threadIdx.x; i < nrow * half; i += blockDim.x) {
     const int t = i / half, pair = i - t * half;
     const int row = row0 + t, b = fdiv(row, a.dT), tt = row - b * a.T;
     const int64_t pi = b * a.p_sb + tt * a.p_st;
@@ -161,41 +189,32 @@ __global__ __launch_bounds__(kRopeThreads) void rope_scaled_kernel(const RopeSca
   }
   __syncthreads();
   while (it < items) {
-    const int next = it + kRopeThreads;
+    const int next = it + blockDim.x;
     Item nx{};
-    Words<N> na{}, nb{};
+    Words<2 * N> y{};
     if (next < items) {
       nx = item(next);
-      na = get<N>(nx.src);
-      nb = get<N>(nx.src + nx.gap);
+      y = load(nx);
     }
     if (cur.pair >= 0) {
-      float xa[PP], xb[PP];
+      float e[2 * PP];
 #pragma unroll
       for (int i = 0; i < PP; ++i) {
-        const float2 y = sc[cur.pair + i];
-        const float p = IL ? (2 * i < PP ? elem<T>(wa, 2 * i) : elem<T>(wb, PP > 1 ? 2 * i - PP : 0)) : elem<T>(wa, i);
-        const float q = IL ? (2 * i + 1 < PP ? elem<T>(wa, 2 * i + 1) : elem<T>(wb, PP > 1 ? 2 * i + 1 - PP : 0))
-                           : elem<T>(wb, i);
-        float u, v;
-        rope_rotate(p, q, y.y, y.x, u, v);
-        if constexpr (IL) {
-          if (2 * i < PP) xa[2 * i] = u; else xb[PP > 1 ? 2 * i - PP : 0] = u;
-          if (2 * i + 1 < PP) xa[2 * i + 1] = v; else xb[PP > 1 ? 2 * i + 1 - PP : 0] = v;
-        } else {
-          xa[i] = u;
-          xb[i] = v;
-        }
+        const float2 v = sc[cur.pair + i];
+        const int p = IL ? 2 * i : i, q = IL ? 2 * i + 1 : PP + i;
+        rope_rotate(elem<T>(x, p), elem<T>(x, q), v.y, v.x, e[p], e[q]);
       }
-      wa = words<T, PP>(xa);
-      wb = words<T, PP>(xb);
+      x = words<T, 2 * PP>(e);
     }
-    put<N>(cur.dst, wa);
-    put<N>(cur.dst + cur.gap, wb);
+    if constexpr (kOneRun) {
+      put<2 * N>(cur.dst, x);
+    } else {
+      put<N>(cur.dst, part<N>(x, 0));
+      put<N>(cur.dst + cur.gap, part<N>(x, 1));
+    }
     it = next;
     cur = nx;
-    wa = na;
-    wb = nb;
+    x = y;
   }
 }
 
@@ -203,9 +222,12 @@ namespace {
 
 template <class T, bool IL>
 int launch_rope_scaled_pp(const RopeScaledArgs& a, int pp, dim3 grid, hipStream_t st) {
-  if (pp == 8) hipLaunchKernelGGL((rope_scaled_kernel<T, IL, 8>), grid, dim3(kRopeThreads), 0, st, a);
-  else if (pp == 4) hipLaunchKernelGGL((rope_scaled_kernel<T, IL, 4>), grid, dim3(kRopeThreads), 0, st, a);
-  else hipLaunchKernelGGL((rope_scaled_kernel<T, IL, 1>), grid, dim3(kRopeThreads), 0, st, a);
+  const dim3 block((unsigned)a.block);
+  // (16 bytes a run: 8 or 4 pairs of 16-bit elements, 4 or 2 of 32-bit ones; half of that; single pairs)
+  constexpr int kMost = 16 / (IL ? 2 * T::bytes : T::bytes);
+  if (pp == kMost) hipLaunchKernelGGL((rope_scaled_kernel<T, IL, kMost>), grid, block, 0, st, a);
+  else if (pp == kMost / 2 && kMost > 2) hipLaunchKernelGGL((rope_scaled_kernel<T, IL, kMost / 2>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((rope_scaled_kernel<T, IL, 1>), grid, block, 0, st, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? SIA_OK : fail(SIA_ERR_LAUNCH, "rope launch: %s", hipGetErrorString(e));
 }
@@ -279,10 +301,12 @@ extern "C" int sia_rope_scaled(const sia_tensor* q, const sia_tensor* k, const s
   a.rows = (int32_t)(B * T); a.T = (int32_t)T; a.Hq = (int32_t)q->shape[2]; a.H = (int32_t)H;
   a.D = (int32_t)D; a.R = (int32_t)R;
   a.scale = scale;
-  // the widest items whose runs of elements start at multiples of their size (at most 16 bytes) everywhere
+  // the widest items whose runs start at multiples of their size everywhere
+  const int most = 16 / (interleaved ? 2 * es : es);
   int pp = 1;
-  for (const int p : {8, 4}) {
-    const int64_t al = std::min(16, p * es);
+  for (const int p : {most, most / 2}) {
+    if (p < 2) break;
+    const int64_t al = (interleaved ? 2 : 1) * p * es;
     bool ok = (R / 2) % p == 0 && (D - R) % (2 * p) == 0;
     for (int w = 0; w < (k != nullptr ? 2 : 1); ++w) {
       const int64_t at[] = {(int64_t)(uintptr_t)a.x[w], (int64_t)(uintptr_t)a.o[w], a.sb[w], a.st[w], a.sh[w], a.ob[w], a.ot[w], a.oh[w]};
@@ -302,10 +326,13 @@ extern "C" int sia_rope_scaled(const sia_tensor* q, const sia_tensor* k, const s
   a.dItems = make_fastdiv((uint32_t)(H * a.head_items));
   int rc;
   if ((rc = device_ok())) return rc;
-  // tokens per work-group: as many as leave four groups per CU, at most 4 items a thread and the sines that fit
-  int64_t tokens = std::max<int64_t>(1, 4LL * kRopeThreads / (H * a.head_items));
-  tokens = std::min(tokens, std::max<int64_t>(1, (B * T) / (4LL * device_info().cus)));
+  // A token per work-group, or as many as give each thread an item (and whose sines fit).  8192 tokens, 32/8 heads of 128
+  // (168 MB), half layout / interleaved, us: groups of 256 threads 30.3 / 32.0 (5.5 TB/s), with four tokens 32.3 / 34.2;
+  // of 320 threads, an item each in the half layout, 34.0 / 37.3, of 128 32.3 / 36.5, of 64 35.5 / 46.5.
+  int64_t tokens = std::max<int64_t>(1, kRopeThreads / (H * a.head_items));
+  tokens = std::min(tokens, B * T);
   tokens = std::min<int64_t>(tokens, kRopeMaxSc / (R / 2));
+  a.block = (int32_t)std::min<int64_t>(kRopeThreads, (tokens * H * a.head_items + 63) / 64 * 64);
   a.tokens = (int32_t)tokens;
   const dim3 grid((unsigned)((B * T + tokens - 1) / tokens));
   const hipStream_t st = (hipStream_t)stream;

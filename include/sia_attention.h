@@ -278,7 +278,8 @@ typedef struct sia_score_options {
 int sia_scored_attention_flash_fwd(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, int32_t causal,
                                    float sm_scale, const sia_score_options* score, const sia_tensor* out,
                                    void* workspace, size_t workspace_bytes, void* stream);
-int sia_scored_attention_flash_fwd_workspace_size(const sia_tensor* q, const sia_tensor* k, size_t* bytes);
+int sia_scored_attention_flash_fwd_workspace_size(const sia_tensor* q, const sia_tensor* k, int32_t causal,
+                                                  const sia_score_options* score, size_t* bytes);
 
 /* One decode step, the query at position kv_len[b] - 1: the arguments of
  * sia_attention_flash_decode (block_table NULL, page_size 0) or

@@ -124,7 +124,7 @@ _SIGNATURES = {
     "sia_attention_flash_fwd_rope": [_P, _P, _P, _P, _P, _I32, _P, _I32, _I32, _F, _P, _VP, _SZ, _VP],
     "sia_attention_flash_fwd_workspace_size": [_P, _P, ctypes.POINTER(_SZ)],
     "sia_scored_attention_flash_fwd": [_P, _P, _P, _I32, _F, ctypes.POINTER(ScoreOptions), _P, _VP, _SZ, _VP],
-    "sia_scored_attention_flash_fwd_workspace_size": [_P, _P, ctypes.POINTER(_SZ)],
+    "sia_scored_attention_flash_fwd_workspace_size": [_P, _P, _I32, ctypes.POINTER(ScoreOptions), ctypes.POINTER(_SZ)],
     "sia_scored_attention_flash_decode": [_P, _P, _P, _P, _P, _P, _P, _I32, _F, ctypes.POINTER(ScoreOptions), _P, _VP,
                                           _SZ, ctypes.POINTER(DecodeOptions), _VP],
     "sia_rope_scaled": [_P, _P, _P, _P, _I32, _I32, _F, _P, _P, _VP],

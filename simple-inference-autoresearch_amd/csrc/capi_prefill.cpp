@@ -2,6 +2,8 @@
 #include <math.h>
 #include <string.h>
 
+#include <algorithm>
+
 #include "attn_f32.hpp"
 #include "host_util.hpp"
 #include "prefill_launch.hpp"
@@ -63,9 +65,11 @@ struct KeySplit {
 // against 39: the partials and the merge cost more than the chain saves).
 // Two groups per CU are counted at head_dim 64, where the registers hold
 // three: the constants were fitted so.
-KeySplit key_splits(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t D, bool bf16, int cus) {
+// (run: the most keys that a work-group's rows see, where a window leaves fewer than Tk)
+KeySplit key_splits(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t D, bool bf16, int cus,
+                    int64_t run = INT64_MAX) {
   KeySplit best;
-  const int64_t nkb = (Tk + kPfBN - 1) / kPfBN;
+  const int64_t nkb = (std::min(Tk, run) + kPfBN - 1) / kPfBN;
   if ((D != 64 && D != 128 && D != 256) || Tq <= 0 || nkb < 8 || cus <= 0) return best;
   const int64_t rows = B * Hq * Tq, row_bytes = (D + 2) * 4;
   const int64_t most_bytes = (int64_t)256 << 20;      // (also keeps rows below 2^31, as the merge indexes them)
@@ -197,6 +201,11 @@ struct ScoreIn {
   const sia_score_options* options;
 };
 
+// Keys that the rows of one work-group see at most under a window (256 rows, whatever the variant).
+int64_t window_run(const ScoreArgs& s) {
+  return s.causal && s.prefix == nullptr ? (int64_t)s.window + 256 : 2 * (int64_t)s.window + 256;
+}
+
 // Scored attention one row per wave: any type.
 int scored_rows(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, float sm_scale, const ScoreArgs& s,
                 const sia_tensor* out, void* stream) {
@@ -288,9 +297,18 @@ int flash_fwd(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, int
   // groups instead (prefill_fwd variant 1): twice the groups, each with half
   // the rows.  (Up to two 8-wave groups per CU this was measured slower.)
   L.var = D == 128 && groups(B, Hkv, a.G, Tq, (int)D, 0) <= dev.cus ? 1 : 0;
+  // Scored calls whose rows see short runs (a window, documents, or few keys) take
+  // the 4-wave groups whatever the grid: two share a CU, and one's prologue and
+  // epilogue overlap the other's blocks.  us, 8 waves / 4: 16384 tokens in 24
+  // documents 254 / 245, 2 x 4096 with a window of 512 103.6 / 96.2, 8 x 700 (G =
+  // 3) 30.3 / 25.2, 4 x 2048 capped 186 / 185; but 8192 tokens unmasked 497 / 512,
+  // 4096 in fp16 169 / 178.
+  if (score != nullptr && D == 128 && (sc.cuts != nullptr || std::min<int64_t>(Tk, sc.window) <= 2048)) L.var = 1;
   // Few query rows over many keys: variant 3 or 4, when the caller's workspace
   // also holds the partials (the size of sia_attention_flash_fwd_workspace_size)
-  const KeySplit ks = v_rows_ok && score == nullptr ? key_splits(B, Hq, Hkv, Tq, Tk, D, q->dtype == SIA_BF16, dev.cus) : KeySplit();
+  const KeySplit ks = v_rows_ok ? key_splits(B, Hq, Hkv, Tq, Tk, D, q->dtype == SIA_BF16, dev.cus,
+                                             score != nullptr ? window_run(sc) : INT64_MAX)
+                                : KeySplit();
   const int64_t images = ks.var == 4 ? need : 0;         // (variant 3 needs none)
   if (ks.ns > 1 && workspace != nullptr && (uintptr_t)workspace % 256 == 0 &&
       workspace_bytes >= (size_t)(images + ks.bytes))
@@ -382,7 +400,7 @@ extern "C" int sia_prefill_workspace_size(int64_t batch, int64_t kv_heads, int64
   return SIA_OK;
 }
 
-extern "C" int sia_attention_flash_fwd_workspace_size(const sia_tensor* q, const sia_tensor* k, size_t* bytes) {
+static int fwd_workspace_size(const sia_tensor* q, const sia_tensor* k, int64_t run, size_t* bytes) {
   if (bytes == nullptr || q == nullptr || k == nullptr) return fail(SIA_ERR_INVALID_ARGUMENT, "q, k or bytes is NULL");
   if (q->ndim != 4 || k->ndim != 4) return fail(SIA_ERR_INVALID_ARGUMENT, "q and k must have 4 dims");
   const int64_t B = q->shape[0], Hq = q->shape[1], Tq = q->shape[2], D = q->shape[3];
@@ -394,11 +412,15 @@ extern "C" int sia_attention_flash_fwd_workspace_size(const sia_tensor* q, const
   *bytes = 0;
   if (q->dtype == SIA_F32) return SIA_OK;
   const int64_t images = q->dtype == SIA_F16 && D >= 32 && D <= 128 ? 0 : image_bytes(B, Hkv, Tk, D);
-  const KeySplit ks = key_splits(B, Hq, Hkv, Tq, Tk, D, q->dtype == SIA_BF16, device_info().cus);
+  const KeySplit ks = key_splits(B, Hq, Hkv, Tq, Tk, D, q->dtype == SIA_BF16, device_info().cus, run);
   // (variant 3 reads no V^T images, but the call asks for room for them in any case)
   const int64_t used = (ks.var == 4 ? images : 0) + ks.bytes;
   *bytes = (size_t)(used > images ? used : images);
   return SIA_OK;
+}
+
+extern "C" int sia_attention_flash_fwd_workspace_size(const sia_tensor* q, const sia_tensor* k, size_t* bytes) {
+  return fwd_workspace_size(q, k, INT64_MAX, bytes);
 }
 
 extern "C" int sia_attention_flash_fwd(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, int32_t causal,
@@ -424,6 +446,11 @@ extern "C" int sia_scored_attention_flash_fwd(const sia_tensor* q, const sia_ten
   return flash_fwd(q, k, v, causal, sm_scale, out, workspace, workspace_bytes, stream, nullptr, &in);
 }
 
-extern "C" int sia_scored_attention_flash_fwd_workspace_size(const sia_tensor* q, const sia_tensor* k, size_t* bytes) {
-  return sia_attention_flash_fwd_workspace_size(q, k, bytes);
+extern "C" int sia_scored_attention_flash_fwd_workspace_size(const sia_tensor* q, const sia_tensor* k, int32_t causal,
+                                                             const sia_score_options* score, size_t* bytes) {
+  if (q == nullptr) return fail(SIA_ERR_INVALID_ARGUMENT, "q, k or bytes is NULL");
+  if (q->ndim != 4) return fail(SIA_ERR_INVALID_ARGUMENT, "q and k must have 4 dims");
+  ScoreArgs s;
+  const int rc = fill_score(score, true, q->shape[0], q->shape[1], 1.0f, causal, s);
+  return rc ? rc : fwd_workspace_size(q, k, window_run(s), bytes);
 }

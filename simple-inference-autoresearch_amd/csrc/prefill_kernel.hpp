@@ -531,6 +531,11 @@ void prefill_fwd(const PfArgs<MOD> a) {
     key_lo = min(row_lo(a.s, sb, p0 + q0, dc.g_below), a.Tk) & ~(kPfBN - 1);
     key_lo = max(key_lo, 0);
     Tk = max(0, row_hi(a.s, sb, p0 + g1, dc.g_above) - key_lo);
+    if constexpr (C::split) {                            // (the group's own blocks in nsplit runs)
+      const int run = (fdiv((Tk + kPfBN - 1) / kPfBN + a.nsplit - 1, a.dS)) * kPfBN;
+      key_lo += split * run;
+      Tk = max(0, min(Tk - split * run, run));
+    }
     const int i = min(l32, nw - 1);                      // (a row past Tq is masked as the last one)
     mlo = row_lo(a.s, sb, p0 + w0 + i, dc.lo(p0 + w0, i)) - key_lo;
     mhi = row_hi(a.s, sb, p0 + w0 + i, dc.hi(p0 + w0, i)) - key_lo;
@@ -976,6 +981,11 @@ void prefill_fwd(const PfArgs<MOD> a) {
       constexpr int TQ = (24 + NQK - 1) / NQK, VQ = (48 + NQK - 1) / NQK;
       constexpr int TP = (8 + 2 * ET - 1) / (2 * ET), VP1 = (16 + 2 * ET - 1) / (2 * ET);
       constexpr int VP2 = (24 + 2 * ET - 1) / (2 * ET);
+      // MOD: a cap is 2 transcendentals and 3 instructions a score, a bias 2, a scale 1, of 32 scores per lane; they
+      // spread over all the PV slots
+      constexpr int TS = mod_cap(MOD) ? 64 : 0;
+      constexpr int VS = 32 * ((mod_cap(MOD) ? 3 : kShape ? 1 : 0) + (mod_bias(MOD) ? 2 : 0));
+      constexpr int TPS = (TS + 8 + NPV - 1) / NPV, VPS = (VS + 40 + NPV - 1) / NPV;
       __builtin_amdgcn_sched_group_barrier(0x100, PD, 0);
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
@@ -992,6 +1002,9 @@ void prefill_fwd(const PfArgs<MOD> a) {
         if (i < NQK) {
           __builtin_amdgcn_sched_group_barrier(0x400, TQ, 0);
           __builtin_amdgcn_sched_group_barrier(0x002, VQ, 0);
+        } else if (kShape) {
+          __builtin_amdgcn_sched_group_barrier(0x400, TPS, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, VPS, 0);
         } else if (i < NQK + 2 * ET) {
           __builtin_amdgcn_sched_group_barrier(0x400, TP, 0);
           __builtin_amdgcn_sched_group_barrier(0x002, VP1, 0);
@@ -1292,12 +1305,15 @@ void prefill_fwd(const PfArgs<MOD> a) {
 // heads x 8 runs, 26 MB at head_dim 128: 6.1 us; 4 runs 4.9 us).
 constexpr int kMergeBatch = 8;
 
-template <int D, class T>
-__global__ __launch_bounds__(256) void prefill_merge(const PrefillArgs a) {
+// (MOD: a row that comes out not finite is computed again, as prefill_fwd does)
+template <int D, class T, int MOD = kModNone>
+__global__ __launch_bounds__(256) void prefill_merge(const PfArgs<MOD> a) {
   constexpr int LPR = D / 4, RPB = 256 / LPR;
   const int li = threadIdx.x % LPR;
-  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
-  if (row >= a.nrows) return;
+  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
+  const bool live = row < a.nrows;
+  if constexpr (MOD != kModNone) row = live ? row : a.nrows - 1;      // (the whole wave takes part in a row computed again)
+  else if (!live) return;
   float M = -INFINITY, L = 0.f;
   f32x4 A = {0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < a.nsplit; s0 += kMergeBatch) {
@@ -1331,6 +1347,28 @@ __global__ __launch_bounds__(256) void prefill_merge(const PrefillArgs a) {
   const float inv = L == 0.f ? 0.f : 1.0f / L;
   const int bh = fdiv((int)row, a.dTq), qi = (int)row - bh * a.Tq;
   const int b = fdiv(bh, a.dHq), hq = bh - b * a.Hq;
+  if constexpr (MOD != kModNone) {
+    float t = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t = __builtin_fmaf(A[e] * inv, 0.f, t);
+    const uint64_t bad = __ballot(live && t != t);
+    constexpr uint64_t kRow = LPR == 64 ? ~0ull : (1ull << (LPR & 63)) - 1;
+#pragma unroll 1
+    for (int r = 0; r < 64 / LPR; ++r) {
+      if ((bad >> (r * LPR) & kRow) == 0) continue;
+      const int rb = __builtin_amdgcn_readlane(b, r * LPR), rh = __builtin_amdgcn_readlane(hq, r * LPR);
+      const int ri = __builtin_amdgcn_readlane(qi, r * LPR), p = a.Tk - a.Tq + ri, lane = threadIdx.x & 63;
+      const SeqBounds sb = seq_bounds(a.s, rb, a.Tk);
+      const Documents dc = documents(a.s, rb, p, p, p, lane);
+      scored_row<D, T>(a.s, a.qk_scale, a.s.slopes != nullptr ? a.s.slopes[rh] * kLog2e : 0.f,
+                       a.q + rb * a.q_sb + (int64_t)rh * a.q_sh + (int64_t)ri * a.q_sm,
+                       a.k + rb * a.k_sb + (int64_t)(rh / a.G) * a.k_sh, a.k_sn,
+                       a.v + rb * a.v_sb + (int64_t)(rh / a.G) * a.v_sh, a.v_sn, p, row_lo(a.s, sb, p, dc.g_below),
+                       row_hi(a.s, sb, p, dc.g_above), a.out + rb * a.o_sb + (int64_t)rh * a.o_sh + (int64_t)ri * a.o_sm,
+                       lane);
+    }
+    if (!live || (bad >> ((threadIdx.x & 63) / LPR * LPR) & kRow) != 0) return;
+  }
   *(u32x2*)(a.out + b * a.o_sb + (int64_t)hq * a.o_sh + (int64_t)qi * a.o_sm + 8 * li) =
       u32x2{pack2(T{}, A[0] * inv, A[1] * inv), pack2(T{}, A[2] * inv, A[3] * inv)};
 }

@@ -36,10 +36,13 @@ int launch_prefill(PrefillLaunch& L);
 // Variants 3 and 4: prefill_fwd over runs of key blocks, then prefill_merge (called by launch_prefill).
 int launch_prefill_split(PrefillLaunch& L);
 
-// Scored calls (variants 0-2; called by launch_prefill), compiled by head_dim: prefill_scored.hip and its _d128 and _d256.
+// Scored calls (called by launch_prefill), compiled by head_dim: prefill_scored.hip and its _d128 and _d256; variants 3 and
+// 4 in prefill_scored_split.hip and its _d128.
 int launch_prefill_scored(PrefillLaunch& L);
 int launch_prefill_scored_128(PrefillLaunch& L);
 int launch_prefill_scored_256(PrefillLaunch& L);
+int launch_prefill_scored_split(PrefillLaunch& L);
+int launch_prefill_scored_split_128(PrefillLaunch& L);
 
 // Rotary variant: none, or split-half / interleaved pairs from 16-bit / fp32 tables.
 inline int rope_variant(const PrefillArgs& a) {

@@ -12,9 +12,16 @@ static int launch_scored_mod(PrefillLaunch& L) {
   ScoredPrefillArgs a;
   (PrefillArgs&)a = L.a;
   a.s = L.s;
-  hipLaunchKernelGGL((prefill_fwd<D, T, kRopeNone, VAR, MOD>), dim3(L.a.nqblk * L.a.nunit), dim3(PfCfg<D, VAR>::waves * 64), 0,
-                     L.stream, a);
-  const hipError_t e = hipGetLastError();
+  constexpr bool kSplit = PfCfg<D, VAR>::split;
+  hipLaunchKernelGGL((prefill_fwd<D, T, kRopeNone, VAR, MOD>), dim3(L.a.nqblk * L.a.nunit * (kSplit ? L.a.nsplit : 1)),
+                     dim3(PfCfg<D, VAR>::waves * 64), 0, L.stream, a);
+  hipError_t e = hipGetLastError();
+  if constexpr (kSplit) {
+    if (e != hipSuccess) return fail(SIA_ERR_LAUNCH, "scored prefill launch: %s", hipGetErrorString(e));
+    constexpr int RPB = 256 / (D / 4);
+    hipLaunchKernelGGL((prefill_merge<D, T, kModMask>), dim3((unsigned)((L.a.nrows + RPB - 1) / RPB)), dim3(256), 0, L.stream, a);
+    e = hipGetLastError();
+  }
   return e == hipSuccess ? SIA_OK : fail(SIA_ERR_LAUNCH, "scored prefill launch: %s", hipGetErrorString(e));
 }
 
@@ -36,6 +43,7 @@ static int launch_scored_typed(PrefillLaunch& L) {
     if (L.var == 2) return launch_scored_var<D, T, 2>(L);
   if constexpr (D == 128)
     if (L.var == 1) return launch_scored_var<D, T, 1>(L);
+  if (L.var >= 3) return launch_prefill_scored_split(L);
   if (L.var != 0) return fail(SIA_ERR_LAUNCH, "prefill variant %d is not built for head_dim %d", L.var, D);
   return launch_scored_var<D, T, 0>(L);
 }

@@ -383,7 +383,7 @@ Tensor prefill_scored(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in
   const sia_tensor dout = desc(view, dev, "out");
   const Score sc(softcap, window, slopes, kv_start, dev, kv_len, prefix_len, cu_seqlens);
   size_t ws_bytes = 0;
-  check(sia_scored_attention_flash_fwd_workspace_size(&dq, &dk, &ws_bytes));
+  check(sia_scored_attention_flash_fwd_workspace_size(&dq, &dk, causal ? 1 : 0, &sc.o, &ws_bytes));
   Tensor ws = ws_bytes > 0 ? at::empty({(int64_t)ws_bytes}, q.options().dtype(at::kByte)) : Tensor();
   check(sia_scored_attention_flash_fwd(&dq, &dk, &dv, causal ? 1 : 0, (float)sm_scale, &sc.o, &dout,
                                        ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, stream_of(dev)));

@@ -186,6 +186,41 @@ def test_without_options_it_is_plain_attention(gpu_pkg):
         check(gpu_pkg, q, k, v, f"no option causal={causal}", causal=causal)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,heads,Tq,Tk", [(128, (8, 2), 5, 4100), (128, (32, 8), 200, 6200), (64, (8, 8), 33, 3100),
+                                           (256, (4, 1), 100, 2050)])
+@pytest.mark.parametrize("name", ["cap", "window long", "all", "alibi full", "padded"])
+def test_few_rows_over_many_keys(gpu_pkg, dtype, D, heads, Tq, Tk, name):
+    """Chunks behind a long prefix, whose keys are split over work-groups and merged."""
+    q, k, v = qkv(1, heads, Tq, Tk, D, dtype, seed=10)
+    o = dict(window=2500) if name == "window long" else options(name, 1, heads, Tk)
+    check(gpu_pkg, q, k, v, f"{name} Tq={Tq} Tk={Tk} D={D} {dtype}", **o)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_hidden_keys_of_split_calls(gpu_pkg, dtype, D):
+    """NaN in padding of every run of a split call; an Inf where only some rows see it."""
+    Tq, Tk = 40, 4000
+    q, k, v = qkv(1, (4, 2), Tq, Tk, D, dtype, seed=11)
+    start, length = i32(1010), i32(3990)
+    args = dict(softcap=30.0, kv_start=start, kv_len=length)
+    announce(f"hidden keys of a split call {dtype} D={D}")
+    ref = S.scored_attention(*(t.double().cpu() for t in (q, k, v)), softcap=30.0, start=start, length=length).numpy()
+    atol = tol(v.float(), dtype)
+    for x in (k, v):
+        x[:, :, :1010] = NAN
+        x[:, :, 3990:] = NAN
+    assert_close(gpu_pkg.scored_attention_flash(q, k, v, **args), ref, atol, "spoiled padding")
+    v[:, 0, 3970, 3] = float("inf")               # query 10 on sees it
+    out = gpu_pkg.scored_attention_flash(q, k, v, **args)
+    assert torch.isposinf(out[0, :2, 10:, 3]).all()
+    rest = [d for d in range(D) if d != 3]
+    assert_close(out[..., rest], ref[..., rest], atol, "another dimension")
+    assert_close(out[:, :, :10], ref[:, :, :10], atol, "rows before it")
+    assert_close(out[:, 2:], ref[:, 2:], atol, "other heads")
+
+
 def test_documents_in_any_order_and_per_sequence(gpu_pkg):
     q, k, v = qkv(2, (8, 2), 333, 333, 128, torch.bfloat16, seed=7)
     announce("cu_seqlens in another order, with others among them")

@@ -336,29 +336,30 @@ void attn_f32_prefill(const F32ArgsOf<(SC != 0)> a) {
   if (wave != 0 || (SC == 0 && chunk * kF32TileCols + l32 >= a.ncol)) return;
   add(sm_o[1]);
   const float inv = L == 0.f ? 0.f : 1.0f / L;     // no visible key: zeros (the reference's l_safe guard)
+  uint32_t again = 0u;                             // SC: columns whose weights are finite and whose result is not
   if constexpr (SC != 0) {
     float z = 0.f;
 #pragma unroll
     for (int e = 0; e < ET; ++e)
 #pragma unroll
       for (int j = 0; j < 16; ++j) z = __builtin_fmaf(o[e][j], 0.f, z);
-    if (__any(z != z)) {
+    const uint64_t bad = __ballot(z != z && L == L && chunk * kF32TileCols + l32 < a.ncol);
+    again = (uint32_t)bad | (uint32_t)(bad >> 32);
 #pragma unroll 1
-      for (int r = 0; r < min(kF32TileCols, a.ncol - chunk * kF32TileCols); ++r) {
-        const int cr = chunk * kF32TileCols + r, ir = cr / a.G, hr = hkv * a.G + cr - ir * a.G;
-        const int pr = a.Tk - a.Tq + ir;
-        const SeqBounds sb = seq_bounds(a.s, b, a.Tk);
-        const Documents dc = documents(a.s, b, pr, pr, pr, lane);
-        scored_row<D, F32>(a.s, a.qk_scale, a.s.slopes != nullptr ? a.s.slopes[hr] * kLog2e : 0.f,
-                           a.q + b * a.q_sb + (int64_t)hr * a.q_sh + (int64_t)ir * a.q_sm, a.k + b * a.k_s0 + (int64_t)hkv * a.k_sh,
-                           a.k_sn, a.v + b * a.v_s0 + (int64_t)hkv * a.v_sh, a.v_sn, pr,
-                           row_lo(a.s, sb, pr, dc.g_below), row_hi(a.s, sb, pr, dc.g_above),
-                           a.out + b * a.o_sb + (int64_t)hr * a.o_sh + (int64_t)ir * a.o_sm, lane);
-      }
-      return;
+    for (uint32_t left = again; left != 0u; left &= left - 1u) {
+      const int r = __builtin_ctz(left), cr = chunk * kF32TileCols + r, ir = cr / a.G, hr = hkv * a.G + cr - ir * a.G;
+      const int pr = a.Tk - a.Tq + ir;
+      const SeqBounds sb = seq_bounds(a.s, b, a.Tk);
+      const Documents dc = documents(a.s, b, pr, pr, pr, lane);
+      scored_row<D, F32>(a.s, a.qk_scale, a.s.slopes != nullptr ? a.s.slopes[hr] * kLog2e : 0.f,
+                         a.q + b * a.q_sb + (int64_t)hr * a.q_sh + (int64_t)ir * a.q_sm, a.k + b * a.k_s0 + (int64_t)hkv * a.k_sh,
+                         a.k_sn, a.v + b * a.v_s0 + (int64_t)hkv * a.v_sh, a.v_sn, pr,
+                         row_lo(a.s, sb, pr, dc.g_below), row_hi(a.s, sb, pr, dc.g_above),
+                         a.out + b * a.o_sb + (int64_t)hr * a.o_sh + (int64_t)ir * a.o_sm, lane);
     }
   }
-  if (SC != 0 && chunk * kF32TileCols + l32 >= a.ncol) return;   // (every lane takes part in a row computed again)
+  // (every lane took part in a column computed again)
+  if (SC != 0 && (chunk * kF32TileCols + l32 >= a.ncol || (again >> l32 & 1u))) return;
   int c2 = (int)threadIdx.x & 31;
   asm volatile("" : "+v"(c2));                     // (computed again: held through the loop, they were spilled)
   c2 += chunk * kF32TileCols;

@@ -118,7 +118,8 @@ def build(jobs: int | None = None, verbose: bool = False) -> str:
         raise RuntimeError(f"hipcc not found at {HIPCC}")
     shutil.rmtree(BUILD, ignore_errors=True)
     os.makedirs(BUILD, exist_ok=True)
-    srcs = sources()
+    # the longest units first
+    srcs = sorted(sources(), key=lambda s: not s.startswith(("prefill", "attn_f32", "decode_scored", "decode_d256")))
     jobs = jobs or min(len(srcs), max(1, min(16, os.cpu_count() or 1)))
     objs = []
     failed = []

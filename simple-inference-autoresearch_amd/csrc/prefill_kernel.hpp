@@ -419,9 +419,9 @@ template <int C> constexpr int kPfWpe = PfCfg<C / 8, C % 8>::wpe;
 // of a wave's runs are masked there.  Masks alone cost nothing inside the block
 // loop; a cap or a bias reshapes each score between the QK product and the row
 // max (see `shape`), and the weights are then taken from the shaped scores.
-// A row whose result is not finite is computed again on the vector ALUs
-// (scored_row): a hidden key's NaN or Inf in V turns up in it as weight 0 times
-// that, and so does a bfloat16 V past float16's range.
+// A row whose result is not finite, though its weights are, is computed again
+// on the vector ALUs (scored_row): a hidden key's NaN or Inf in V turns up in it
+// as weight 0 times that, and so does a bfloat16 V past float16's range.
 template <int D, class T, int ROPE, int VAR, int MOD = kModNone>
 __global__ __launch_bounds__(kPfThreads<8 * D + VAR>) __attribute__((amdgpu_waves_per_eu(kPfWpe<8 * D + VAR>)))
 void prefill_fwd(const PfArgs<MOD> a) {
@@ -1254,25 +1254,27 @@ void prefill_fwd(const PfArgs<MOD> a) {
     tile += (wave & 1) * 32 * RB;
     const float lt = half_swap_sum(l);
     const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+    uint32_t again = 0u;                                 // MOD: rows of the wave computed again
     if constexpr (kMod) {
-      // not finite: from what the row sees, or from a hidden key's value times 0
-      float t = 0.f;
+      float t = 0.f;                                     // (0 x Inf and 0 x NaN are NaN, and stay)
 #pragma unroll
       for (int e = 0; e < ET; ++e)
 #pragma unroll
         for (int j = 0; j < 16; ++j) t = __builtin_fmaf(o[e][j], 0.f, t);
-      if (__any(t != t && qi < a.Tq)) {
+      const uint64_t bad = __ballot(t != t && lt == lt && qi < a.Tq);
+      again = (uint32_t)bad | (uint32_t)(bad >> 32);
+      if (again != 0u) {
         const char* kr = a.k + b * a.k_sb + (int64_t)hkv * a.k_sh;
         const char* vr = a.v + b * a.v_sb + (int64_t)hkv * a.v_sh;
         const float sl = a.s.slopes != nullptr ? a.s.slopes[hq] * kLog2e : 0.f;
 #pragma unroll 1
-        for (int r = 0; r < min(32, a.Tq - wrow0); ++r) {
+        for (uint32_t left = again; left != 0u; left &= left - 1u) {
+          const int r = __builtin_ctz(left);
           const int lo = __builtin_amdgcn_readlane(mlo, r) + key_lo, hi = __builtin_amdgcn_readlane(mhi, r) + key_lo;
           scored_row<D, T>(a.s, a.qk_scale, sl, a.q + b * a.q_sb + (int64_t)hq * a.q_sh + (int64_t)(wrow0 + r) * a.q_sm,
                            kr, a.k_sn, vr, a.v_sn, a.Tk - a.Tq + wrow0 + r, lo, hi,
                            a.out + b * a.o_sb + (int64_t)hq * a.o_sh + (int64_t)(wrow0 + r) * a.o_sm, lane);
         }
-        return;
       }
     }
 #pragma unroll
@@ -1292,7 +1294,7 @@ void prefill_fwd(const PfArgs<MOD> a) {
       const int row = i * RPI + lane / NCH;
       const u32x4 w = *(const u32x4*)(tile + row * RB + ((c ^ (row % NCH)) * 16));
       const int qrow = q0 + rg * 32 + row;
-      if (qrow < a.Tq)
+      if (qrow < a.Tq && (!kMod || !(again >> row & 1u)))
         *(u32x4*)(a.out + b * a.o_sb + (int64_t)hq * a.o_sh + (int64_t)qrow * a.o_sm + c * 16) = w;
     }
   }
@@ -1351,7 +1353,7 @@ __global__ __launch_bounds__(256) void prefill_merge(const PfArgs<MOD> a) {
     float t = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) t = __builtin_fmaf(A[e] * inv, 0.f, t);
-    const uint64_t bad = __ballot(live && t != t);
+    const uint64_t bad = __ballot(live && t != t && L == L);
     constexpr uint64_t kRow = LPR == 64 ? ~0ull : (1ull << (LPR & 63)) - 1;
 #pragma unroll 1
     for (int r = 0; r < 64 / LPR; ++r) {

@@ -36,9 +36,10 @@ int launch_prefill(PrefillLaunch& L);
 // Variants 3 and 4: prefill_fwd over runs of key blocks, then prefill_merge (called by launch_prefill).
 int launch_prefill_split(PrefillLaunch& L);
 
-// Scored calls (called by launch_prefill), compiled by head_dim: prefill_scored.hip and its _d128 and _d256; variants 3 and
+// Scored calls (called by launch_prefill), compiled by head_dim: prefill_scored.hip and its _small, _d128 and _d256; variants 3 and
 // 4 in prefill_scored_split.hip and its _d128.
 int launch_prefill_scored(PrefillLaunch& L);
+int launch_prefill_scored_small(PrefillLaunch& L);
 int launch_prefill_scored_128(PrefillLaunch& L);
 int launch_prefill_scored_256(PrefillLaunch& L);
 int launch_prefill_scored_split(PrefillLaunch& L);

@@ -70,15 +70,15 @@ __device__ __forceinline__ float capped_f32(const ScoreArgs& s, float raw) {
   return s.cap_out * (y < 0.0625f ? t : u);
 }
 
-// What one sequence's bounds are made of, clamped to [0, Tk].
+// What one sequence's bounds are made of, clamped to [0, Tk] (so that no sum of them passes 32 bits).
 struct SeqBounds {
   int start, len, prefix;
 };
 __device__ __forceinline__ SeqBounds seq_bounds(const ScoreArgs& s, int b, int Tk) {
   SeqBounds r;
-  r.start = s.start != nullptr ? max(0, s.start[s.start_per_seq ? b : 0]) : 0;
-  r.len = s.len != nullptr ? min(Tk, s.len[s.len_per_seq ? b : 0]) : Tk;
-  r.prefix = s.prefix != nullptr ? s.prefix[s.prefix_per_seq ? b : 0] : 0;
+  r.start = s.start != nullptr ? min(Tk, max(0, s.start[s.start_per_seq ? b : 0])) : 0;
+  r.len = s.len != nullptr ? min(Tk, max(0, s.len[s.len_per_seq ? b : 0])) : Tk;
+  r.prefix = s.prefix != nullptr ? min(Tk, max(0, s.prefix[s.prefix_per_seq ? b : 0])) : 0;
   return r;
 }
 // Bounds of the row at position p inside the document [dlo, dhi).

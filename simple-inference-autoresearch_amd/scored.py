@@ -42,6 +42,12 @@ def _score(softcap, window):
     return float(softcap), int(window)
 
 
+def _in_place(t: torch.Tensor) -> bool:
+    """Whether the decode kernels read a view as it is: head_dim contiguous, rows aligned to 16 bytes."""
+    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+            and all(s * t.element_size() % 16 == 0 for s in t.stride()[:-1]))
+
+
 def is_scored(softcap=None, alibi_slopes=None, window=None, kv_start=None) -> bool:
     """Whether one of a decode call's options is given."""
     return softcap is not None or alibi_slopes is not None or window is not None or kv_start is not None
@@ -79,7 +85,8 @@ def scored_attention_flash(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ca
     cap, win = _score(softcap, window)
     ops = _lib.gpu_ops()
     if (Tq == 1 and k.shape[2] >= 1 and D in _DECODE_DIMS and cu_seqlens is None and kv_len is None and q.is_cuda
-            and k.dtype == q.dtype and v.dtype == q.dtype and (causal or prefix_len is None)):
+            and k.dtype == q.dtype and v.dtype == q.dtype and (causal or prefix_len is None)
+            and all(_in_place(t) for t in (q, k, v))):
         # one query row at the end of the keys: a decode step (a causal row there sees every key, prefix or not)
         n = torch.full((1,), k.shape[2], dtype=torch.int32, device=q.device)
         out = scored_attention_flash_decode(q, k, v, n, sm_scale=sm_scale, softcap=softcap, alibi_slopes=alibi_slopes,

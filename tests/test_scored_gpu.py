@@ -284,6 +284,46 @@ def test_captured_and_replayed(gpu_pkg, dtype):
         assert torch.equal(out, gpu_pkg.scored_attention_flash(q, k, v, **args))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D,Tq,Tk", [(128, 100, 160), (64, 33, 3000), (256, 40, 40)])
+def test_bounds_far_outside(gpu_pkg, dtype, D, Tq, Tk):
+    """First keys, lengths, prefixes and windows at the ends of their types mean none or all."""
+    q, k, v = qkv(1, (4, 2), Tq, Tk, D, dtype, seed=12)
+    lo, hi = -2 ** 31, 2 ** 31 - 1
+    announce(f"bounds far outside {dtype} D={D}")
+    plain = gpu_pkg.scored_attention_flash(q, k, v, softcap=30.0)
+    for same in (dict(kv_start=i32(lo)), dict(kv_len=i32(hi)), dict(prefix_len=i32(lo)), dict(window=hi), dict(window=2 ** 40),
+                 dict(kv_start=i32(lo), kv_len=i32(hi), prefix_len=i32(-1), window=hi, cu_seqlens=i32(lo, hi, 0))):
+        assert torch.equal(gpu_pkg.scored_attention_flash(q, k, v, softcap=30.0, **same), plain), same
+    full = gpu_pkg.scored_attention_flash(q, k, v, causal=False, softcap=30.0)
+    check(gpu_pkg, q, k, v, "a prefix of everything", softcap=30.0, prefix=i32(hi))
+    assert_close(gpu_pkg.scored_attention_flash(q, k, v, softcap=30.0, prefix_len=i32(hi)), full.double().cpu().numpy(),
+                 2 * tol(v.float(), dtype), "prefix of everything, full")
+    for none in (dict(kv_start=i32(hi)), dict(kv_len=i32(lo)), dict(kv_len=i32(0)), dict(kv_start=i32(Tk), prefix_len=i32(hi)),
+                 dict(kv_start=i32(hi), kv_len=i32(lo), window=hi, cu_seqlens=i32(hi, lo))):
+        assert (gpu_pkg.scored_attention_flash(q, k, v, softcap=30.0, **none) == 0).all(), none
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_a_query_that_is_not_finite_stays_alone(gpu_pkg, dtype):
+    q, k, v = qkv(2, (8, 2), 150, 150, 128, dtype, seed=13)
+    announce(f"NaN in q {dtype}")
+    want = gpu_pkg.scored_attention_flash(q, k, v, softcap=30.0, window=60)
+    q[1, 3, 77] = NAN
+    out = gpu_pkg.scored_attention_flash(q, k, v, softcap=30.0, window=60)
+    assert torch.isnan(out[1, 3, 77]).all()
+    out[1, 3, 77] = want[1, 3, 77]
+    assert torch.equal(out, want)
+
+
+def test_single_queries_of_any_view(gpu_pkg):
+    q, k, v = qkv(2, (8, 2), 1, 90, 128, torch.bfloat16, seed=14)
+    odd = torch.zeros(2, 2, 90, 131, dtype=k.dtype, device=DEV)[..., 1:129]
+    odd.copy_(k)
+    announce("a single query over a view whose rows start anywhere")
+    check(gpu_pkg, q, odd, v, "odd rows", softcap=30.0, window=50)
+
+
 def test_refusals(gpu_pkg):
     f = gpu_pkg.scored_attention_flash
     q, k, v = qkv(2, (8, 2), 20, 20, 64, torch.bfloat16)

@@ -828,7 +828,10 @@ void prefill_fwd(const PfArgs<MOD> a) {
     }
   };
   auto masked = [&](int j) { return j >= wfull || (kMod && j < mfront); };   // some row of the wave sees block j not whole
-  // MOD with a cap or a bias: the scores of one block in log2 units
+  // MOD with a cap or a bias: the scores of one block in log2 units.  A cap alone
+  // holds h = -1 / (1 + e^(2 x / c)) instead, of which the capped score is c +
+  // 2 c h: as rising, and the sum is part of the weight's exponent.
+  constexpr bool kCapOnly = mod_cap(MOD) && !mod_bias(MOD);
   float slope2 = 0.f;
   int kp = 0;                                              // position of key 4 h of block 0 less this lane's query's
   if constexpr (mod_bias(MOD)) {
@@ -843,7 +846,8 @@ void prefill_fwd(const PfArgs<MOD> a) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           float x = t ? s1[j] : s0[j];
-          if constexpr (mod_cap(MOD)) x = capped(a.s, x);
+          if constexpr (kCapOnly) x = __builtin_amdgcn_rcpf(-1.0f - fast_exp2(x * a.s.cap_in));
+          else if constexpr (mod_cap(MOD)) x = capped(a.s, x);
           else x *= a.qk_scale;
           if constexpr (mod_bias(MOD)) x = __builtin_fmaf(-slope2, fabsf(d + (float)(32 * t + (j >> 2) * 8 + (j & 3))), x);
           if (t) s1[j] = x;
@@ -852,7 +856,10 @@ void prefill_fwd(const PfArgs<MOD> a) {
     }
   };
   // the weight's exponent from a score as the block loop holds it
-  auto above = [&](float x, float mu) { return kShape ? x - mu : __builtin_fmaf(x, a.qk_scale, -mu); };
+  auto above = [&](float x, float mu) {
+    if constexpr (kCapOnly) return __builtin_fmaf(x, 2.0f * a.s.cap_out, a.s.cap_out - mu);
+    else return kShape ? x - mu : __builtin_fmaf(x, a.qk_scale, -mu);
+  };
   // row max over the 64 keys: a lane-local tree plus the partner half of the wave
   // (a three-input tree, 32 values in 16 v_maximum3; pairs of two-input
   // maxima had compiled to 21, several of them with a repeated operand)
@@ -879,7 +886,9 @@ void prefill_fwd(const PfArgs<MOD> a) {
   // lazy running max: (l, o) are rescaled only when the block max exceeds m by
   // 2^8 (p <= 2^8 otherwise, well inside f16)
   auto raise_max = [&](float rmax) {
-    const float smax = kShape ? rmax : rmax * a.qk_scale;
+    float smax;
+    if constexpr (kCapOnly) smax = __builtin_fmaf(rmax, 2.0f * a.s.cap_out, a.s.cap_out);
+    else smax = kShape ? rmax : rmax * a.qk_scale;
     if (__any(smax > m + 8.0f)) {
       const float m_new = __builtin_elementwise_maximum(m, smax);
       const float alpha = m_new == -INFINITY ? 1.0f : fast_exp2(m - m_new);   // row still sees nothing
@@ -981,11 +990,15 @@ void prefill_fwd(const PfArgs<MOD> a) {
       constexpr int TQ = (24 + NQK - 1) / NQK, VQ = (48 + NQK - 1) / NQK;
       constexpr int TP = (8 + 2 * ET - 1) / (2 * ET), VP1 = (16 + 2 * ET - 1) / (2 * ET);
       constexpr int VP2 = (24 + 2 * ET - 1) / (2 * ET);
-      // MOD: a cap is 2 transcendentals and 3 instructions a score, a bias 2, a scale 1, of 32 scores per lane; they
+      // MOD: a cap is 2 transcendentals and 2 or 3 instructions a score, a bias 2, a scale 1, of 32 scores per lane; they
       // spread over all the PV slots
       constexpr int TS = mod_cap(MOD) ? 64 : 0;
-      constexpr int VS = 32 * ((mod_cap(MOD) ? 3 : kShape ? 1 : 0) + (mod_bias(MOD) ? 2 : 0));
-      constexpr int TPS = (TS + 8 + NPV - 1) / NPV, VPS = (VS + 40 + NPV - 1) / NPV;
+      constexpr int VS = 32 * ((kCapOnly ? 2 : mod_cap(MOD) ? 3 : kShape ? 1 : 0) + (mod_bias(MOD) ? 2 : 0));
+      // (but a cap's at head_dim 64 and below: 4 x 2048 tokens, 32/8 heads, 127 us spread, 118 left to the compiler)
+      constexpr bool kSpread = kShape && (D > 64 || !mod_cap(MOD));
+      // (room above what is needed, so that the row max ends inside the last slots: exact counts 180 us, these 170-175 at
+      // 4 x 2048 tokens capped, 32/8 heads of 128; with twice the room no better)
+      constexpr int TPS = (TS + 24 + NPV - 1) / NPV, VPS = (VS + 80 + NPV - 1) / NPV;
       __builtin_amdgcn_sched_group_barrier(0x100, PD, 0);
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
@@ -1002,7 +1015,7 @@ void prefill_fwd(const PfArgs<MOD> a) {
         if (i < NQK) {
           __builtin_amdgcn_sched_group_barrier(0x400, TQ, 0);
           __builtin_amdgcn_sched_group_barrier(0x002, VQ, 0);
-        } else if (kShape) {
+        } else if (kSpread) {
           __builtin_amdgcn_sched_group_barrier(0x400, TPS, 0);
           __builtin_amdgcn_sched_group_barrier(0x002, VPS, 0);
         } else if (i < NQK + 2 * ET) {

@@ -206,7 +206,7 @@ int64_t window_run(const ScoreArgs& s) {
   return s.causal && s.prefix == nullptr ? (int64_t)s.window + 256 : 2 * (int64_t)s.window + 256;
 }
 
-// Scored attention one row per wave: any type.
+// Scored attention one row per wave (16 bits).
 int scored_rows(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, float sm_scale, const ScoreArgs& s,
                 const sia_tensor* out, void* stream) {
   ScoredRowsArgs a;

@@ -181,10 +181,11 @@ __global__ __launch_bounds__(kRopeThreads) void rope_scaled_kernel(const RopeSca
     const int64_t pi = b * a.p_sb + tt * a.p_st;
     const int64_t n = a.pos64 ? ((const int64_t*)a.pos)[pi] : (int64_t)((const int32_t*)a.pos)[pi];
     double f = (a.freq64 ? ((const double*)a.freq)[pair] : (double)((const float*)a.freq)[pair]) * 0.15915494309189535;
-    f -= floor(f);
-    float2 y = sincos_turn((uint64_t)n * (uint64_t)(f * 18446744073709551616.0));
-    y.x *= a.scale;
-    y.y *= a.scale;
+    f -= floor(f);                                   // (a negative f next to 0 may round up to 1: a whole turn, 0)
+    float2 y = sincos_turn((uint64_t)n * (f < 1.0 ? (uint64_t)(f * 18446744073709551616.0) : 0u));
+    const float scale = f <= 1.0 ? a.scale : NAN;    // (a frequency that is not finite has no angle)
+    y.x *= scale;
+    y.y *= scale;
     sc[i] = y;
   }
   __syncthreads();

@@ -1,4 +1,5 @@
-// Scored attention one query row per wave (score.hpp), for every type and head_dim.
+// Scored attention of 16-bit prompts one query row per wave (score.hpp): the calls whose cap is too large for the matrix
+// kernels' form of it.  K and V are read once per row, from the caches.
 #include "host_util.hpp"
 #include "scored.hpp"
 
@@ -42,11 +43,7 @@ int launch_scored_rows(const ScoredRowsArgs& a, int D, int dtype, hipStream_t st
   const int64_t groups = (a.rows + 3) / 4;
   if (groups > 0x7fffffff) return fail(SIA_ERR_UNSUPPORTED, "too many query rows");
   const dim3 grid((unsigned)groups);
-  switch (dtype) {
-    case SIA_F16: return launch_rows_t<F16>(a, D, grid, stream);
-    case SIA_BF16: return launch_rows_t<BF16>(a, D, grid, stream);
-    default: return launch_rows_t<F32>(a, D, grid, stream);
-  }
+  return dtype == SIA_F16 ? launch_rows_t<F16>(a, D, grid, stream) : launch_rows_t<BF16>(a, D, grid, stream);
 }
 
 }  // namespace sia

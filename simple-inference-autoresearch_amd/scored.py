@@ -27,14 +27,15 @@ from .decode import _HEAD_DIMS, _common, _kv_len_tensor, _options
 from . import decode as _decode
 
 _DECODE_DIMS = (64, 128, 256)   # head dims of the matrix decode kernels (single-query calls)
+_CAP_RANGE = (1e-37, 1e37)      # with room for its products in float32
 
 
 def _score(softcap, window):
     """(softcap, window) as the extension takes them, 0 for none."""
     if softcap is None:
         softcap = 0.0
-    elif not 0.0 < softcap < float("inf"):
-        raise ValueError("softcap must be a positive finite number")
+    elif not _CAP_RANGE[0] <= softcap <= _CAP_RANGE[1]:
+        raise ValueError("softcap must be a positive finite number (1e-37 to 1e37)")
     if window is None:
         window = 0
     elif window < 1:

@@ -137,6 +137,23 @@ def test_scaled_contexts(gpu_pkg, kind):
         assert r.scale > 1 and torch.equal(r.inv_freq[:8], base[:8]) and torch.allclose(r.inv_freq[-4:], base[-4:] / 8)
 
 
+def test_frequencies_of_any_value(gpu_pkg):
+    """Negative ones turn backwards, ones next to zero not at all, and one without a value reaches its own pair alone."""
+    q, pos = torch.randn(1, 9, 2, 64, device=DEV), torch.arange(9, device=DEV) * 1000
+    announce("negative, vanishing and missing frequencies")
+    for f in (-freqs(64), torch.full((32,), -1e-20, dtype=torch.float64), torch.zeros(32, dtype=torch.float64)):
+        out, _ = gpu_pkg.rope_scaled(q, None, pos, f.to(DEV))
+        check(out, q, pos, f, 64, False, 1.0, "negative frequencies")
+    want, _ = gpu_pkg.rope_scaled(q, None, pos, freqs(64).to(DEV))
+    for bad in (float("nan"), float("inf")):
+        f = freqs(64)
+        f[5] = bad
+        out, _ = gpu_pkg.rope_scaled(q, None, pos, f.to(DEV))
+        assert torch.isnan(out[..., [5, 37]]).all()
+        out[..., [5, 37]] = want[..., [5, 37]]
+        assert torch.equal(out, want)
+
+
 def test_refusals(gpu_pkg):
     q, k = torch.randn(2, 5, 4, 64, device=DEV), torch.randn(2, 5, 2, 64, device=DEV)
     pos, f = torch.arange(5, device=DEV), freqs(64).to(DEV)

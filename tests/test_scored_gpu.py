@@ -316,6 +316,17 @@ def test_a_query_that_is_not_finite_stays_alone(gpu_pkg, dtype):
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("cap", [1e-30, 1e30])
+def test_caps_without_measure(gpu_pkg, cap):
+    """A cap far below every score leaves equal weights, one far above every score leaves the scores."""
+    q, k, v = qkv(1, (4, 2), 70, 70, 64, torch.bfloat16, seed=15)
+    announce(f"cap {cap}")
+    check(gpu_pkg, q, k, v, f"cap {cap}", softcap=cap)
+    for none in (1e-50, 1e39):                       # no float32 holds them
+        with pytest.raises(ValueError):
+            gpu_pkg.scored_attention_flash(q, k, v, softcap=none)
+
+
 def test_single_queries_of_any_view(gpu_pkg):
     q, k, v = qkv(2, (8, 2), 1, 90, 128, torch.bfloat16, seed=14)
     odd = torch.zeros(2, 2, 90, 131, dtype=k.dtype, device=DEV)[..., 1:129]

@@ -263,7 +263,9 @@ int flash_fwd(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, int
     if ((rc = device_ok())) return rc;
     if (Tq == 0) return SIA_OK;
     if (q->dtype == SIA_F32) return prefill_f32(q, k, v, causal, sm_scale, out, stream, &sc);
-    if (sc.cap_out > kMaxFastCap * kLog2e) return scored_rows(q, k, v, sm_scale, sc, out, stream);
+    const float unit = sc.cap_out > 0.f ? sc.cap_out : sm_scale;
+    if (sc.cap_out > kMaxFastCap * kLog2e || (sc.slopes != nullptr && unit < kMinFastUnit))
+      return scored_rows(q, k, v, sm_scale, sc, out, stream);
   }
   if (q->dtype == SIA_F32) {
     if (rope != nullptr)

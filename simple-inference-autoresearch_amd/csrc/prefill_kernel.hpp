@@ -828,14 +828,17 @@ void prefill_fwd(const PfArgs<MOD> a) {
     }
   };
   auto masked = [&](int j) { return j >= wfull || (kMod && j < mfront); };   // some row of the wave sees block j not whole
-  // MOD with a cap or a bias: the scores of one block in log2 units.  A cap alone
-  // holds h = -1 / (1 + e^(2 x / c)) instead, of which the capped score is c +
-  // 2 c h: as rising, and the sum is part of the weight's exponent.
-  constexpr bool kCapOnly = mod_cap(MOD) && !mod_bias(MOD);
-  float slope2 = 0.f;
+  // MOD with a cap or a bias: each score becomes a y of which up y + base is the
+  // shaped score in log2 units, as the row max and the weights' exponents take
+  // it in one FMA.  A cap makes of it h = -1 / (1 + e^(2 x / c)), with up = 2 c and
+  // base = c (capped); a bias adds -slope / up times the distance.
+  constexpr bool kCap = mod_cap(MOD), kBias = mod_bias(MOD);
+  const float up = [&] { if constexpr (kCap) return 2.0f * a.s.cap_out; else return a.qk_scale; }();
+  const float base = [&] { if constexpr (kCap) return a.s.cap_out; else return 0.f; }();
+  float slope_up = 0.f;
   int kp = 0;                                              // position of key 4 h of block 0 less this lane's query's
-  if constexpr (mod_bias(MOD)) {
-    slope2 = a.s.slopes[hq] * kLog2e;
+  if constexpr (kBias) {
+    slope_up = a.s.slopes[hq] * kLog2e / up;
     kp = key_lo + 4 * h - (a.Tk - a.Tq + qi);
   }
   auto shape = [&](f32x16& s0, f32x16& s1, int key0) {
@@ -846,20 +849,15 @@ void prefill_fwd(const PfArgs<MOD> a) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           float x = t ? s1[j] : s0[j];
-          if constexpr (kCapOnly) x = __builtin_amdgcn_rcpf(-1.0f - fast_exp2(x * a.s.cap_in));
-          else if constexpr (mod_cap(MOD)) x = capped(a.s, x);
-          else x *= a.qk_scale;
-          if constexpr (mod_bias(MOD)) x = __builtin_fmaf(-slope2, fabsf(d + (float)(32 * t + (j >> 2) * 8 + (j & 3))), x);
+          if constexpr (kCap) x = __builtin_amdgcn_rcpf(-1.0f - fast_exp2(x * a.s.cap_in));
+          if constexpr (kBias) x = __builtin_fmaf(-slope_up, fabsf(d + (float)(32 * t + (j >> 2) * 8 + (j & 3))), x);
           if (t) s1[j] = x;
           else s0[j] = x;
         }
     }
   };
-  // the weight's exponent from a score as the block loop holds it
-  auto above = [&](float x, float mu) {
-    if constexpr (kCapOnly) return __builtin_fmaf(x, 2.0f * a.s.cap_out, a.s.cap_out - mu);
-    else return kShape ? x - mu : __builtin_fmaf(x, a.qk_scale, -mu);
-  };
+  // the weight's exponent
+  auto above = [&](float x, float mu) { return __builtin_fmaf(x, up, kCap ? base - mu : -mu); };
   // row max over the 64 keys: a lane-local tree plus the partner half of the wave
   // (a three-input tree, 32 values in 16 v_maximum3; pairs of two-input
   // maxima had compiled to 21, several of them with a repeated operand)
@@ -886,9 +884,7 @@ void prefill_fwd(const PfArgs<MOD> a) {
   // lazy running max: (l, o) are rescaled only when the block max exceeds m by
   // 2^8 (p <= 2^8 otherwise, well inside f16)
   auto raise_max = [&](float rmax) {
-    float smax;
-    if constexpr (kCapOnly) smax = __builtin_fmaf(rmax, 2.0f * a.s.cap_out, a.s.cap_out);
-    else smax = kShape ? rmax : rmax * a.qk_scale;
+    const float smax = kCap ? __builtin_fmaf(rmax, up, base) : rmax * up;
     if (__any(smax > m + 8.0f)) {
       const float m_new = __builtin_elementwise_maximum(m, smax);
       const float alpha = m_new == -INFINITY ? 1.0f : fast_exp2(m - m_new);   // row still sees nothing
@@ -990,12 +986,11 @@ void prefill_fwd(const PfArgs<MOD> a) {
       constexpr int TQ = (24 + NQK - 1) / NQK, VQ = (48 + NQK - 1) / NQK;
       constexpr int TP = (8 + 2 * ET - 1) / (2 * ET), VP1 = (16 + 2 * ET - 1) / (2 * ET);
       constexpr int VP2 = (24 + 2 * ET - 1) / (2 * ET);
-      // MOD: a cap is 2 transcendentals and 2 or 3 instructions a score, a bias 2, a scale 1, of 32 scores per lane; they
-      // spread over all the PV slots
-      constexpr int TS = mod_cap(MOD) ? 64 : 0;
-      constexpr int VS = 32 * ((kCapOnly ? 2 : mod_cap(MOD) ? 3 : kShape ? 1 : 0) + (mod_bias(MOD) ? 2 : 0));
+      // MOD: a cap is 2 transcendentals and 2 instructions a score, a bias 2, of 32 scores per lane; they spread over all
+      // the PV slots
+      constexpr int TS = kCap ? 64 : 0, VS = (kCap ? 64 : 0) + (kBias ? 64 : 0);
       // (but a cap's at head_dim 64 and below: 4 x 2048 tokens, 32/8 heads, 127 us spread, 118 left to the compiler)
-      constexpr bool kSpread = kShape && (D > 64 || !mod_cap(MOD));
+      constexpr bool kSpread = kShape && (D > 64 || !kCap);
       // (room above what is needed, so that the row max ends inside the last slots: exact counts 180 us, these 170-175 at
       // 4 x 2048 tokens capped, 32/8 heads of 128; with twice the room no better)
       constexpr int TPS = (TS + 24 + NPV - 1) / NPV, VPS = (VS + 80 + NPV - 1) / NPV;

@@ -44,15 +44,13 @@ constexpr float kLog2e = 1.4426950408889634f;
 // The largest cap of the matrix kernels: their `capped` is off by 2^-22 of it, at 512 as much as the weights' rounding to
 // fp16 (2^-11 half a step; 512 2^-22 log2(e) = 2^-12.5).  Larger ones go to the vector kernels.
 constexpr float kMaxFastCap = 512.0f;
+// The prompts' matrix kernels take slopes in units of the cap or of the scale; below this the products could pass fp32's
+// range, and the vector kernels take the call.
+constexpr float kMinFastUnit = 1e-20f;
 
-// c tanh(x / c) in log2 units from the raw product, as c (1 - 2 / (1 + e^(2 x / c))): two transcendentals and three
+// c tanh(x / c) in log2 units from a score x in log2 units, as c (1 - 2 / (1 + e^(2 x / c))): two transcendentals and three
 // instructions.  Off by at most about 3 ulp of c, 2^-22 c: below every rounding of 16-bit inputs and weights (c = 50: 2e-5
-// of a weight).  float32 calls use capped_f32.
-__device__ __forceinline__ float capped(const ScoreArgs& s, float raw) {
-  const float e = fast_exp2(raw * s.cap_in);
-  return __builtin_fmaf(__builtin_amdgcn_rcpf(1.0f + e), -2.0f * s.cap_out, s.cap_out);
-}
-// The same from a score in log2 units.
+// of a weight).  The prompts' kernels take the same formula apart (`shape` in prefill_fwd); float32 calls use capped_f32.
 __device__ __forceinline__ float capped_log2(const ScoreArgs& s, float x) {
   const float e = fast_exp2(x * s.cap_log2);
   return __builtin_fmaf(__builtin_amdgcn_rcpf(1.0f + e), -2.0f * s.cap_out, s.cap_out);

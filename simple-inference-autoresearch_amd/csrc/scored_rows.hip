@@ -1,5 +1,5 @@
-// Scored attention of 16-bit prompts one query row per wave (score.hpp): the calls whose cap is too large for the matrix
-// kernels' form of it.  K and V are read once per row, from the caches.
+// Scored attention of 16-bit prompts one query row per wave (score.hpp): the calls whose cap, or whose scale beside
+// slopes, is out of the matrix kernels' range.  K and V are read once per row, from the caches.
 #include "host_util.hpp"
 #include "scored.hpp"
 

@@ -327,6 +327,17 @@ def test_caps_without_measure(gpu_pkg, cap):
             gpu_pkg.scored_attention_flash(q, k, v, softcap=none)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("scale,cap", [(1e-30, None), (0.1, 1e-30), (1e-30, 20.0)])
+def test_slopes_beside_a_vanishing_unit(gpu_pkg, D, scale, cap):
+    """Scores or a cap next to 0 leave the bias alone, however far the keys."""
+    q, k, v = qkv(1, (4, 2), 300, 300, D, torch.bfloat16, seed=16)
+    announce(f"scale {scale} cap {cap}")
+    out = gpu_pkg.scored_attention_flash(q, k, v, sm_scale=scale, softcap=cap, alibi_slopes=slopes_of(4))
+    ref = S.scored_attention(*(t.double().cpu() for t in (q, k, v)), sm_scale=scale, softcap=cap, slopes=slopes_of(4).cpu())
+    assert_close(out, ref.numpy(), tol(v.float(), q.dtype), f"scale {scale} cap {cap}")
+
+
 def test_single_queries_of_any_view(gpu_pkg):
     q, k, v = qkv(2, (8, 2), 1, 90, 128, torch.bfloat16, seed=14)
     odd = torch.zeros(2, 2, 90, 131, dtype=k.dtype, device=DEV)[..., 1:129]

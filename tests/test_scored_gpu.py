@@ -35,6 +35,10 @@ def i32(*x):
     return torch.tensor(x, dtype=torch.int32, device=DEV)
 
 
+def i32cpu(*x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
 def slopes_of(n):
     return torch.tensor([2.0 ** (-8.0 * (h + 1) / n) for h in range(n)], device=DEV)
 
@@ -325,6 +329,32 @@ def test_caps_without_measure(gpu_pkg, cap):
     for none in (1e-50, 1e39):                       # no float32 holds them
         with pytest.raises(ValueError):
             gpu_pkg.scored_attention_flash(q, k, v, softcap=none)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("heads", [(4, 1), (2, 2)])
+@pytest.mark.parametrize("kw", [dict(), dict(causal=False), dict(softcap=30.0, window=700), dict(prefix=i32cpu(650)),
+                                dict(cuts=[0, 33, 640, 1000]), dict(start=i32cpu(0, 950), length=i32cpu(560, 1055))],
+                         ids=["causal", "full", "window", "prefix", "documents", "padding"])
+def test_biases_over_many_blocks(gpu_pkg, dtype, D, heads, kw):
+    """Slopes that raise the scores towards the last block, or (negative) towards the first, whoever sees it."""
+    q, k, v = qkv(2, heads, 1055, 1055, D, dtype, seed=17)
+    kw = {n: x.to(DEV) if isinstance(x, torch.Tensor) else x for n, x in kw.items()}
+    slopes = torch.tensor([0.7, -0.02, 0.004, -0.3][:heads[0]], device=DEV)
+    check(gpu_pkg, q, k, v, f"many blocks {dtype} {D} {heads} {list(kw)}", slopes=slopes, **kw)
+
+
+def test_biases_of_a_large_call(gpu_pkg):
+    q, k, v = qkv(8, (4, 1), 2100, 2100, 128, torch.bfloat16, seed=18)
+    slopes = torch.tensor([0.7, 0.1, 0.004, -0.01], device=DEV)
+    k[:, :, :3], v[:, :, :3] = NAN, NAN
+    announce("2100 tokens in 8 rows, biased")
+    out = gpu_pkg.scored_attention_flash(q, k, v, alibi_slopes=slopes, kv_start=i32(3))
+    for b in (0, 7):
+        ref = S.scored_attention(*(t[b:b + 1].double().cpu() for t in (q, torch.nan_to_num(k), torch.nan_to_num(v))),
+                                 slopes=slopes.cpu(), start=torch.tensor([3]))
+        assert_close(out[b:b + 1], ref.numpy(), tol(v.float(), q.dtype), f"row {b}")
 
 
 @pytest.mark.parametrize("D", [64, 128])

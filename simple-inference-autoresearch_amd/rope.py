@@ -159,8 +159,10 @@ class ScaledRope:
     * ``"ntk"``: ``theta`` times ``factor^(R / (R - 2))``;
     * ``"yarn"``: ``f_i`` for pairs that turn more than ``beta_fast`` times in
       ``original_max_seq_len`` positions, ``f_i / factor`` below ``beta_slow``
-      turns, a linear blend over the pairs between; rotated elements are
-      multiplied by ``attention_factor`` (default ``0.1 ln(factor) + 1``);
+      turns, a linear blend over the pairs between (its ends are
+      rounded outwards, to at least 0 and at most ``R - 1``, past the last
+      pair); rotated elements are multiplied by ``attention_factor`` (default
+      ``0.1 ln(factor) + 1``);
     * ``"llama3"``: :class:`RopeFrequencies`' rule.
 
     ``inv_freq`` is kept in float64 on ``device``.  Call the object with ``q``,
@@ -192,7 +194,7 @@ class ScaledRope:
         elif rope_type == "yarn":
             low, high = (R * math.log(original_max_seq_len / (turns * 2 * math.pi)) / (2 * math.log(theta))
                          for turns in (beta_fast, beta_slow))
-            low, high = max(math.floor(low), 0), min(math.ceil(high), R // 2 - 1)
+            low, high = max(math.floor(low), 0), min(math.ceil(high), R - 1)   # (past the last pair: it is blended too)
             ramp = ((i - low) / max(high - low, 0.001)).clamp(0, 1)
             freq = freq / factor * ramp + freq * (1 - ramp)
             self.scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0

@@ -421,7 +421,8 @@ template <int C> constexpr int kPfWpe = PfCfg<C / 8, C % 8>::wpe;
 // max (see `shape`), and the weights are then taken from the shaped scores.
 // A row whose result is not finite, though its weights are, is computed again
 // on the vector ALUs (scored_row): a hidden key's NaN or Inf in V turns up in it
-// as weight 0 times that, and so does a bfloat16 V past float16's range.
+// as weight 0 times that, and so does a bfloat16 V past float16's range.  So is a
+// row of bfloat16 values that all lie below what float16 holds well (SmallValues).
 template <int D, class T, int ROPE, int VAR, int MOD = kModNone>
 __global__ __launch_bounds__(kPfThreads<8 * D + VAR>) __attribute__((amdgpu_waves_per_eu(kPfWpe<8 * D + VAR>)))
 void prefill_fwd(const PfArgs<MOD> a) {
@@ -1298,9 +1299,24 @@ void prefill_fwd(const PfArgs<MOD> a) {
         for (int j = 0; j < 16; ++j) t = __builtin_fmaf(o[e][j], 0.f, t);
       const uint64_t bad = __ballot(t != t && lt == lt && qi < a.Tq);
       again = (uint32_t)bad | (uint32_t)(bad >> 32);
+      const char* vr = a.v + b * a.v_sb + (int64_t)hkv * a.v_sh;
+      if constexpr (std::is_same<T, BF16>::value) {
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < ET; ++e)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(o[e][j]));
+        SmallValues sv;
+        uint32_t left = (uint32_t)__ballot(half_swap_max(top) * inv < kSmallV && lt > 0.f && qi < a.Tq);   // (both halves alike)
+#pragma unroll 1
+        for (; left != 0u; left &= left - 1u) {
+          const int r = __builtin_ctz(left);
+          const int lo = __builtin_amdgcn_readlane(mlo, r) + key_lo, hi = __builtin_amdgcn_readlane(mhi, r) + key_lo;
+          if (sv.lost<D>(vr, a.v_sn, lo, hi, lane)) again |= left & -left;
+        }
+      }
       if (again != 0u) {
         const char* kr = a.k + b * a.k_sb + (int64_t)hkv * a.k_sh;
-        const char* vr = a.v + b * a.v_sb + (int64_t)hkv * a.v_sh;
         const float sl = a.s.slopes != nullptr ? a.s.slopes[hq] * kLog2e : 0.f;
 #pragma unroll 1
         for (uint32_t left = again; left != 0u; left &= left - 1u) {
@@ -1342,7 +1358,7 @@ void prefill_fwd(const PfArgs<MOD> a) {
 // heads x 8 runs, 26 MB at head_dim 128: 6.1 us; 4 runs 4.9 us).
 constexpr int kMergeBatch = 8;
 
-// (MOD: a row that comes out not finite is computed again, as prefill_fwd does)
+// (MOD: a row that comes out not finite, or of bfloat16 values that fp16 does not hold, is computed again, as in prefill_fwd)
 template <int D, class T, int MOD = kModNone>
 __global__ __launch_bounds__(256) void prefill_merge(const PfArgs<MOD> a) {
   constexpr int LPR = D / 4, RPB = 256 / LPR;
@@ -1388,21 +1404,30 @@ __global__ __launch_bounds__(256) void prefill_merge(const PfArgs<MOD> a) {
     float t = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) t = __builtin_fmaf(A[e] * inv, 0.f, t);
-    const uint64_t bad = __ballot(live && t != t && L == L);
+    uint64_t bad = __ballot(live && t != t && L == L);
     constexpr uint64_t kRow = LPR == 64 ? ~0ull : (1ull << (LPR & 63)) - 1;
+    uint64_t ample = ~0ull;                              // lanes whose results are not small (SmallValues)
+    if constexpr (std::is_same<T, BF16>::value)
+      ample = __ballot(!(live && L > 0.f && fmaxf(fmaxf(fabsf(A[0]), fabsf(A[1])), fmaxf(fabsf(A[2]), fabsf(A[3]))) * inv < kSmallV));
 #pragma unroll 1
     for (int r = 0; r < 64 / LPR; ++r) {
-      if ((bad >> (r * LPR) & kRow) == 0) continue;
+      const bool spoiled = (bad >> (r * LPR) & kRow) != 0, small = (ample >> (r * LPR) & kRow) == 0;
+      if (!spoiled && !small) continue;
       const int rb = __builtin_amdgcn_readlane(b, r * LPR), rh = __builtin_amdgcn_readlane(hq, r * LPR);
       const int ri = __builtin_amdgcn_readlane(qi, r * LPR), p = a.Tk - a.Tq + ri, lane = threadIdx.x & 63;
       const SeqBounds sb = seq_bounds(a.s, rb, a.Tk);
       const Documents dc = documents(a.s, rb, p, p, p, lane);
+      const char* vr = a.v + rb * a.v_sb + (int64_t)(rh / a.G) * a.v_sh;
+      const int lo = row_lo(a.s, sb, p, dc.g_below), hi = row_hi(a.s, sb, p, dc.g_above);
+      if (!spoiled) {
+        SmallValues sv;
+        if (!sv.lost<D>(vr, a.v_sn, lo, hi, lane)) continue;
+        bad |= kRow << (r * LPR);
+      }
       scored_row<D, T>(a.s, a.qk_scale, a.s.slopes != nullptr ? a.s.slopes[rh] * kLog2e : 0.f,
                        a.q + rb * a.q_sb + (int64_t)rh * a.q_sh + (int64_t)ri * a.q_sm,
-                       a.k + rb * a.k_sb + (int64_t)(rh / a.G) * a.k_sh, a.k_sn,
-                       a.v + rb * a.v_sb + (int64_t)(rh / a.G) * a.v_sh, a.v_sn, p, row_lo(a.s, sb, p, dc.g_below),
-                       row_hi(a.s, sb, p, dc.g_above), a.out + rb * a.o_sb + (int64_t)rh * a.o_sh + (int64_t)ri * a.o_sm,
-                       lane);
+                       a.k + rb * a.k_sb + (int64_t)(rh / a.G) * a.k_sh, a.k_sn, vr, a.v_sn, p, lo, hi,
+                       a.out + rb * a.o_sb + (int64_t)rh * a.o_sh + (int64_t)ri * a.o_sm, lane);
     }
     if (!live || (bad >> ((threadIdx.x & 63) / LPR * LPR) & kRow) != 0) return;
   }

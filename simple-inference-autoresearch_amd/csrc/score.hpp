@@ -164,6 +164,49 @@ __device__ __forceinline__ float elem_at(const char* p) {
   else return to_f32(T{}, *(const uint16_t*)p);
 }
 
+// What fp16 makes of a bfloat16 V.  The prompts' kernels take V to fp16 for P V: exact from 2^-17 on, off by at most 2^-25 of
+// a smaller value, so by as much of the result (the weights add up to 1).  Beside a value of 2^-13 or more that is under 2^-12
+// of the largest one a row sees; a row that sees none, and some that are rounded, is computed again in fp32 (scored_row).
+// Only rows whose results all lie below 2^-13 can be such, and only for those is V read again.
+constexpr float kSmallV = 0x1p-13f;
+// Keys of one KV head as a wave's rows see them, in rising order of their runs: scanned up to `done` as far as the rows need
+// it, the last key found with a value that fp16 rounds, and the last one with a value of kSmallV or more.
+// 4 x 2048 tokens, 32/8 heads of 128, capped: us 173, 395 over values that are all zero (V read once per wave), 17400 over
+// values of 1e-6 (every row computed again).
+struct SmallValues {
+  int done = 0, rounded = -1, ample = -1;
+  // Whether the row of keys [lo, hi) is to be computed again.  (Every lane active, every argument uniform; 16 bytes of a
+  // key's row per lane.)
+  template <int D>
+  __device__ __forceinline__ bool lost(const char* v, int64_t v_sn, int lo, int hi, int lane) {
+    constexpr int LPK = D / 8, KPL = 64 / LPK, U = 4;
+    asm volatile("" : "+v"(lane));   // (its row and piece computed here: held through the block loop, they cost a wave per SIMD)
+    done = max(lo, done);
+#pragma unroll 1
+    while (ample < lo && done < hi) {
+      u32x4 w[U];
+      int key[U], r = -1, m = -1;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        key[u] = min(done + u * KPL + lane / LPK, hi - 1);
+        w[u] = *(const u32x4*)(v + (int64_t)key[u] * v_sn + 16 * (lane % LPK));
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t x = (w[u][i >> 1] >> (16 * (i & 1))) & 0x7fffu;   // |value|: 0x3700 is 2^-17, 0x3900 2^-13
+          if (x - 1u < 0x3700u - 1u) r = key[u];
+          if (x >= 0x3900u) m = key[u];
+        }
+      if (__any(r >= 0)) rounded = uniform(wave_max_i(r));
+      if (__any(m >= 0)) ample = uniform(wave_max_i(m));
+      done = min(hi, done + U * KPL);
+    }
+    return rounded >= lo && ample < lo;
+  }
+};
+
 template <int D, class T>
 __device__ __forceinline__ void scored_row(const ScoreArgs& s, float qk_scale, float slope2, const char* q, const char* k,
                                            int64_t k_sn, const char* v, int64_t v_sn, int p, int lo, int hi, char* out,

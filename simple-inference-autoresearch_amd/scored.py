@@ -27,6 +27,7 @@ from .decode import _HEAD_DIMS, _common, _kv_len_tensor, _options
 from . import decode as _decode
 
 _DECODE_DIMS = (64, 128, 256)   # head dims of the matrix decode kernels (single-query calls)
+_DECODE_BATCH = 16384           # most sequences of a decode call
 _CAP_RANGE = (1e-37, 1e37)      # with room for its products in float32
 
 
@@ -44,9 +45,19 @@ def _score(softcap, window):
 
 
 def _in_place(t: torch.Tensor) -> bool:
-    """Whether the decode kernels read a view as it is: head_dim contiguous, rows aligned to 16 bytes."""
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and all(s * t.element_size() % 16 == 0 for s in t.stride()[:-1]))
+    """Whether the decode kernels read a view as it is: head_dim contiguous, rows aligned to 16 bytes, tokens within 2 GiB."""
+    es = t.element_size()
+    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * es % 16 == 0 for s in t.stride()[:-1])
+            and t.stride(-2) * es < 1 << 31)
+
+
+def _is_step(q, k, v, causal, cu_seqlens, prefix_len, kv_len) -> bool:
+    """Whether a prompt call is a decode step that :func:`scored_attention_flash_decode` takes: one query row at the end
+    of the keys (a causal row there sees every key, prefix or not).  What that refuses goes to the prompts' kernels."""
+    B, _, Tq, D = q.shape
+    return (Tq == 1 and k.shape[2] >= 1 and D in _DECODE_DIMS and B <= _DECODE_BATCH and cu_seqlens is None and kv_len is None and q.is_cuda and k.dtype == q.dtype and v.dtype == q.dtype
+            and (causal or prefix_len is None)
+            and all(_in_place(t) for t in (q, k, v)))
 
 
 def is_scored(softcap=None, alibi_slopes=None, window=None, kv_start=None) -> bool:
@@ -85,10 +96,7 @@ def scored_attention_flash(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ca
         sm_scale = 1.0 / (D ** 0.5)
     cap, win = _score(softcap, window)
     ops = _lib.gpu_ops()
-    if (Tq == 1 and k.shape[2] >= 1 and D in _DECODE_DIMS and cu_seqlens is None and kv_len is None and q.is_cuda
-            and k.dtype == q.dtype and v.dtype == q.dtype and (causal or prefix_len is None)
-            and all(_in_place(t) for t in (q, k, v))):
-        # one query row at the end of the keys: a decode step (a causal row there sees every key, prefix or not)
+    if _is_step(q, k, v, causal, cu_seqlens, prefix_len, kv_len):
         n = torch.full((1,), k.shape[2], dtype=torch.int32, device=q.device)
         out = scored_attention_flash_decode(q, k, v, n, sm_scale=sm_scale, softcap=softcap, alibi_slopes=alibi_slopes,
                                             window=window, kv_start=kv_start)

@@ -51,12 +51,19 @@ def _in_place(t: torch.Tensor) -> bool:
             and t.stride(-2) * es < 1 << 31)
 
 
+def _per_sequence(t: torch.Tensor, q: torch.Tensor) -> bool:
+    """Whether the prompts' kernels take ``t`` as an option with an entry for all sequences or for each."""
+    return (t.dtype == torch.int32 and t.device == q.device and t.dim() <= 1
+            and (t.numel() == 1 or (t.numel() == q.shape[0] and t.stride(0) == 1)))
+
+
 def _is_step(q, k, v, causal, cu_seqlens, prefix_len, kv_len) -> bool:
     """Whether a prompt call is a decode step that :func:`scored_attention_flash_decode` takes: one query row at the end
     of the keys (a causal row there sees every key, prefix or not).  What that refuses goes to the prompts' kernels."""
     B, _, Tq, D = q.shape
-    return (Tq == 1 and k.shape[2] >= 1 and D in _DECODE_DIMS and B <= _DECODE_BATCH and cu_seqlens is None and kv_len is None and q.is_cuda and k.dtype == q.dtype and v.dtype == q.dtype
-            and (causal or prefix_len is None)
+    return (Tq == 1 and k.shape[2] >= 1 and D in _DECODE_DIMS and B <= _DECODE_BATCH and k.shape[0] == B
+            and cu_seqlens is None and kv_len is None and q.is_cuda and k.dtype == q.dtype and v.dtype == q.dtype
+            and (prefix_len is None or (causal and _per_sequence(prefix_len, q)))
             and all(_in_place(t) for t in (q, k, v)))
 
 

@@ -40,6 +40,20 @@ def test_single_queries_of_large_batches(gpu_pkg, B):
     assert (out[start == 5] == 0).all()
 
 
+def test_single_queries_are_checked_as_any_others(gpu_pkg):
+    f = gpu_pkg.scored_attention_flash
+    for Tq in (1, 2):
+        q, k, v = rand(2, 4, Tq, 64), rand(2, 2, 30, 64), rand(2, 2, 30, 64)
+        for args, kw in (((q, rand(3, 2, 30, 64), rand(3, 2, 30, 64)), {}), ((q, k, rand(3, 2, 30, 64)), {}),
+                         ((q, k, v), dict(prefix_len=i32(1, 2, 3))), ((q, k, v), dict(prefix_len=i32(1).long())),
+                         ((q, k, v), dict(prefix_len=torch.tensor([1], dtype=torch.int32)))):
+            announce(f"Tq={Tq} refused {list(kw)}")
+            with pytest.raises(ValueError):
+                f(*args, softcap=20.0, **kw)
+    q, k, v = rand(2, 4, 1, 64), rand(2, 2, 30, 64), rand(2, 2, 30, 64)
+    assert torch.equal(f(q, k, v, softcap=20.0, prefix_len=i32(3, 40)), f(q, k, v, softcap=20.0))
+
+
 def test_keys_far_apart(gpu_pkg):
     """A token stride that a decode call refuses: the view is copied, whether for one query or for two."""
     # 2 tokens 2^31 bytes apart of a buffer that only they touch

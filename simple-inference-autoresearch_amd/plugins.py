@@ -67,7 +67,7 @@ def _padding_free(attention_mask) -> bool:
     The mask builder registered with this function (transformers'
     ``flash_attention_2`` one) already returns ``None`` for a batch without
     padding, once per forward; any mask it does return marks padded keys (or
-    a static cache's unfilled slots), which no kernel here handles.  So the
+    a static cache's unfilled slots), which no kernel here reads.  So the
     decision needs no look at the mask's values: no device-to-host copy per
     layer, and a decode step stays capturable in a HIP graph.  The
     reference's Qwen3.5 plugin calls the backbone without a mask
@@ -77,14 +77,22 @@ def _padding_free(attention_mask) -> bool:
 
 
 def _documents(query: torch.Tensor, key: torch.Tensor, kwargs: dict) -> torch.Tensor | None:
-    """First positions of the documents packed into one row, from the lengths that the caller's collator passes."""
+    """First positions of the documents packed into one row, from the lengths that the caller's collator passes.
+
+    Lengths of as many documents as there are rows are one document a row, whatever is cached in front of it (a decode
+    step's, say): nothing to cut.  Only shapes are looked at; the lengths stay on the device.
+    """
     cuts, of_keys = kwargs.get("cu_seq_lens_q"), kwargs.get("cu_seq_lens_k")
     if cuts is None and of_keys is None:
         return None
-    if query.shape[0] != 1 or query.shape[2] != key.shape[2] or cuts is None or of_keys is None:
-        raise NotImplementedError("packed documents are supported in one row without a cached prefix, with cu_seq_lens_q "
-                                  "and cu_seq_lens_k alike")
-    return cuts if cuts.dtype == torch.int32 else cuts.to(torch.int32)
+    rows, whole = query.shape[0], query.shape[2] == key.shape[2]
+    if cuts is not None and of_keys is not None and cuts.shape == of_keys.shape:
+        if cuts.numel() == rows + 1 and not (rows == 1 and whole):
+            return None
+        if rows == 1 and whole:
+            return cuts if cuts.dtype == torch.int32 else cuts.to(torch.int32)
+    raise NotImplementedError("packed documents are supported in one row without a cached prefix, with cu_seq_lens_q and "
+                              "cu_seq_lens_k alike, or one a row")
 
 
 def sia_attention_forward(module, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, attention_mask,
@@ -97,9 +105,13 @@ def sia_attention_forward(module, query: torch.Tensor, key: torch.Tensor, value:
     GQA is resolved by head index, with no ``repeat_kv`` copy.  ``softcap`` and
     ``sliding_window`` (a key is seen from fewer than that many positions away)
     run the scored kernels, as do the documents of a packed row, passed as
-    ``cu_seq_lens_q`` and ``cu_seq_lens_k`` for a batch of one.  Padding masks
-    and dropout have no kernel here and raise ``NotImplementedError`` rather
-    than being ignored.
+    ``cu_seq_lens_q`` and ``cu_seq_lens_k`` for a batch of one without a cached
+    prefix (equal by the caller's word: their values are not compared, which
+    would wait for the device); lengths of one document a row are taken with
+    any batch and prefix.  Mask tensors (padding) and dropout raise
+    ``NotImplementedError`` rather than being ignored: a batch padded at one
+    end runs through :func:`~.scored.scored_attention_flash`, whose
+    ``kv_start`` and ``kv_len`` say where each row's keys lie.
     """
     if dropout:
         raise NotImplementedError("attention dropout is not supported by the gfx950 kernels")

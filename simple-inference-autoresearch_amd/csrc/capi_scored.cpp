@@ -26,7 +26,8 @@ int per_sequence(const sia_tensor* t, const char* name, int64_t B, const int32_t
 
 int fill_score(const sia_score_options* o, bool prompt, int64_t B, int64_t Hq, float sm_scale, int causal, ScoreArgs& s) {
   memset(&s, 0, sizeof(s));
-  s.window = 1 << 30;
+  // (no window: the largest one; prompts, whose positions lie below 2^30, add it to them in 32 bits)
+  s.window = prompt ? 1 << 30 : 0x7fffffff;
   s.causal = causal != 0;
   if (o == nullptr) return SIA_OK;
   for (int i = 0; i < 4; ++i)

@@ -29,7 +29,7 @@ struct ScoreArgs {
   int64_t cuts_sb;               // elements from one sequence's to the next's (0: shared)
   int32_t ncuts;
   int32_t start_per_seq, len_per_seq, prefix_per_seq;
-  int32_t window;                // W, at most 2^30
+  int32_t window;                // W, of prompts at most 2^30
   int32_t causal;
 };
 

@@ -417,8 +417,8 @@ int sia_rope_qk(const sia_tensor* q, const sia_tensor* k, const sia_tensor* cos,
  * (rotary_dim / 2) f32 or f64, contiguous.  Pair i, elements (i, i +
  * rotary_dim / 2) or, interleaved, (2 i, 2 i + 1), is turned by the angle
  * position x inv_freq[i] and multiplied by scale; elements from rotary_dim on
- * are copied.  Angles are reduced to one turn in 64-bit integers, exact for any
- * position, and their sines and cosines are off by at most 2^-23; products and
+ * are copied.  Angles are reduced to one turn in 64-bit integers (off by |position| 2^-64
+ * turns at most), and their sines and cosines are off by 2^-23 at most; products and
  * sums in fp32, one rounding to the output type.  q_out, k_out: the inputs'
  * shapes and types, head_dim contiguous. */
 int sia_rope_scaled(const sia_tensor* q, const sia_tensor* k, const sia_tensor* positions, const sia_tensor* inv_freq,

@@ -2,10 +2,10 @@
 //
 // Pair i of a token at position n is turned by the angle n f_i (frequency f_i per position) and stretched by a factor.
 // A table of cosines costs its reads and a row per position that a long context reaches, and one built in fp32 is off by
-// n 2^-24 radians, 0.06 at a million.  Here the angle is taken modulo one turn in 64-bit integers: F = frac(f / 2 pi) 2^64
-// (f / 2 pi in fp64), and n F mod 2^64 is the fraction of a turn whatever n is; its top 32 bits give a quadrant and a rest
-// of at most an eighth of a turn, where the Taylor series of sine and cosine to the 9th and 10th power are off by less
-// than 2^-28.  (What remains is F's own error, 2^-52 of the number of turns.)
+// n 2^-24 radians, 0.06 at a million.  Here the angle is taken modulo one turn in 64-bit integers: F = frac(f / 2 pi) 2^64,
+// and n F mod 2^64 is the fraction of a turn whatever n is; its top 32 bits give a quadrant and a rest of at most an eighth of
+// a turn, where the Taylor series of sine and cosine to the 9th and 10th power are off by less than 2^-28.  F is rounded to a
+// whole number, so a turn is off by |n| 2^-64 at most, that is 2^-24 at 2^40 positions.
 //
 // Memory-bound: q and k once in, once out.  A work-group takes a few tokens: it computes each token's R / 2 pairs of sine
 // and cosine once, into LDS, while its first elements are in flight, and every head's items read them there.  An item is
@@ -33,6 +33,20 @@ struct RopeScaledArgs {
   int32_t head_items;                                  // items of a head
   int32_t rot_items;                                   // of them in the rotated part
 };
+
+// f / 2 pi modulo 1 in units of 2^-64, for any finite f: 1 / 2 pi as a sum of two numbers, the product with the first as
+// two (itself and what its rounding left), and whole turns taken out of each part.  (In fp64 alone f / 2 pi is off by
+// 2^-53 of itself, 2^-13 of a radian after 2^40 positions.)
+__device__ __forceinline__ uint64_t turn_per_position(double f) {
+#pragma clang fp contract(off)
+  constexpr double kHi = 0x1.45f306dc9c883p-3, kLo = -0x1.6b01ec5417056p-57;
+  auto fixed = [](double x) {                       // |x| <= 1/2
+    const double y = rint(x * 18446744073709551616.0);
+    return y < 0.0 ? 0u - (uint64_t)-y : (uint64_t)y;
+  };
+  const double p = f * kHi, e = __builtin_fma(f, kLo, __builtin_fma(f, kHi, -p));
+  return fixed(p - rint(p)) + fixed(e - rint(e));
+}
 
 // sine and cosine of `turn` / 2^64 of a turn
 __device__ __forceinline__ float2 sincos_turn(uint64_t turn) {
@@ -180,10 +194,10 @@ __global__ __launch_bounds__(kRopeThreads) void rope_scaled_kernel(const RopeSca
     const int row = row0 + t, b = fdiv(row, a.dT), tt = row - b * a.T;
     const int64_t pi = b * a.p_sb + tt * a.p_st;
     const int64_t n = a.pos64 ? ((const int64_t*)a.pos)[pi] : (int64_t)((const int32_t*)a.pos)[pi];
-    double f = (a.freq64 ? ((const double*)a.freq)[pair] : (double)((const float*)a.freq)[pair]) * 0.15915494309189535;
-    f -= floor(f);                                   // (a negative f next to 0 may round up to 1: a whole turn, 0)
-    float2 y = sincos_turn((uint64_t)n * (f < 1.0 ? (uint64_t)(f * 18446744073709551616.0) : 0u));
-    const float scale = f <= 1.0 ? a.scale : NAN;    // (a frequency that is not finite has no angle)
+    const double f = a.freq64 ? ((const double*)a.freq)[pair] : (double)((const float*)a.freq)[pair];
+    const bool finite = __builtin_isfinite(f);
+    float2 y = sincos_turn((uint64_t)n * turn_per_position(finite ? f : 0.0));
+    const float scale = finite ? a.scale : NAN;      // (a frequency that is not finite has no angle)
     y.x *= scale;
     y.y *= scale;
     sc[i] = y;

@@ -138,10 +138,10 @@ def rope_scaled(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
     ``positions``: int32 or int64 ``(T,)`` or ``(B, T)``; ``inv_freq``: float32
     or float64 ``(rotary_dim / 2,)``, the angle per position of each pair, which
     is ``(i, i + rotary_dim / 2)`` or, ``interleaved``, ``(2i, 2i + 1)``.  The
-    rotated part is multiplied by ``scale``, the rest copied.  Angles are exact
-    modulo a turn whatever the position (no table, no limit).  Strided views
-    are read in place; returns contiguous ``(q_rot, k_rot)``, ``k_rot`` None
-    where ``k`` is.
+    rotated part is multiplied by ``scale``, the rest copied.  There is no table
+    and no last position: an angle is off by ``|position| 2^-64`` of a turn at
+    most (2^-24 at 2^40), its sine and cosine by 2^-23.  Strided views are read
+    in place; returns contiguous ``(q_rot, k_rot)``, ``k_rot`` None where ``k`` is.
     """
     if rotary_dim is None:
         rotary_dim = q.shape[-1]

@@ -65,7 +65,8 @@ struct KeySplit {
 // against 39: the partials and the merge cost more than the chain saves).
 // Two groups per CU are counted at head_dim 64, where the registers hold
 // three: the constants were fitted so.
-// (run: the most keys that a work-group's rows see, where a window leaves fewer than Tk)
+// (run: the most keys that a work-group's rows see, where a window leaves fewer than Tk; documents, whose lengths are on the
+// device, count as all of Tk, so a chunk whose document is short is cut into runs of few blocks or none)
 KeySplit key_splits(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t Tk, int64_t D, bool bf16, int cus,
                     int64_t run = INT64_MAX) {
   KeySplit best;
@@ -301,10 +302,16 @@ int flash_fwd(const sia_tensor* q, const sia_tensor* k, const sia_tensor* v, int
   L.var = D == 128 && groups(B, Hkv, a.G, Tq, (int)D, 0) <= dev.cus ? 1 : 0;
   // Scored calls whose rows see short runs (a window, documents, or few keys) take
   // the 4-wave groups whatever the grid: two share a CU, and one's prologue and
-  // epilogue overlap the other's blocks.  us, 8 waves / 4: 16384 tokens in 24
-  // documents 254 / 245, 2 x 4096 with a window of 512 103.6 / 96.2, 8 x 700 (G =
-  // 3) 30.3 / 25.2, 4 x 2048 capped 186 / 185; but 8192 tokens unmasked 497 / 512,
-  // 4096 in fp16 169 / 178.
+  // epilogue overlap the other's blocks.  us, 8 waves / 4, bf16, 32/8 heads:
+  //   capped: 8 x 1000 115.0 / 107.9, 4 x 1500 108.9 / 106.0, 4 x 2048 184.7 / 180.2,
+  //     3 x 2500 204.5 / 201.0, 2 x 3500 252.8 / 251.2, 2 x 4096 330.8 / 332.3, 1 x
+  //     6000 364.2 / 354.7, 1 x 8192 625.5 / 632.1; masks alone: 4 x 2048 170.1 / 170.2, 2 x 4096 312.8 / 319.1
+  //   windows over 8192: 256 80.3 / 71.7, 1024 162.4 / 156.6, 2048 265.6 / 264.4, 2500
+  //     309.4 / 311.1, 4000 404.3 / 411.7
+  //   16384 in documents: 64 153.0 / 139.9, 24 274.3 / 263.3, 8 393 / 386, 4 595 / 600,
+  //     2 1086 / 1113, 1 2012 / 2094
+  // (fp16: the same signs, each within 3%.  Documents' lengths are on the device:
+  // where they are over 4000 keys the rule costs up to 4%.)
   if (score != nullptr && D == 128 && (sc.cuts != nullptr || std::min<int64_t>(Tk, sc.window) <= 2048)) L.var = 1;
   // Few query rows over many keys: variant 3 or 4, when the caller's workspace
   // also holds the partials (the size of sia_attention_flash_fwd_workspace_size)
